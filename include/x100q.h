@@ -102,6 +102,154 @@ int x100q_lin_gemv_dev_flags(const x100q_lin *lin, const float *x, float *y, int
 #define X100Q_PACK_HP  3
 int x100q_pack_act_dev(int mode, const float *x, int K, int batch, void *out, void *stream);
 
+/* ---- paged KV cache held in 4 bits ----------------------------------------- */
+/* No counterpart in the reference, whose cache is fp32 [kv head][ctx][dim]
+ * (qwen_moe_q3k.c:1868-1880).  Keys and values are kept in 4.5 bits each, in
+ * pages of `page_size` positions that sequences share one pool of, so that a
+ * context of ctx 131072 and 16 sequences of the decode model (206 GB in
+ * fp16) takes 58 GB.
+ *
+ * A value is d * (code - 8): one scale d per 32 values of a head, codes 0..15,
+ * as Q4_0.  d = m / -8 of the block's value m of largest magnitude (the
+ * maximum where the minimum is as large), code = floor(x * (-8 / m) + 8.5) at
+ * most 15; d is then rounded to 8 significand bits (bf16, held in fp16, at
+ * most 8160 in magnitude), so that d * (code - 8) is an fp16 value and the
+ * tensor cores read the cache exactly.  Blocks with max |x| < 2^-100 are
+ * zeros.  A block with a NaN or an infinity is stored as zeros, and the next
+ * synchronising call reports X100_E_ARG.
+ *
+ * Layout: page p holds, for each kv head, page_size / 16 tiles of 16 positions;
+ * a tile (D = head_dim, NB = D / 32) is 18 D bytes:
+ *   0      K codes: position s at s * D / 2; its 32-bit word t * NB + b (t < 4)
+ *          has the codes of dims 32 b + 8 t .. + 7, lowest bits first
+ *   8 D    V codes: the D / 8 dims from g * D / 8 (g < 8) of position
+ *          s = 4 m + t, D / 16 bytes, at ((m / r * 8 + g) * 4 + t) * r + m % r
+ *          times D / 16, r = 2 (D = 128) or 4 (D = 64)
+ *   16 D   K scales, fp16 [s][b];  17 D   V scales, fp16 [b][t][m]
+ *
+ * The pool is the caller's device memory: `pages` (16-byte aligned) of
+ * x100q_kv4_bytes() bytes, which need not be cleared.  page_table
+ * [n_seqs][table_stride] (device) names the page of positions
+ * [i * page_size, (i + 1) * page_size) of a sequence in entry i; entries past a
+ * sequence's length are not read.  Two sequences may name the same page (a
+ * shared prompt) as long as neither appends to it.  A page out of range, a
+ * position or length that the table does not cover, or a sequence index out
+ * of range is never read or written: its positions count as masked (append:
+ * are not stored), and the next synchronising call reports X100_E_ARG.
+ * All calls below are asynchronous on `stream`, allocate nothing, keep no
+ * state and may be captured into a graph.                                   */
+typedef struct {
+    void *pages;
+    int n_pages;
+    int page_size;      /* 16, 32, 64 or 128 positions                       */
+    int n_kv_heads;
+    int head_dim;       /* 64 or 128                                         */
+} x100q_kv4;
+
+/* Bytes of the pool; 0 when the shape is not taken.                         */
+size_t x100q_kv4_bytes(const x100q_kv4 *kv);
+
+/* Append the step's tokens.  Token i goes to position pos[i] of sequence
+ * seq[i] (NULL: sequence i); pos[i] < 0 marks a padding token, which is left
+ * out and whose q_out row stays as it was.  Per head of
+ * q and k: x * norm weight (NULL: none), NEOX rotation by rope[pos] (NULL:
+ * none; element j with j + head_dim / 2, as rope_apply, qwen_moe_q3k.c:1173-1175),
+ * then times 1 / sqrt(mean(x^2) + eps) where there is a norm weight: the
+ * order rmsnorm-then-rope of the model's step up to rounding.  The rotated q goes
+ * to q_out (may be q itself), k and v to the cache.  Codes come from the
+ * value before the factor 1 / rms, which only scales d.
+ * q, k, v, q_out: dtype elements, 16-byte aligned; token i's heads lie side by
+ * side from element i * stride; strides in elements, multiples of 16 bytes.
+ * Several tokens of one sequence may be appended at once, at different
+ * positions; the same position twice is the caller's error.                 */
+typedef struct {
+    int dtype;                    /* X100Q_F32 or X100Q_F16                  */
+    int n_tokens, n_heads;        /* n_heads: query heads (0 without q)      */
+    const void *q, *k, *v;        /* q NULL: only k and v                    */
+    void *q_out;
+    long q_stride, k_stride, v_stride, q_out_stride;
+    const float *q_norm, *k_norm; /* [head_dim] or NULL                      */
+    float eps;
+    const float *rope;            /* [rope_len][head_dim / 2][cos, sin] or NULL */
+    int rope_len;                 /* a position past it is out of range      */
+    const int *pos, *seq;         /* [n_tokens]                              */
+    const int *page_table;
+    int table_stride, n_seqs;
+} x100q_kv4_append_args;
+int x100q_kv4_append_dev(const x100q_kv4 *kv, const x100q_kv4_append_args *a, void *stream);
+
+/* The values that positions stand for: k_out and v_out [n_tokens][n_kv_heads]
+ * [head_dim] fp16 (either may be NULL) of position pos[i] of sequence seq[i]
+ * (NULL: sequence i).  Padding tokens' rows and those out of range stay as
+ * they were.                                                                */
+int x100q_kv4_read_dev(const x100q_kv4 *kv, const int *pos, const int *seq, int n_tokens,
+                       const int *page_table, int table_stride, int n_seqs, void *k_out,
+                       void *v_out, void *stream);
+
+/* The (cos, sin) table of x100q_kv4_append_dev: rope[p][i] of the angle
+ * p * base^(-2i / head_dim) for p < n_pos, i < head_dim / 2, the angle in 64
+ * bits (in 32 the far positions of a long context are off by hundredths of a
+ * radian).                                                                  */
+int x100q_rope_table_dev(float *rope, int n_pos, int head_dim, float base, void *stream);
+
+/* Attention over the cache: out = softmax(scale * q K^T) V per query head,
+ * head h reading kv head h / (n_heads / n_kv_heads).  Sequence b holds kv_len[b]
+ * positions and its tokens are rows q_start[b] .. q_start[b + 1] - 1 of q and out
+ * (NULL: one token each, row b); they are its last positions, and each attends to
+ * all positions up to its own.  A row that sees no position (kv_len[b]
+ * shorter than the sequence's tokens) is zero.  Rows past q_start[n_seqs] stay as
+ * they were.  max_q bounds the tokens of any one sequence, and q_start must
+ * not decrease or pass n_tokens; a sequence that breaks this is left out, and the
+ * next synchronising call reports X100_E_ARG.
+ * X100Q_F32 q is used to 22 bits and all sums are fp32; X100Q_F16 out is
+ * rounded once.  The result does not depend on the order in which blocks run.
+ * work: 16-byte aligned device scratch of x100q_kv4_attn_work() bytes; its
+ * contents need not be kept or cleared, but calls that overlap on the GPU
+ * (other streams, replayed graphs) need one each.                          */
+typedef struct {
+    int dtype;                    /* of q and out: X100Q_F32 or X100Q_F16    */
+    int n_heads;                  /* a multiple of n_kv_heads                */
+    const void *q;
+    void *out;
+    long q_stride, out_stride;    /* elements between tokens, multiples of 16 bytes */
+    const int *q_start;           /* [n_seqs + 1] (device) or NULL           */
+    int n_tokens, max_q;
+    const int *kv_len;            /* [n_seqs] (device)                       */
+    const int *page_table;
+    int table_stride, n_seqs;
+    float scale;                  /* > 0                                     */
+    void *work;
+    size_t work_bytes;
+} x100q_kv4_attn_args;
+size_t x100q_kv4_attn_work(const x100q_kv4 *kv, int n_tokens, int n_heads, int n_seqs);
+int x100q_kv4_attn_dev(const x100q_kv4 *kv, const x100q_kv4_attn_args *a, void *stream);
+
+/* ---- residual RMS norm with 8-bit output ------------------------------------ */
+/* Per row of d elements: h = x + residual (rounded to dtype, stored to
+ * residual_out; no addition where residual is NULL), y = h * w / sqrt(mean(h^2) +
+ * eps), and y in int8 with one fp32 scale per `group` elements (0: per row;
+ * 32, 64 or 128, dividing d): y ~ q * scale.  The rows are the A operand of
+ * gemm_ime_i8_dev_ld, as x100q_pack_act_dev makes the packed records.
+ * With a = max |h w| over the group: q = rint(h w * (127 / a)), scale = a / 127 / rms.
+ * Groups with a < 2^-110 are zeros with scale 0; a group with a NaN or an
+ * infinity has q = 0 and scale NaN.
+ * x, residual, residual_out: dtype elements (X100Q_F32 or X100Q_F16), row pitches in
+ * elements; residual_out may be residual, or x.  q: int8, row pitch ldq
+ * >= d; the pad is left as it was.  scales [rows][d / group] (or [rows]).
+ * Fastest when the pointers are 16-byte aligned and d and the pitches are
+ * multiples of 16.                                                          */
+typedef struct {
+    int dtype, rows, d, group;
+    const void *x, *residual;
+    void *residual_out;
+    long ldx, ldr, ldo, ldq;      /* pitches of x, residual, residual_out, q */
+    const float *w;               /* [d]                                     */
+    float eps;                    /* > 0                                     */
+    int8_t *q;
+    float *scales;
+} x100q_norm_q8_args;
+int x100q_add_rmsnorm_q8_dev(const x100q_norm_q8_args *a, void *stream);
+
 /* ---- mixture-of-experts FFN ---------------------------------------------- */
 typedef struct x100q_moe x100q_moe;
 

@@ -23,6 +23,7 @@ X100_OK, X100_E_ARG, X100_E_NODEV, X100_E_ARCH, X100_E_ALLOC, X100_E_COPY, X100_
     X100_E_TIMEOUT, X100_E_COMM, X100_E_INJECTED, X100_E_UNSUPPORTED, X100_E_TOO_LARGE, X100_E_FORMAT = range(13)
 
 Q_F32, Q4_0, Q8_0, Q3_K, Q4_K = 0, 2, 8, 11, 12
+Q_F16 = 1
 
 
 class X100Error(RuntimeError):
@@ -117,6 +118,14 @@ _SIGS = {
     "x100q_gguf_dequant_dev": ([i32, vp, C.c_long, vp, vp], i32),
     "x100q_quantize_q8_0_dev": ([vp, C.c_long, vp, vp], i32),
     "x100q_pack_act_dev": ([i32, vp, i32, i32, vp, vp], i32),
+    # paged 4-bit KV cache, residual RMS norm with 8-bit output
+    "x100q_kv4_bytes": ([vp], C.c_size_t),
+    "x100q_kv4_append_dev": ([vp, vp, vp], i32),
+    "x100q_kv4_read_dev": ([vp, vp, vp, i32, vp, i32, i32, vp, vp, vp], i32),
+    "x100q_rope_table_dev": ([vp, i32, i32, C.c_float, vp], i32),
+    "x100q_kv4_attn_work": ([vp, i32, i32, i32], C.c_size_t),
+    "x100q_kv4_attn_dev": ([vp, vp, vp], i32),
+    "x100q_add_rmsnorm_q8_dev": ([vp, vp], i32),
 }
 
 
@@ -132,6 +141,32 @@ class ModelCfg(C.Structure):
                                        "n_act", "moe_ffn", "attn_qtype", "expert_qtype", "lm_qtype", "ctx",
                                        "max_batch", "expert_lo", "expert_hi")] + \
                [("rope_base", C.c_float), ("eps", C.c_float)]
+
+
+class Kv4(C.Structure):
+    """x100q_kv4 (include/x100q.h)."""
+    _fields_ = [("pages", vp)] + [(n, i32) for n in ("n_pages", "page_size", "n_kv_heads", "head_dim")]
+
+
+class Kv4AppendArgs(C.Structure):
+    """x100q_kv4_append_args (include/x100q.h)."""
+    _fields_ = [(n, i32) for n in ("dtype", "n_tokens", "n_heads")] + [(n, vp) for n in ("q", "k", "v", "q_out")] + \
+               [(n, i64) for n in ("q_stride", "k_stride", "v_stride", "q_out_stride")] + \
+               [("q_norm", vp), ("k_norm", vp), ("eps", C.c_float), ("rope", vp), ("rope_len", i32), ("pos", vp),
+                ("seq", vp), ("page_table", vp), ("table_stride", i32), ("n_seqs", i32)]
+
+
+class Kv4AttnArgs(C.Structure):
+    """x100q_kv4_attn_args (include/x100q.h)."""
+    _fields_ = [("dtype", i32), ("n_heads", i32), ("q", vp), ("out", vp), ("q_stride", i64), ("out_stride", i64),
+                ("q_start", vp), ("n_tokens", i32), ("max_q", i32), ("kv_len", vp), ("page_table", vp),
+                ("table_stride", i32), ("n_seqs", i32), ("scale", C.c_float), ("work", vp), ("work_bytes", C.c_size_t)]
+
+
+class NormQ8Args(C.Structure):
+    """x100q_norm_q8_args (include/x100q.h)."""
+    _fields_ = [(n, i32) for n in ("dtype", "rows", "d", "group")] + [(n, vp) for n in ("x", "residual", "residual_out")] + \
+               [(n, i64) for n in ("ldx", "ldr", "ldo", "ldq")] + [("w", vp), ("eps", C.c_float), ("q", vp), ("scales", vp)]
 
 
 def lib():
@@ -475,6 +510,154 @@ def pack_act_dev(mode: int, x, K: int, batch: int, out, stream=None) -> None:
 
 def quantize_q8_0_dev(x, n: int, blocks, stream=None) -> None:
     check(lib().x100q_quantize_q8_0_dev(_p(x), n, _p(blocks), _stream(stream)), "x100q_quantize_q8_0_dev")
+
+
+# ---- paged 4-bit KV cache, residual RMS norm with 8-bit output (torch tensors) ---------------
+def _on_device(what: str, dtypes: dict) -> None:
+    """Every tensor of `dtypes` (name -> (tensor or None, dtype)) has its type and lies on the current device."""
+    import torch
+    dev = torch.cuda.current_device()
+    for name, (t, dt) in dtypes.items():
+        if t is not None and (t.dtype is not dt or t.get_device() != dev):
+            raise X100Error(X100_E_ARG, f"{what}: {name} has to be {dt} on the current device (cuda:{dev}), "
+                                        f"not {t.dtype} on {t.device}")
+
+
+def _dtype_id(t, what: str) -> int:
+    import torch
+    if t.dtype is torch.float32:
+        return Q_F32
+    if t.dtype is torch.float16:
+        return Q_F16
+    raise X100Error(X100_E_UNSUPPORTED, f"{what}: float32 or float16 is taken, not {t.dtype}")
+
+
+def _heads(t, name: str, what: str, dim: int):
+    """Token stride of [tokens, heads, dim] with the heads of a token side by side."""
+    if t.dim() != 3 or t.shape[2] != dim or t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != dim):
+        raise X100Error(X100_E_ARG, f"{what}: {name} has to be [tokens, heads, {dim}], a token's heads side by side")
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1] * dim)
+
+
+def _ints(what: str, **named):
+    import torch
+    _on_device(what, {n: (t, torch.int32) for n, t in named.items()})
+    for n, t in named.items():
+        if t is not None and not t.is_contiguous():
+            raise X100Error(X100_E_ARG, f"{what}: {n} has to be contiguous")
+
+
+class Kv4Cache:
+    """A pool of 4-bit KV pages (x100q_kv4): `pages` is a uint8 tensor of the pool's bytes, allocated on
+    the current device unless given.  Page tables are int32 [sequences, entries]; see include/x100q.h for the
+    layout, the masks and what is out of range.  Methods allocate nothing unless an output or the scratch is left out."""
+
+    def __init__(self, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, pages=None):
+        import torch
+        self.kv = Kv4(None, n_pages, page_size, n_kv_heads, head_dim)
+        self._ref = C.byref(self.kv)
+        n = lib().x100q_kv4_bytes(self._ref)
+        if n == 0:
+            raise X100Error(X100_E_ARG, f"Kv4Cache: {n_pages} pages of {page_size} x {n_kv_heads} x {head_dim}")
+        if pages is None:
+            pages = torch.zeros(n, dtype=torch.uint8, device="cuda")
+        if pages.dtype is not torch.uint8 or not pages.is_cuda or not pages.is_contiguous() or pages.numel() < n:
+            raise X100Error(X100_E_ARG, f"Kv4Cache: pages has to be {n} contiguous uint8 on a GPU")
+        self.pages, self.kv.pages = pages, pages.data_ptr()
+        self.head_dim, self.n_kv_heads = head_dim, n_kv_heads
+
+    def append(self, k, v, pos, table, seq=None, q=None, q_out=None, q_norm=None, k_norm=None, eps=1e-6, rope=None, stream=None):
+        """x100q_kv4_append_dev: k, v [tokens, kv heads, dim] into the pages; returns q_out, the normed and rotated q."""
+        import torch
+        what, D = "Kv4Cache.append", self.head_dim
+        dt = _dtype_id(k, what)
+        if q is not None and q_out is None:
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        _on_device(what, {"pages": (self.pages, torch.uint8), "k": (k, k.dtype), "v": (v, k.dtype), "q": (q, k.dtype), "q_out": (q_out, k.dtype),
+                          "q_norm": (q_norm, torch.float32), "k_norm": (k_norm, torch.float32), "rope": (rope, torch.float32)})
+        _ints(what, pos=pos, seq=seq, table=table)
+        n = pos.numel()
+        ks, vs = _heads(k, "k", what, D), _heads(v, "v", what, D)
+        qs = qos = nh = 0
+        if q is not None:
+            qs, qos, nh = _heads(q, "q", what, D), _heads(q_out, "q_out", what, D), q.shape[1]
+        if (k.shape[0] != n or v.shape[0] != n or k.shape[1] != self.n_kv_heads or v.shape[1] != self.n_kv_heads or table.dim() != 2
+                or (seq is not None and seq.numel() != n) or (q is not None and (q.shape[0] != n or q_out.shape != q.shape))
+                or any(w is not None and (w.numel() != D or not w.is_contiguous()) for w in (q_norm, k_norm))
+                or (rope is not None and (rope.numel() % D or not rope.is_contiguous()))):
+            raise X100Error(X100_E_ARG, f"{what}: shapes do not agree")
+        a = Kv4AppendArgs(dt, n, nh, _p(q), k.data_ptr(), v.data_ptr(), _p(q_out), qs, ks, vs, qos, _p(q_norm), _p(k_norm), eps,
+                          _p(rope), rope.numel() // D if rope is not None else 0, pos.data_ptr(), _p(seq), table.data_ptr(),
+                          table.shape[1], table.shape[0])
+        check(lib().x100q_kv4_append_dev(self._ref, C.byref(a), _stream(stream)), "x100q_kv4_append_dev")
+        return q_out
+
+    def read(self, pos, table, seq=None, k_out=None, v_out=None, stream=None):
+        """x100q_kv4_read_dev: the values (k, v) of the positions, fp16 [tokens, kv heads, dim]; both are made when neither is given."""
+        import torch
+        what = "Kv4Cache.read"
+        n = pos.numel()
+        if k_out is None and v_out is None:
+            k_out, v_out = (torch.zeros(n, self.n_kv_heads, self.head_dim, dtype=torch.float16, device=pos.device) for _ in range(2))
+        _on_device(what, {"pages": (self.pages, torch.uint8), "k_out": (k_out, torch.float16), "v_out": (v_out, torch.float16)})
+        _ints(what, pos=pos, seq=seq, table=table)
+        if (table.dim() != 2 or (seq is not None and seq.numel() != n)
+                or any(t is not None and (t.numel() != n * self.n_kv_heads * self.head_dim or not t.is_contiguous()) for t in (k_out, v_out))):
+            raise X100Error(X100_E_ARG, f"{what}: shapes do not agree")
+        check(lib().x100q_kv4_read_dev(self._ref, pos.data_ptr(), _p(seq), n, table.data_ptr(), table.shape[1], table.shape[0],
+                                       _p(k_out), _p(v_out), _stream(stream)), "x100q_kv4_read_dev")
+        return k_out, v_out
+
+    def attend_work(self, n_tokens: int, n_heads: int, n_seqs: int):
+        """Scratch for attend(); calls that overlap on the GPU need one each."""
+        import torch
+        return torch.empty(lib().x100q_kv4_attn_work(self._ref, n_tokens, n_heads, n_seqs), dtype=torch.uint8, device=self.pages.device)
+
+    def attend(self, q, out, table, kv_len, q_start=None, max_q=1, scale=None, work=None, stream=None):
+        """x100q_kv4_attn_dev: q [tokens, heads, dim] over the pages into out (made when None); q_start None: one token per sequence."""
+        import torch
+        what, D = "Kv4Cache.attend", self.head_dim
+        dt = _dtype_id(q, what)
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        if work is None:
+            work = self.attend_work(q.shape[0], q.shape[1], kv_len.numel())
+        _on_device(what, {"pages": (self.pages, torch.uint8), "q": (q, q.dtype), "out": (out, q.dtype), "work": (work, torch.uint8)})
+        _ints(what, q_start=q_start, kv_len=kv_len, table=table)
+        qs, os_, n = _heads(q, "q", what, D), _heads(out, "out", what, D), kv_len.numel()
+        if (out.shape != q.shape or table.dim() != 2 or table.shape[0] != n or (q_start is not None and q_start.numel() != n + 1)
+                or not work.is_contiguous()):
+            raise X100Error(X100_E_ARG, f"{what}: shapes do not agree")
+        a = Kv4AttnArgs(dt, q.shape[1], q.data_ptr(), out.data_ptr(), qs, os_, _p(q_start), q.shape[0], max_q, kv_len.data_ptr(),
+                        table.data_ptr(), table.shape[1], n, D ** -0.5 if scale is None else scale, work.data_ptr(), work.numel())
+        check(lib().x100q_kv4_attn_dev(self._ref, C.byref(a), _stream(stream)), "x100q_kv4_attn_dev")
+        return out
+
+
+def rope_table(n_pos: int, head_dim: int, base: float, stream=None):
+    """x100q_rope_table_dev: (cos, sin) [n_pos, head_dim / 2, 2] for Kv4Cache.append."""
+    import torch
+    t = torch.empty(n_pos, head_dim // 2, 2, dtype=torch.float32, device="cuda")
+    check(lib().x100q_rope_table_dev(t.data_ptr(), n_pos, head_dim, base, _stream(stream)), "x100q_rope_table_dev")
+    return t
+
+
+def add_rmsnorm_q8(x, w, q, scales, residual=None, residual_out=None, eps=1e-6, group=0, stream=None):
+    """x100q_add_rmsnorm_q8_dev: rows of x (+ residual, the sum to residual_out) RMS-normed with w into int8 q and its scales."""
+    import torch
+    what = "add_rmsnorm_q8"
+    dt = _dtype_id(x, what)
+    _on_device(what, {"x": (x, x.dtype), "residual": (residual, x.dtype), "residual_out": (residual_out, x.dtype),
+                      "w": (w, torch.float32), "q": (q, torch.int8), "scales": (scales, torch.float32)})
+    rows, d = x.shape if x.dim() == 2 else (0, 0)
+    if (x.dim() != 2 or w.numel() != d or not w.is_contiguous() or not scales.is_contiguous()
+            or scales.numel() != rows * (d // group if group else 1)
+            or any(t is not None and (t.shape != x.shape or (d > 1 and t.stride(1) != 1)) for t in (x, q, residual, residual_out))):
+        raise X100Error(X100_E_ARG, f"{what}: shapes do not agree, or rows are not contiguous")
+    ld = lambda t: 0 if t is None else t.stride(0) if rows > 1 else d  # noqa: E731
+    a = NormQ8Args(dt, rows, d, group, x.data_ptr(), _p(residual), _p(residual_out), ld(x), ld(residual), ld(residual_out), ld(q),
+                   w.data_ptr(), eps, q.data_ptr(), scales.data_ptr())
+    check(lib().x100q_add_rmsnorm_q8_dev(C.byref(a), _stream(stream)), "x100q_add_rmsnorm_q8_dev")
 
 
 EP_HANDLE_BYTES = 64
