@@ -9,6 +9,7 @@
 // merge_kernel joins them in run order, so results do not depend on timing.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "kv4.cuh"
 #include "ptx.cuh"
@@ -22,7 +23,6 @@ using q::pdl_launch_dependents;
 using q::pdl_wait;
 
 constexpr int kWarps = 8;
-constexpr int kUnit = kWarps * kTile;   // positions per unit: a tile for each warp
 constexpr int kMaxCtas = 320;           // bound of the grid, which sizes the workspace
 
 struct AttnArgs {
@@ -33,6 +33,7 @@ struct AttnArgs {
     long qs, os;
     const int *q_start, *kv_len;
     int n_tokens, max_q, nh, G;
+    int unit_shift;                      // positions per unit, a power of two (128 unless the list would pass 2^31 units)
     float sl;                            // scale * log2(e)
     float *part;                         // [grid][2][8 NR * D] fragment-ordered o, then [grid][2][8 NR][2] m, l
     float *ml;
@@ -44,7 +45,7 @@ struct AttnArgs {
 // tile) item, at least one so that rows without positions are written.
 struct Seq {
     int q0, nq, len, nrt, cu;
-    __device__ long units(int nkv) const { return (long)nkv * nrt * cu; }
+    uint32_t units;                      // of all its items
 };
 __device__ __forceinline__ Seq load_seq(const AttnArgs &a, int b, int R, bool report) {
     Seq s;
@@ -58,31 +59,38 @@ __device__ __forceinline__ Seq load_seq(const AttnArgs &a, int b, int R, bool re
         if (report) atomicCAS(a.status, 0, X100_E_ARG);
         s.len = s.len < 0 ? 0 : min(s.len, cover);
     }
-    s.nrt = (s.nq * a.G + R - 1) / R;
-    s.cu = max(1, (s.len + kUnit - 1) / kUnit);
+    s.nrt = (int)((unsigned)(s.nq * a.G + R - 1) / (unsigned)R);
+    s.cu = max(1, (s.len >> a.unit_shift) + ((s.len & ((1 << a.unit_shift) - 1)) != 0));
+    s.units = (uint32_t)a.pool.nkv * s.nrt * s.cu;
     return s;
 }
-// Units of all sequences, and the sequence holding unit u with the units before
-// it.  Called by one whole warp.
-__device__ __forceinline__ long total_units(const AttnArgs &a, int R, bool report) {
-    long n = 0;
-    for (int b0 = 0; b0 < a.tab.n_seqs; b0 += 32) {
-        const int b = b0 + (threadIdx.x & 31);
-        if (b < a.tab.n_seqs) n += load_seq(a, b, R, report).units(a.pool.nkv);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-    return n;
+// Run i of nc equal runs of U units starts at floor(i U / nc).
+struct Runs {
+    uint32_t U, nc, q, r;
+    __device__ uint32_t start(uint32_t i) const { return i * q + i * r / nc; }   // r < nc <= 320
+};
+// The runs, by one whole warp.
+__device__ __forceinline__ Runs make_runs(const AttnArgs &a, int R, uint32_t grid, bool report) {
+    uint32_t n = 0;
+    for (int b = threadIdx.x & 31; b < a.tab.n_seqs; b += 32) n += load_seq(a, b, R, report).units;
+    Runs w;
+    w.U = __reduce_add_sync(0xffffffffu, n);
+    w.nc = min(grid, w.U);               // no run is empty
+    w.q = w.nc ? w.U / w.nc : 0;
+    w.r = w.nc ? w.U % w.nc : 0;
+    return w;
 }
-__device__ __forceinline__ int find_unit(const AttnArgs &a, int R, long u, long &before) {
-    long base = 0;
+// The sequence holding unit u < U, and the units before it; by one whole warp.
+__device__ __forceinline__ int find_unit(const AttnArgs &a, int R, uint32_t u, uint32_t &before) {
+    uint32_t base = 0;
+    const int lane = threadIdx.x & 31;
     for (int b0 = 0; b0 < a.tab.n_seqs; b0 += 32) {
-        const int lane = threadIdx.x & 31, b = b0 + lane;
-        const long mine = b < a.tab.n_seqs ? load_seq(a, b, R, false).units(a.pool.nkv) : 0;
-        long incl = mine;
+        const int b = b0 + lane;
+        const uint32_t mine = b < a.tab.n_seqs ? load_seq(a, b, R, false).units : 0;
+        uint32_t incl = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long up = __shfl_up_sync(0xffffffffu, incl, o);
+            const uint32_t up = __shfl_up_sync(0xffffffffu, incl, o);
             if (lane >= o) incl += up;
         }
         const uint32_t hit = __ballot_sync(0xffffffffu, base + incl > u);
@@ -99,7 +107,6 @@ __device__ __forceinline__ int find_unit(const AttnArgs &a, int R, long u, long 
 // Row tile of an item index: from both ends in turn, so that a run of neighbouring
 // items of a causal prompt holds early (short) and late (long) ones alike.
 __device__ __forceinline__ int row_tile(int j, int n) { return j & 1 ? n - 1 - (j >> 1) : j >> 1; }
-__device__ __forceinline__ int item_of_row_tile(int rt, int n) { return 2 * rt < n ? 2 * rt : 2 * (n - 1 - rt) + 1; }
 
 // ---- fragments --------------------------------------------------------------------
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -116,15 +123,45 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 }
 __device__ __forceinline__ uint32_t u32(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
 __device__ __forceinline__ __half2 h2(uint32_t u) { return *reinterpret_cast<__half2 *>(&u); }
-// Bits 0-3 (or 4-7) of both halves of w as fp16 code - 8, exactly: the bits under
-// the exponent of 1024 read as 1024 + code (or 1024 + 16 code).
-__device__ __forceinline__ __half2 low_codes(uint32_t w) {
-    return __hsub2(h2((w & 0x000f000fu) | 0x64006400u), __float2half2_rn(1032.f));
+// D = A B + C with C apart (registers or zeros)
+__device__ __forceinline__ void mma_init(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1, float c0, float c1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
 }
-__device__ __forceinline__ __half2 high_codes(uint32_t w) {
-    return __hfma2(h2((w & 0x00f000f0u) | 0x64006400u), __float2half2_rn(0.0625f), __float2half2_rn(-72.f));
+// Codes of both halves of a word as fp16 by placing them under an exponent:
+// bits 0-3 under 1024's read as 1024 + code, bits 4-7 as 1024 + 16 code, and bits
+// 4-7 under 64's as 64 + code.  The exponents come in registers that the
+// compiler cannot see through: with both as immediates each (w & mask) | exponent
+// would be two instructions instead of one.
+struct Exponents {
+    uint32_t e1024, e64;
+    __device__ Exponents() {
+        asm volatile("mov.b32 %0, 0x64006400;" : "=r"(e1024));
+        asm volatile("mov.b32 %0, 0x54005400;" : "=r"(e64));
+    }
+};
+__device__ __forceinline__ uint32_t field(uint32_t w, uint32_t mask, uint32_t expo) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(expo));
+    return r;
 }
-__device__ __forceinline__ float ex2(float x) { return exp2f(x); }
+constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
+// code - 8, exactly
+__device__ __forceinline__ __half2 low_codes(uint32_t w, const Exponents &x) {
+    return __hsub2(h2(field(w, kLow, x.e1024)), __float2half2_rn(1032.f));
+}
+__device__ __forceinline__ __half2 high_codes(uint32_t w, const Exponents &x) {
+    return __hfma2(h2(field(w, kHigh, x.e1024)), __float2half2_rn(0.0625f), __float2half2_rn(-72.f));
+}
+// 2^x: x <= 8 here; results under 2^-126 are zeros
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 // x = hi + lo to 22 bits
 __device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t &lo) {
     const __half2 h = __floats2half2_rn(x, y);
@@ -135,34 +172,41 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t 
 
 template <int D, int NR>
 struct Cfg {
-    static constexpr int ST = 4;                              // ring stages per warp
-    static constexpr int RING = kWarps * ST * Lay<D>::BYTES;
+    static constexpr int ST = 3;                              // ring stages per warp, two tiles each
+    static constexpr int RING = kWarps * ST * 2 * Lay<D>::BYTES;
+    static constexpr int RED = kWarps * 8 * D * 4;            // one 8-row group of every warp, over the idle ring
     static constexpr int QF = NR * (D / 16) * 32 * 16;        // Q fragments: (hi b0, b1, lo b0, b1) per lane
-    static constexpr int RED = kWarps * 8 * D * 4;            // one 8-row group of every warp
+    static constexpr int QB = NR * (D / 32) * 8 * 4;          // -bias sums of every row and block
     static constexpr int ML = kWarps * 8 * NR * 2 * 4;
-    static constexpr int SMEM = RING + QF + RED + ML;
+    static constexpr int SMEM = RING + QF + QB + ML;
+    static_assert(RED <= RING, "");
 };
 
 // S^T = K Q^T and O^T = V^T P^T: positions (then dims) are the M side of
 // m16n8k16, the 8 query rows the N side, so that a group of 8 heads wastes no
-// tensor rows.  The codes become fp16 in registers (K: code - 8, the block's scale
-// applied to the fp32 score sums; V: scale * (code - 8), an exact fp16).
+// tensor rows.  K codes go into the product as 64 + code (fp16 q: every second
+// pair as 1024 + code), one instruction each, and the sum starts from
+// -sum (72 or 1032) q, which each row and block has once: what is left is
+// sum (code - 8) q, which the block's scale multiplies in fp32.  V codes become scale * (code - 8), an exact fp16.
 // Position k of a tile's MMA rows r: r / 2 + 4 (r % 2) of each half, so that
 // transposing the score fragment gives P^T's B fragment for the positions t,
 // t + 4, t + 8, t + 12 that a lane's V codes hold.  HL: q as hi + lo halves.
+// Every warp walks its own positions with its own ring of bulk copies (two tiles a
+// stage), so the loop has no CTA barrier.
 template <typename T, int D, int NR>
 __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(const AttnArgs a) {
     using L = Lay<D>;
     using C = Cfg<D, NR>;
-    constexpr int NB = L::NB, R = 8 * NR, MT = D / 16;
+    constexpr int NB = L::NB, R = 8 * NR, MT = D / 16, TT = NR == 1 ? 2 : 1;   // TT tiles worked on at once
     constexpr bool HL = sizeof(T) == 4;
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t *ring = smem;
+    float4 *red = reinterpret_cast<float4 *>(smem);
     uint4 *qf = reinterpret_cast<uint4 *>(smem + C::RING);
-    float4 *red = reinterpret_cast<float4 *>(smem + C::RING + C::QF);
-    float *sm = reinterpret_cast<float *>(smem + C::RING + C::QF + C::RED), *sl = sm + kWarps * R;
+    float *qb = reinterpret_cast<float *>(smem + C::RING + C::QF);
+    float *sm = reinterpret_cast<float *>(smem + C::RING + C::QF + C::QB), *sl = sm + kWarps * R;
     __shared__ uint64_t bars[kWarps * C::ST];
-    __shared__ long s_u0, s_u1, s_before;
+    __shared__ uint32_t s_u0, s_u1, s_before;
     __shared__ int s_b, abort_flag;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     if (threadIdx.x == 0) abort_flag = 0;
@@ -172,54 +216,79 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
     pdl_launch_dependents();
     pdl_wait();
     if (warp == 0) {
-        const long U = total_units(a, R, blockIdx.x == 0);
-        const long nc = min((long)gridDim.x, U);   // runs: none is empty
-        const long u0 = blockIdx.x < nc ? U * blockIdx.x / nc : 0, u1 = blockIdx.x < nc ? U * (blockIdx.x + 1) / nc : 0;
-        long before = 0;
-        const int b = u0 < u1 ? find_unit(a, R, u0, before) : a.tab.n_seqs;
+        const Runs w = make_runs(a, R, gridDim.x, blockIdx.x == 0);
+        const bool on = blockIdx.x < w.nc;
+        const uint32_t u0 = on ? w.start(blockIdx.x) : 0, u1 = on ? w.start(blockIdx.x + 1) : 0;
+        uint32_t before = 0;
+        const int b = on ? find_unit(a, R, u0, before) : a.tab.n_seqs;
         if (lane == 0) s_u0 = u0, s_u1 = u1, s_before = before, s_b = b;
     }
     __syncthreads();
-    const long u1 = s_u1;
-    long u = s_u0, before = s_before;
+    const uint32_t u1 = s_u1;
+    uint32_t u = s_u0, before = s_before;
     int b = s_b;
     if (u >= u1) return;
+    const Exponents expo;
     Seq sq = load_seq(a, b, R, false);
     int nseg = 0;                              // segments done
-    uint32_t cnt = 0;                          // tiles this warp has consumed
+    uint32_t st = 0, phase = 0;                // this warp's ring: next stage to read, and its parity
     uint64_t *bar = bars + warp * C::ST;
-    uint8_t *wring = ring + warp * C::ST * L::BYTES;
+    uint8_t *wring = ring + warp * C::ST * 2 * L::BYTES;
     while (u < u1) {
-        while (u - before >= sq.units(a.pool.nkv)) {
-            before += sq.units(a.pool.nkv);
+        while (u - before >= sq.units) {
+            before += sq.units;
             sq = load_seq(a, ++b, R, false);
         }
-        const long off = u - before;
-        const long item = off / sq.cu;
-        const int c0 = (int)(off % sq.cu), c1 = (int)min((long)sq.cu, c0 + (u1 - u));
-        const int kvh = (int)(item / sq.nrt), rt = row_tile((int)(item % sq.nrt), sq.nrt);
+        const uint32_t off = u - before, item = off / (uint32_t)sq.cu;
+        const int c0 = (int)(off - item * sq.cu), c1 = (int)min((uint32_t)sq.cu, c0 + (u1 - u));
+        const int kvh = (int)(item / (uint32_t)sq.nrt), rt = row_tile((int)(item - (uint32_t)kvh * sq.nrt), sq.nrt);
         const int rows = min(R, sq.nq * a.G - rt * R);                   // live rows of the tile
         const int first = sq.len - sq.nq;                               // position of token 0
         const int nk = max(0, min(sq.len, first + (rt * R + rows - 1) / a.G + 1));   // positions the last row sees
-        const int t0 = c0 * kWarps, t1 = min(c1 * kWarps, (nk + kTile - 1) / kTile);
-        const int n_mine = t1 > t0 + warp ? (t1 - t0 - warp + kWarps - 1) / kWarps : 0;
-        // ---- start the ring: tile j of this warp is t0 + warp + 8 j ----
-        const uint32_t base = cnt;
-        uint32_t bad = 0;                       // bit s: stage s holds a position without a page
-        auto issue = [&](int j) {
-            const uint8_t *src = tile_of(a.pool, a.tab, b, (t0 + warp + kWarps * j) * kTile, kvh);
-            const int s = (base + j) % C::ST;
-            bad = (bad & ~(1u << s)) | (src ? 0u : 1u << s);
-            if (!src) src = a.pool.pages;       // some page: it is masked
-            if (lane == 0) {
-                if (bad >> s & 1) atomicCAS(a.status, 0, X100_E_ARG);
-                mbar_arrive_expect_tx(&bar[s], L::BYTES);
-                bulk_load(wring + s * L::BYTES, src, L::BYTES, &bar[s]);
-            }
+        const int t0 = c0 << (a.unit_shift - 4), t1 = min(c1 << (a.unit_shift - 4), (nk + kTile - 1) / kTile);
+        // stage j of this warp: `tps` tiles from t0 + tps (warp + 8 j); one each where two would leave warps idle
+        const int tps = t1 - t0 > kWarps ? 2 : 1, ts0 = t0 + tps * warp;
+        const int n_mine = t1 > ts0 ? (t1 - ts0 + tps * kWarps - 1) / (tps * kWarps) : 0;
+        // ---- start the ring (lane 0).  128 or 256 positions between a warp's stages are whole pages, so the place in
+        // the page stays; a page out of range is read as page 0 here and masked below ----
+        const int ps = a.pool.page_shift, tp = ps - 4;       // log2 tiles per page
+        const int *row = a.tab.page + (long)b * a.tab.stride;
+        const int *nxt = row + (ts0 >> tp);                   // table entry of the stage to be issued next
+        const int pstep = (tps * kWarps) >> tp;
+        const bool two = ps == 4 && tps == 2;                 // a stage's tiles lie on two pages
+        const uint8_t *const src0 = a.pool.pages + (long)kvh * a.pool.page_bytes + (ts0 & ((1 << tp) - 1)) * L::BYTES;
+        const long page_step = a.pool.page_bytes * a.pool.nkv;
+        int left = n_mine, id0 = 0, id1 = 0;                  // stages to issue, and the next one's pages
+        auto fetch = [&](int tile) {
+            id0 = __ldg(nxt);
+            if (two && tile + 1 < t1) id1 = __ldg(nxt + 1);
+            nxt += pstep;
         };
-        for (int j = 0; j < min(C::ST, n_mine); ++j) issue(j);
-        // ---- query fragments: rows are the N side ----
-        __syncthreads();                        // the previous segment's readers of qf are done
+        auto issue = [&](uint32_t s, int tile) {              // a stage whose first tile is `tile`
+            uint8_t *dst = wring + s * 2 * L::BYTES;
+            const uint32_t bytes = tps == 2 && tile + 1 < t1 ? 2 * L::BYTES : L::BYTES;
+            mbar_arrive_expect_tx(&bar[s], bytes);
+            const uint8_t *src = src0 + ((unsigned)id0 < (unsigned)a.pool.n_pages ? id0 : 0) * page_step;
+            if (!two) bulk_load(dst, src, bytes, &bar[s]);
+            else {
+                bulk_load(dst, src, L::BYTES, &bar[s]);
+                if (bytes > L::BYTES)
+                    bulk_load(dst + L::BYTES, src0 + ((unsigned)id1 < (unsigned)a.pool.n_pages ? id1 : 0) * page_step, L::BYTES, &bar[s]);
+            }
+            if (--left > 0) fetch(tile + tps * kWarps);
+        };
+        if (lane == 0 && n_mine) {
+            fetch(ts0);
+            uint32_t s = st;
+            for (int j = 0; j < min(C::ST, n_mine); ++j) {
+                issue(s, ts0 + j * tps * kWarps);
+                s = s + 1 == C::ST ? 0 : s + 1;
+            }
+        }
+        // ---- pages out of range, and query fragments: rows are the N side ----
+        bool hole = false;
+        for (int i = (t0 >> tp) + threadIdx.x; i << tp < t1; i += kWarps * 32) hole = hole || (unsigned)__ldg(row + i) >= (unsigned)a.pool.n_pages;
+        if (hole) atomicCAS(a.status, 0, X100_E_ARG);
         for (int e = threadIdx.x; e < NR * NB * 32; e += kWarps * 32) {
             const int nr = e / (NB * 32), blk = e / 32 % NB, ln = e % 32, r = rt * R + nr * 8 + ln / 4;
             float x[8] = {};
@@ -240,175 +309,234 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
                 }
             }
             // half2 number j of a block's K words holds codes j and j + 4
+            float bias = 0.f;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 uint4 f;
                 split2(x[2 * j], x[2 * j + 4], f.x, f.z);
                 split2(x[2 * j + 1], x[2 * j + 5], f.y, f.w);
                 qf[(nr * (D / 16) + 2 * blk + j) * 32 + ln] = f;
+                bias = fmaf(HL ? -72.f : -1032.f, x[2 * j] + x[2 * j + 4], fmaf(-72.f, x[2 * j + 1] + x[2 * j + 5], bias));
             }
+            bias += __shfl_xor_sync(0xffffffffu, bias, 1);    // e runs over whole warps
+            bias += __shfl_xor_sync(0xffffffffu, bias, 2);
+            if ((ln & 3) == 0) qb[(nr * NB + blk) * 8 + ln / 4] = bias;
         }
-        __syncthreads();
-        float m[NR][2], l[NR][2], o[NR][MT][4];
-        int lim[NR][2], minlim = 0x7fffffff;    // positions that rows 2 t, 2 t + 1 of a group see
+        const bool any_hole = __syncthreads_or(hole);
+        float m[NR][2], nm[NR][2], l[NR][2], o[NR][MT][4];   // m in units of log2: score * sl; nm = -m, or 0 at the start
+        int lim[NR][2];                         // positions that rows 2 t, 2 t + 1 of a group see
+        float qi[NR == 1 ? NB : 1][2];          // the lane's qb, in registers where they fit
 #pragma unroll
         for (int nr = 0; nr < NR; ++nr) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                m[nr][i] = -INFINITY, l[nr][i] = 0.f;
+                m[nr][i] = -INFINITY, nm[nr][i] = 0.f, l[nr][i] = 0.f;
                 const int r = nr * 8 + 2 * t + i;
                 lim[nr][i] = r < rows ? min(sq.len, first + (rt * R + r) / a.G + 1) : 0;
             }
 #pragma unroll
             for (int i = 0; i < MT; ++i) o[nr][i][0] = o[nr][i][1] = o[nr][i][2] = o[nr][i][3] = 0.f;
         }
-        minlim = max(0, first + rt * R / a.G + 1);
-        for (int j = 0; j < n_mine; ++j) {
-            const int s = cnt % C::ST, p0 = (t0 + warp + kWarps * j) * kTile;
-            const bool ok = mbar_wait(&bar[s], cnt / C::ST & 1, &abort_flag, a.status);
-            if (!__all_sync(0xffffffffu, ok)) {     // gave up: let the copies in flight land, then leave with the CTA
-                abort_flag = 1;
-                for (int i = j; i < min(j + C::ST, n_mine); ++i)
-                    mbar_wait_drain(&bar[(base + i) % C::ST], (base + i) / C::ST & 1, kWaitLimitNs);
-                break;
-            }
-            const uint8_t *sp = wring + s * L::BYTES;
-            const int k0 = (g >> 1) + 4 * (g & 1);          // this lane's two positions of the tile: k0, k0 + 8
+        if constexpr (NR == 1) {
+#pragma unroll
+            for (int blk = 0; blk < NB; ++blk) qi[blk][0] = qb[blk * 8 + 2 * t], qi[blk][1] = qb[blk * 8 + 2 * t + 1];
+        }
+        const int minlim = max(0, first + rt * R / a.G + 1);
+        const int k0 = (g >> 1) + 4 * (g & 1);              // this lane's two positions of a tile: k0, k0 + 8
+
+        // n <= TT tiles at position p0; EDGE: fewer than TT, masked positions, or missing pages.
+        auto stage = [&](const uint8_t *sp, int p0, int n, auto edge_c) {
+            constexpr bool EDGE = decltype(edge_c)::value;
+            bool gone[TT] = {};
+            if (EDGE && any_hole)
+                for (int tt = 0; tt < n; ++tt) gone[tt] = (unsigned)__ldg(row + ((p0 + tt * kTile) >> ps)) >= (unsigned)a.pool.n_pages;
             // ---- scores ----
-            float sc[NR][4];
+            float sc[TT][NR][4];
 #pragma unroll
-            for (int nr = 0; nr < NR; ++nr) sc[nr][0] = sc[nr][1] = sc[nr][2] = sc[nr][3] = 0.f;
-            uint32_t kw[2][NB];
-            __half kd[2][NB];
+            for (int tt = 0; tt < TT; ++tt) {
+                if (EDGE && tt >= n) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const uint8_t *kp = sp + L::k_word(k0 + 8 * i, 0, t), *dp = sp + L::k_scale(k0 + 8 * i, 0);
-                if constexpr (NB == 4) {
-                    *reinterpret_cast<uint4 *>(kw[i]) = *reinterpret_cast<const uint4 *>(kp);
-                    *reinterpret_cast<uint2 *>(kd[i]) = *reinterpret_cast<const uint2 *>(dp);
-                } else {
-                    *reinterpret_cast<uint2 *>(kw[i]) = *reinterpret_cast<const uint2 *>(kp);
-                    *reinterpret_cast<uint32_t *>(kd[i]) = *reinterpret_cast<const uint32_t *>(dp);
+                    for (int nr = 0; nr < NR; ++nr) sc[tt][nr][0] = sc[tt][nr][1] = sc[tt][nr][2] = sc[tt][nr][3] = -INFINITY;
+                    continue;
                 }
-            }
-#pragma unroll
-            for (int blk = 0; blk < NB; ++blk) {
-                uint32_t f[2][4];
+                uint32_t kw[2][NB];
+                __half kd[2][NB];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const uint32_t w = kw[i][blk], w8 = w >> 8;
-                    f[i][0] = u32(low_codes(w)), f[i][1] = u32(high_codes(w));
-                    f[i][2] = u32(low_codes(w8)), f[i][3] = u32(high_codes(w8));
-                }
-                const float d0 = __half2float(kd[0][blk]), d1 = __half2float(kd[1][blk]);
-#pragma unroll
-                for (int nr = 0; nr < NR; ++nr) {
-                    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const uint4 q = qf[(nr * (D / 16) + 2 * blk + h) * 32 + lane];
-                        mma(acc, f[0][2 * h], f[1][2 * h], f[0][2 * h + 1], f[1][2 * h + 1], q.x, q.y);
-                        if (HL) mma(acc, f[0][2 * h], f[1][2 * h], f[0][2 * h + 1], f[1][2 * h + 1], q.z, q.w);
+                    const uint8_t *kp = sp + tt * L::BYTES + L::k_word(k0 + 8 * i, 0, t), *dp = sp + tt * L::BYTES + L::k_scale(k0 + 8 * i, 0);
+                    if constexpr (NB == 4) {
+                        *reinterpret_cast<uint4 *>(kw[i]) = *reinterpret_cast<const uint4 *>(kp);
+                        *reinterpret_cast<uint2 *>(kd[i]) = *reinterpret_cast<const uint2 *>(dp);
+                    } else {
+                        *reinterpret_cast<uint2 *>(kw[i]) = *reinterpret_cast<const uint2 *>(kp);
+                        *reinterpret_cast<uint32_t *>(kd[i]) = *reinterpret_cast<const uint32_t *>(dp);
                     }
-                    sc[nr][0] = fmaf(acc[0], d0, sc[nr][0]);
-                    sc[nr][1] = fmaf(acc[1], d0, sc[nr][1]);
-                    sc[nr][2] = fmaf(acc[2], d1, sc[nr][2]);
-                    sc[nr][3] = fmaf(acc[3], d1, sc[nr][3]);
+                }
+#pragma unroll
+                for (int blk = 0; blk < NB; ++blk) {
+                    uint32_t f[2][4];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t w = kw[i][blk];
+                        if constexpr (HL) {
+                            f[i][0] = field(w << 4, kHigh, expo.e64), f[i][1] = field(w, kHigh, expo.e64);
+                            f[i][2] = field(w >> 4, kHigh, expo.e64), f[i][3] = field(w >> 8, kHigh, expo.e64);
+                        } else {
+                            f[i][0] = field(w, kLow, expo.e1024), f[i][1] = field(w, kHigh, expo.e64);
+                            f[i][2] = field(w >> 8, kLow, expo.e1024), f[i][3] = field(w >> 8, kHigh, expo.e64);
+                        }
+                    }
+                    const float d0 = __half2float(kd[0][blk]), d1 = __half2float(kd[1][blk]);
+#pragma unroll
+                    for (int nr = 0; nr < NR; ++nr) {
+                        float acc[4], i0, i1;
+                        if constexpr (NR == 1) i0 = qi[blk][0], i1 = qi[blk][1];
+                        else {
+                            const float2 v = *reinterpret_cast<const float2 *>(qb + (nr * NB + blk) * 8 + 2 * t);
+                            i0 = v.x, i1 = v.y;
+                        }
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint4 *qp = qf + (nr * (D / 16) + 2 * blk + h) * 32 + lane;
+                            uint4 q;
+                            if constexpr (HL) q = *qp;
+                            else *reinterpret_cast<uint2 *>(&q) = *reinterpret_cast<const uint2 *>(qp);
+                            if (h == 0) mma_init(acc, f[0][0], f[1][0], f[0][1], f[1][1], q.x, q.y, i0, i1);
+                            else mma(acc, f[0][2], f[1][2], f[0][3], f[1][3], q.x, q.y);
+                            if (HL) mma(acc, f[0][2 * h], f[1][2 * h], f[0][2 * h + 1], f[1][2 * h + 1], q.z, q.w);
+                        }
+                        float(&x)[4] = sc[tt][nr];
+                        if (blk == 0) x[0] = acc[0] * d0, x[1] = acc[1] * d0, x[2] = acc[2] * d1, x[3] = acc[3] * d1;
+                        else {
+                            x[0] = fmaf(acc[0], d0, x[0]), x[1] = fmaf(acc[1], d0, x[1]);
+                            x[2] = fmaf(acc[2], d1, x[2]), x[3] = fmaf(acc[3], d1, x[3]);
+                        }
+                    }
                 }
             }
             // ---- mask, running max ----
-            const bool missing = bad >> s & 1;
-            const bool edge = missing || p0 + kTile > minlim;
-            bool grow = false;
+            if (EDGE) {
 #pragma unroll
-            for (int nr = 0; nr < NR; ++nr) {
-                if (edge) {
+                for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (missing || p0 + k0 + 8 * (i >> 1) >= lim[nr][i & 1]) sc[nr][i] = -INFINITY;
-                }
-                // the running max follows only when a score passes it by 2^8: until then
-                // exp2 of the difference stays within fp16 and the sums need no rescaling
+                    for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) grow = grow || (sc[nr][i] - m[nr][i & 1]) * a.sl > 8.f;
+                        for (int i = 0; i < 4; ++i)
+                            if (gone[tt] || p0 + tt * kTile + k0 + 8 * (i >> 1) >= lim[nr][i & 1]) sc[tt][nr][i] = -INFINITY;
             }
+            // The running max follows only when a score passes it by 2^8: until then exp2 of the
+            // difference stays within fp16 and the sums need no rescaling.
+            bool grow = false;
+            float top[NR][2];
+#pragma unroll
+            for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    top[nr][i] = fmaxf(sc[0][nr][i], sc[0][nr][i + 2]);
+                    if constexpr (TT == 2) top[nr][i] = fmaxf(top[nr][i], fmaxf(sc[1][nr][i], sc[1][nr][i + 2]));
+                    grow = grow || top[nr][i] * a.sl > m[nr][i] + 8.f;
+                }
             if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
                 for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        float x = fmaxf(sc[nr][i], sc[nr][i + 2]);
+                        float x = top[nr][i];
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                        const float mn = fmaxf(m[nr][i], x);
-                        const float f = mn == -INFINITY ? 1.f : ex2((m[nr][i] - mn) * a.sl);
+                        const float mn = fmaxf(m[nr][i], x * a.sl);
+                        const float f = mn == -INFINITY ? 1.f : ex2(m[nr][i] - mn);
                         m[nr][i] = mn;
+                        nm[nr][i] = mn == -INFINITY ? 0.f : -mn;
                         l[nr][i] *= f;
 #pragma unroll
                         for (int k = 0; k < MT; ++k) o[nr][k][i] *= f, o[nr][k][i + 2] *= f;
                     }
             }
-            uint32_t ph[NR][2], pl[NR][2];
 #pragma unroll
-            for (int nr = 0; nr < NR; ++nr) {
-                float p[4];
+            for (int tt = 0; tt < TT; ++tt) {
+                if (EDGE && tt >= n) break;
+                uint32_t ph[NR][2], pl[NR][2];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float mm = m[nr][i & 1];
-                    p[i] = ex2((sc[nr][i] - (mm == -INFINITY ? 0.f : mm)) * a.sl);
+                for (int nr = 0; nr < NR; ++nr) {
+                    float p[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) p[i] = ex2(fmaf(sc[tt][nr][i], a.sl, nm[nr][i & 1]));
+                    l[nr][0] += p[0] + p[2];
+                    l[nr][1] += p[1] + p[3];
+                    split2(p[0], p[1], ph[nr][0], pl[nr][0]);
+                    split2(p[2], p[3], ph[nr][1], pl[nr][1]);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) ph[nr][i] = transpose8(ph[nr][i]), pl[nr][i] = transpose8(pl[nr][i]);
                 }
-                l[nr][0] += p[0] + p[2];
-                l[nr][1] += p[1] + p[3];
-                split2(p[0], p[1], ph[nr][0], pl[nr][0]);
-                split2(p[2], p[3], ph[nr][1], pl[nr][1]);
+                // ---- O += P V: this lane's positions t + 4 m, dims g * D / 8 .. ----
+                const uint8_t *vp = sp + tt * L::BYTES;
+                __half vd[4];
+                *reinterpret_cast<uint2 *>(vd) = *reinterpret_cast<const uint2 *>(vp + L::v_scale(t, g * (D / 8) / 32));
+                if (EDGE) {
+                    // codes past the sequence's end are any bytes, their scales maybe NaN: 0 * NaN must not reach the sums
 #pragma unroll
-                for (int i = 0; i < 2; ++i) ph[nr][i] = transpose8(ph[nr][i]), pl[nr][i] = transpose8(pl[nr][i]);
-            }
-            // ---- O += P V: this lane's positions t + 4 m, dims g * D / 8 .. ----
-            __half vd[4];
-            *reinterpret_cast<uint2 *>(vd) = *reinterpret_cast<const uint2 *>(sp + L::v_scale(t, g * (D / 8) / 32));
-            if (p0 + kTile > sq.len || missing) {
-                // codes past the sequence's end are any bytes, their scales maybe NaN: 0 * NaN must not reach the sums
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (missing || p0 + t + 4 * i >= sq.len) vd[i] = __ushort_as_half(0);
-            }
-            constexpr int W = D / 64;             // words per V piece
-            uint32_t vw[4][W];
-            {
-                const uint4 x = *reinterpret_cast<const uint4 *>(sp + L::V0 + lane * 16);
-                if constexpr (W == 2) {
-                    const uint4 y = *reinterpret_cast<const uint4 *>(sp + L::V0 + 512 + lane * 16);
-                    vw[0][0] = x.x, vw[0][1] = x.y, vw[1][0] = x.z, vw[1][1] = x.w;
-                    vw[2][0] = y.x, vw[2][1] = y.y, vw[3][0] = y.z, vw[3][1] = y.w;
-                } else {
-                    vw[0][0] = x.x, vw[1][0] = x.y, vw[2][0] = x.z, vw[3][0] = x.w;
+                    for (int i = 0; i < 4; ++i)
+                        if (gone[tt] || p0 + tt * kTile + t + 4 * i >= sq.len) vd[i] = __ushort_as_half(0);
                 }
-            }
-            const __half2 da = __halves2half2(vd[0], vd[1]), db = __halves2half2(vd[2], vd[3]);
-#pragma unroll
-            for (int w = 0; w < W; ++w)
-#pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    // 16-bit halves of two positions side by side: 4 dims x 2 positions
-                    const uint32_t x = __byte_perm(vw[0][w], vw[1][w], hf ? 0x7632 : 0x5410);
-                    const uint32_t y = __byte_perm(vw[2][w], vw[3][w], hf ? 0x7632 : 0x5410);
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {   // dims 8 w + 4 hf + 2 e, + 1
-                        const uint32_t xe = x >> (8 * e), ye = y >> (8 * e);
-                        const uint32_t a0 = u32(__hmul2(low_codes(xe), da)), a1 = u32(__hmul2(high_codes(xe), da));
-                        const uint32_t a2 = u32(__hmul2(low_codes(ye), db)), a3 = u32(__hmul2(high_codes(ye), db));
-#pragma unroll
-                        for (int nr = 0; nr < NR; ++nr) {
-                            mma(o[nr][4 * w + 2 * hf + e], a0, a1, a2, a3, ph[nr][0], ph[nr][1]);
-                            mma(o[nr][4 * w + 2 * hf + e], a0, a1, a2, a3, pl[nr][0], pl[nr][1]);
-                        }
+                constexpr int W = D / 64;             // words per V piece
+                uint32_t vw[4][W];
+                {
+                    const uint4 x = *reinterpret_cast<const uint4 *>(vp + L::V0 + lane * 16);
+                    if constexpr (W == 2) {
+                        const uint4 y = *reinterpret_cast<const uint4 *>(vp + L::V0 + 512 + lane * 16);
+                        vw[0][0] = x.x, vw[0][1] = x.y, vw[1][0] = x.z, vw[1][1] = x.w;
+                        vw[2][0] = y.x, vw[2][1] = y.y, vw[3][0] = y.z, vw[3][1] = y.w;
+                    } else {
+                        vw[0][0] = x.x, vw[1][0] = x.y, vw[2][0] = x.z, vw[3][0] = x.w;
                     }
                 }
+                const __half2 da = __halves2half2(vd[0], vd[1]), db = __halves2half2(vd[2], vd[3]);
+#pragma unroll
+                for (int w = 0; w < W; ++w)
+#pragma unroll
+                    for (int hf = 0; hf < 2; ++hf) {
+                        // 16-bit halves of two positions side by side: 4 dims x 2 positions
+                        const uint32_t x = __byte_perm(vw[0][w], vw[1][w], hf ? 0x7632 : 0x5410);
+                        const uint32_t y = __byte_perm(vw[2][w], vw[3][w], hf ? 0x7632 : 0x5410);
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {   // dims 8 w + 4 hf + 2 e, + 1
+                            const uint32_t xe = x >> (8 * e), ye = y >> (8 * e);
+                            const uint32_t a0 = u32(__hmul2(low_codes(xe, expo), da)), a1 = u32(__hmul2(high_codes(xe, expo), da));
+                            const uint32_t a2 = u32(__hmul2(low_codes(ye, expo), db)), a3 = u32(__hmul2(high_codes(ye, expo), db));
+#pragma unroll
+                            for (int nr = 0; nr < NR; ++nr) {
+                                mma(o[nr][4 * w + 2 * hf + e], a0, a1, a2, a3, ph[nr][0], ph[nr][1]);
+                                mma(o[nr][4 * w + 2 * hf + e], a0, a1, a2, a3, pl[nr][0], pl[nr][1]);
+                            }
+                        }
+                    }
+            }
+        };
+        for (int j = 0, tile = ts0; j < n_mine; ++j, tile += tps * kWarps) {
+            const bool ok = mbar_wait(&bar[st], phase, &abort_flag, a.status);
+            if (!__all_sync(0xffffffffu, ok)) {     // gave up: let the copies in flight land, then leave with the CTA
+                abort_flag = 1;
+                for (int i = j; i < min(j + C::ST, n_mine); ++i) {
+                    mbar_wait_drain(&bar[st], phase, kWaitLimitNs);
+                    st = st + 1 == C::ST ? (phase ^= 1, 0) : st + 1;
+                }
+                break;
+            }
+            const uint8_t *sp = wring + st * 2 * L::BYTES;
+            const int p0 = tile * kTile, n = min(tps, t1 - tile);
+            if constexpr (TT == 2) {
+                if (n == 2 && p0 + 2 * kTile <= minlim && !any_hole) stage(sp, p0, 2, std::false_type{});
+                else stage(sp, p0, n, std::true_type{});
+            } else {
+                for (int tt = 0; tt < n; ++tt)
+                    if (p0 + (tt + 1) * kTile <= minlim && !any_hole) stage(sp + tt * L::BYTES, p0 + tt * kTile, 1, std::false_type{});
+                    else stage(sp + tt * L::BYTES, p0 + tt * kTile, 1, std::true_type{});
+            }
             __syncwarp();                          // the stage is read: refill it
-            if (j + C::ST < n_mine) issue(j + C::ST);
-            ++cnt;
+            if (lane == 0 && left > 0) issue(st, tile + C::ST * tps * kWarps);
+            st = st + 1 == C::ST ? (phase ^= 1, 0) : st + 1;
         }
         // ---- join the warps ----
 #pragma unroll
@@ -434,7 +562,7 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
                 M[i] = -INFINITY;
 #pragma unroll
                 for (int w = 0; w < kWarps; ++w) M[i] = fmaxf(M[i], sm[w * R + nr * 8 + 2 * t + i]);
-                f[i] = M[i] == -INFINITY ? 0.f : ex2((m[nr][i] - M[i]) * a.sl);
+                f[i] = M[i] == -INFINITY ? 0.f : ex2(m[nr][i] - M[i]);
             }
 #pragma unroll
             for (int k = 0; k < MT; ++k)
@@ -456,7 +584,7 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
 #pragma unroll
                     for (int w = 0; w < kWarps; ++w) {
                         const int e = w * R + nr * 8 + 2 * t + i;
-                        if (M[i] != -INFINITY) Ls[i] += sl[e] * ex2((sm[e] - M[i]) * a.sl);
+                        if (M[i] != -INFINITY) Ls[i] += sl[e] * ex2(sm[e] - M[i]);
                     }
                 }
                 if (whole) {
@@ -484,6 +612,7 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
                         }
                 }
             }
+            if (nr == NR - 1) fence_proxy_async_smem();   // the next copies into the ring come after these accesses
             __syncthreads();
         }
         u += c1 - c0;
@@ -491,60 +620,80 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
     }
 }
 
-// One warp per (item, 8-row group, 16-dim fragment): joins the partials of an item
-// that several runs share, in run order.  Items that lie in one run are done.
+// One CTA per (cut between two runs, 8-row group, 16-dim fragment).  The first cut
+// inside an item joins the partials of all runs that share the item, each warp
+// every 8th run, in a fixed order.
 template <typename T, int D, int NR>
-__global__ void __launch_bounds__(32) merge_kernel(const AttnArgs a, int grid, int nrt_max) {
+__global__ void __launch_bounds__(kWarps * 32) merge_kernel(const AttnArgs a, uint32_t grid) {
     constexpr int R = 8 * NR, MT = D / 16;
-    const int lane = threadIdx.x, g = lane >> 2, t = lane & 3;
-    const int b = blockIdx.x / (a.pool.nkv * nrt_max), kvh = blockIdx.x / nrt_max % a.pool.nkv, rt = blockIdx.x % nrt_max;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int nr = blockIdx.y / MT, k = blockIdx.y % MT;
+    __shared__ float2 s_ml[kMaxCtas][8];
+    __shared__ float4 s_o[kWarps][32];
+    __shared__ float s_l[kWarps][8];
     pdl_launch_dependents();
     pdl_wait();
+    const Runs w = make_runs(a, R, grid, false);
+    const uint32_t c = blockIdx.x + 1;                       // the cut before run c
+    if (c >= w.nc) return;
+    const uint32_t u = w.start(c);
+    uint32_t before;
+    const int b = find_unit(a, R, u, before);
     const Seq sq = load_seq(a, b, R, false);
-    if (rt >= sq.nrt) return;
+    const uint32_t item = (u - before) / (uint32_t)sq.cu, ua = before + item * sq.cu, ub = ua + sq.cu;
+    if (u == ua || w.start(c - 1) > ua) return;              // a whole item on each side, or not the item's first cut
+    const int kvh = (int)(item / (uint32_t)sq.nrt), rt = row_tile((int)(item - (uint32_t)kvh * sq.nrt), sq.nrt);
     const int rows = min(R, sq.nq * a.G - rt * R);
     if (nr * 8 >= rows) return;
-    long U = 0, before = 0;
-    for (int b0 = 0; b0 < a.tab.n_seqs; b0 += 32) {
-        const int bb = b0 + lane;
-        const long n = bb < a.tab.n_seqs ? load_seq(a, bb, R, false).units(a.pool.nkv) : 0;
-        U += n;
-        before += bb < b ? n : 0;
+    const uint32_t last = (uint32_t)(((uint64_t)ub * w.nc - 1) / w.U);   // the run holding the item's last unit
+    const int np = (int)(last - c) + 2;                      // runs c - 1 .. last
+    const int slot0 = 2 * (int)(c - 1) + (w.start(c - 1) != ua ? 1 : 0);
+    for (int e = threadIdx.x; e < np * 8; e += kWarps * 32) {
+        const int slot = e < 8 ? slot0 : 2 * (int)(c - 1 + e / 8);
+        s_ml[e / 8][e % 8] = __ldcg(reinterpret_cast<const float2 *>(a.ml) + (long)slot * R + nr * 8 + e % 8);
     }
+    __syncthreads();
+    float M[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    for (int p = g; p < np; p += 8)
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        U += __shfl_xor_sync(0xffffffffu, U, o);
-        before += __shfl_xor_sync(0xffffffffu, before, o);
-    }
-    const long ua = before + ((long)kvh * sq.nrt + item_of_row_tile(rt, sq.nrt)) * sq.cu, ub = ua + sq.cu;
-    const long nc = min((long)grid, U);
-    const int c_first = (int)(((ua + 1) * nc - 1) / U), c_last = (int)((ub * nc - 1) / U);
-    if (c_first == c_last) return;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+        for (int i = 0; i < 2; ++i) M[i] = fmaxf(M[i], s_ml[p][2 * t + i].x);
+#pragma unroll
+    for (int sh = 4; sh < 32; sh <<= 1)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) M[i] = fmaxf(M[i], __shfl_xor_sync(0xffffffffu, M[i], sh));
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int c = c_first; c <= c_last; ++c) {
-        const int slot = 2 * c + (c == c_first && U * c / nc != ua ? 1 : 0);
+#pragma unroll 4
+    for (int p = warp; p < np; p += kWarps) {
+        const int slot = p == 0 ? slot0 : 2 * (int)(c - 1 + p);
         const float4 y = __ldcg(reinterpret_cast<const float4 *>(a.part) + ((long)slot * NR + nr) * MT * 32 + k * 32 + lane);
-        float f[2], h[2];
+        float f[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const float2 p = __ldcg(reinterpret_cast<const float2 *>(a.ml) + (long)slot * R + nr * 8 + 2 * t + i);
-            const float mn = fmaxf(m[i], p.x);
-            f[i] = mn == -INFINITY ? 0.f : ex2((m[i] - mn) * a.sl);
-            h[i] = mn == -INFINITY ? 0.f : ex2((p.x - mn) * a.sl);
-            m[i] = mn;
-            l[i] = l[i] * f[i] + p.y * h[i];
+            const float2 ml = s_ml[p][2 * t + i];
+            f[i] = M[i] == -INFINITY ? 0.f : ex2(ml.x - M[i]);
+            l[i] = fmaf(ml.y, f[i], l[i]);
         }
-        x.x = x.x * f[0] + y.x * h[0], x.y = x.y * f[1] + y.y * h[1];
-        x.z = x.z * f[0] + y.z * h[0], x.w = x.w * f[1] + y.w * h[1];
+        x.x = fmaf(y.x, f[0], x.x), x.y = fmaf(y.y, f[1], x.y);
+        x.z = fmaf(y.z, f[0], x.z), x.w = fmaf(y.w, f[1], x.w);
+    }
+    s_o[warp][lane] = x;
+    if (g == 0) s_l[warp][2 * t] = l[0], s_l[warp][2 * t + 1] = l[1];
+    __syncthreads();
+    if (warp) return;
+#pragma unroll
+    for (int i = 1; i < kWarps; ++i) {
+        const float4 y = s_o[i][lane];
+        x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int rr = nr * 8 + 2 * t + i;
         if (rr >= rows) continue;
+        float ls = 0.f;
+#pragma unroll
+        for (int j = 0; j < kWarps; ++j) ls += s_l[j][2 * t + i];
         const int r = rt * R + rr;
-        const float inv = l[i] > 0.f ? 1.f / l[i] : 0.f;
+        const float inv = ls > 0.f ? 1.f / ls : 0.f;
         const float y0 = (i ? x.y : x.x) * inv, y1 = (i ? x.w : x.z) * inv;
         T *p = static_cast<T *>(a.out) + (long)(sq.q0 + r / a.G) * a.os + (long)(kvh * a.G + r % a.G) * D + g * (D / 8) + 2 * k;
         if constexpr (sizeof(T) == 4) *reinterpret_cast<float2 *>(p) = make_float2(y0, y1);
@@ -560,14 +709,16 @@ static int launch(DevCtx *c, AttnArgs &a, cudaStream_t s) {
         set_qkernel_attrs(attn_kernel<T, D, NR>, Cfg<D, NR>::SMEM);
         attr[c->device] = true;
     }
-    const long nrt = ((long)a.max_q * a.G + R - 1) / R, cover = (long)a.tab.stride << a.pool.page_shift;
-    const long most = std::min<long>((long)a.tab.n_seqs * a.pool.nkv * nrt, kMaxCtas) * std::max<long>(1, (cover + kUnit - 1) / kUnit);
+    const long nrt = ((long)a.max_q * a.G + R - 1) / R, cover = std::min(0x7fffffffl, (long)a.tab.stride << a.pool.page_shift);
+    const long items = (long)a.tab.n_seqs * a.pool.nkv * nrt;
+    a.unit_shift = 7;
+    while (items * ((cover >> a.unit_shift) + 1) > 0x7fffffffl) ++a.unit_shift;   // items <= 2^24: ends by 25
+    const long most = std::min<long>(items, kMaxCtas) * ((cover >> a.unit_shift) + 1);
     const int grid = (int)std::min<long>(std::min(kMaxCtas, c->sm_count * (NR == 1 ? 2 : 1)), most);
     a.ml = a.part + (size_t)kMaxCtas * 2 * R * D;
     int st = launch_pdl(attn_kernel<T, D, NR>, dim3(grid), dim3(kWarps * 32), Cfg<D, NR>::SMEM, s, a);
-    if (st) return st;
-    const long items = (long)a.tab.n_seqs * a.pool.nkv * nrt;
-    return launch_pdl(merge_kernel<T, D, NR>, dim3((unsigned)items, NR * (D / 16)), dim3(32), 0, s, a, grid, (int)nrt);
+    if (st || grid == 1) return st;
+    return launch_pdl(merge_kernel<T, D, NR>, dim3(grid - 1, NR * (D / 16)), dim3(kWarps * 32), 0, s, a, (uint32_t)grid);
 }
 
 template <typename T, int D>
@@ -623,7 +774,7 @@ int x100q_kv4_attn_dev(const x100q_kv4 *kv, const x100q_kv4_attn_args *a, void *
     p.part = static_cast<float *>(a->work);
     p.status = c->d_status;
     const long items = (long)a->n_seqs * kv->n_kv_heads * (((long)p.max_q * p.G + 7) / 8);
-    if (items > 0x7fffffffl || (long)p.max_q * p.G > (1l << 30)) return refuse(X100_E_TOO_LARGE);
+    if (items > (1l << 24) || (long)p.max_q * p.G > (1l << 30)) return refuse(X100_E_TOO_LARGE);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (a->dtype == X100Q_F32)
         return kv->head_dim == 128 ? launch_rows<float, 128>(c, p, s) : launch_rows<float, 64>(c, p, s);
