@@ -3,7 +3,7 @@
 // A sequence's query rows of one kv head are its tokens x the group's heads,
 // row r = (token r / G, head r % G), in row tiles of 8 NR.  The work list is every
 // (sequence, kv head, row tile) cut into units of 128 positions; CTA i of
-// the grid takes the i-th equal run of units, so ragged lengths and a single long
+// the grid takes the i-th run of equally many units, so ragged lengths and a single long
 // sequence both fill the card, whatever the lengths (which only the device
 // knows).  Row tiles that a run cuts leave partial (o, m, l) sums in `work`;
 // merge_kernel joins them in run order, so results do not depend on timing.
@@ -33,12 +33,21 @@ struct AttnArgs {
     long qs, os;
     const int *q_start, *kv_len;
     int n_tokens, max_q, nh, G;
+    uint32_t g_mul;                      // ceil(2^32 / G): n / G = umulhi(n, g_mul) for n < 2^32 / G
     int unit_shift;                      // positions per unit, a power of two (128 unless the list would pass 2^31 units)
     float sl;                            // scale * log2(e)
-    float *part;                         // [grid][2][8 NR * D] fragment-ordered o, then [grid][2][8 NR][2] m, l
-    float *ml;
+    // work: of the first (slot 0) and last (slot 1) item that a run has a part of only
+    float *part;                         // [kMaxCtas][2][8 NR * D] o in fragment order
+    float2 *ml;                          // [kMaxCtas][2][8 NR] running max (log2 units) and sum
+    int4 *meta;                          // [kMaxCtas][2] the item: first unit, sequence, kv head, row tile | kInside; or -1
     int *status;
 };
+
+constexpr int kInside = 1 << 30;         // the run starts inside the item
+
+// Row number over the group's heads: rows of a sequence are at most 2^20 and G 4096 (the host checks), and the rounding of
+// g_mul, under 1 in 2^32 / G, reaches a quotient only from 2^32 / G on.
+__device__ __forceinline__ int div_g(const AttnArgs &a, int n) { return a.G == 1 ? n : (int)__umulhi((uint32_t)n, a.g_mul); }
 
 // ---- the work list -------------------------------------------------------------
 // Sequence b: first row of q, tokens, positions; `cu` units of every (kv head, row
@@ -64,45 +73,49 @@ __device__ __forceinline__ Seq load_seq(const AttnArgs &a, int b, int R, bool re
     s.units = (uint32_t)a.pool.nkv * s.nrt * s.cu;
     return s;
 }
-// Run i of nc equal runs of U units starts at floor(i U / nc).
-struct Runs {
-    uint32_t U, nc, q, r;
-    __device__ uint32_t start(uint32_t i) const { return i * q + i * r / nc; }   // r < nc <= 320
+// A run's share of the list, found by one whole warp: its units, and the
+// sequence holding the first with the units before it.
+struct Share {
+    uint32_t u0, u1, before;
+    int b;
 };
-// The runs, by one whole warp.
-__device__ __forceinline__ Runs make_runs(const AttnArgs &a, int R, uint32_t grid, bool report) {
-    uint32_t n = 0;
-    for (int b = threadIdx.x & 31; b < a.tab.n_seqs; b += 32) n += load_seq(a, b, R, report).units;
-    Runs w;
-    w.U = __reduce_add_sync(0xffffffffu, n);
-    w.nc = min(grid, w.U);               // no run is empty
-    w.q = w.nc ? w.U / w.nc : 0;
-    w.r = w.nc ? w.U % w.nc : 0;
-    return w;
-}
-// The sequence holding unit u < U, and the units before it; by one whole warp.
-__device__ __forceinline__ int find_unit(const AttnArgs &a, int R, uint32_t u, uint32_t &before) {
-    uint32_t base = 0;
+__device__ __forceinline__ Share my_share(const AttnArgs &a, int R) {
     const int lane = threadIdx.x & 31;
+    uint32_t n = 0, mine = 0, incl = 0;
     for (int b0 = 0; b0 < a.tab.n_seqs; b0 += 32) {
-        const int b = b0 + lane;
-        const uint32_t mine = b < a.tab.n_seqs ? load_seq(a, b, R, false).units : 0;
-        uint32_t incl = mine;
+        mine = b0 + lane < a.tab.n_seqs ? load_seq(a, b0 + lane, R, blockIdx.x == 0).units : 0;
+        n += mine;
+    }
+    incl = mine;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t up = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += up;
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += up;
+    }
+    const uint32_t U = __reduce_add_sync(0xffffffffu, n), per = (U + gridDim.x - 1) / gridDim.x;
+    Share s = {0, 0, 0, 0};
+    if (per * blockIdx.x >= U) return s;     // the longest run is as long as with more, shorter ones; fewer items are cut
+    s.u0 = per * blockIdx.x, s.u1 = min(U, s.u0 + per);
+    uint32_t base = 0;
+    for (int b0 = 0;; b0 += 32) {        // ends: u0 < U
+        if (a.tab.n_seqs > 32) {         // else the one chunk's sums are still here
+            mine = b0 + lane < a.tab.n_seqs ? load_seq(a, b0 + lane, R, false).units : 0;
+            incl = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t up = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += up;
+            }
         }
-        const uint32_t hit = __ballot_sync(0xffffffffu, base + incl > u);
+        const uint32_t hit = __ballot_sync(0xffffffffu, base + incl > s.u0);
         if (hit) {
             const int l = __ffs(hit) - 1;
-            before = base + __shfl_sync(0xffffffffu, incl - mine, l);
-            return b0 + l;
+            s.before = base + __shfl_sync(0xffffffffu, incl - mine, l);
+            s.b = b0 + l;
+            return s;
         }
         base += __shfl_sync(0xffffffffu, incl, 31);
     }
-    before = base;
-    return a.tab.n_seqs;
 }
 // Row tile of an item index: from both ends in turn, so that a run of neighbouring
 // items of a causal prompt holds early (short) and late (long) ones alike.
@@ -206,8 +219,8 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
     float *qb = reinterpret_cast<float *>(smem + C::RING + C::QF);
     float *sm = reinterpret_cast<float *>(smem + C::RING + C::QF + C::QB), *sl = sm + kWarps * R;
     __shared__ uint64_t bars[kWarps * C::ST];
-    __shared__ uint32_t s_u0, s_u1, s_before;
-    __shared__ int s_b, abort_flag;
+    __shared__ Share s_share;
+    __shared__ int abort_flag;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     if (threadIdx.x == 0) abort_flag = 0;
     if (lane == 0)
@@ -216,17 +229,14 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
     pdl_launch_dependents();
     pdl_wait();
     if (warp == 0) {
-        const Runs w = make_runs(a, R, gridDim.x, blockIdx.x == 0);
-        const bool on = blockIdx.x < w.nc;
-        const uint32_t u0 = on ? w.start(blockIdx.x) : 0, u1 = on ? w.start(blockIdx.x + 1) : 0;
-        uint32_t before = 0;
-        const int b = on ? find_unit(a, R, u0, before) : a.tab.n_seqs;
-        if (lane == 0) s_u0 = u0, s_u1 = u1, s_before = before, s_b = b;
+        const Share s = my_share(a, R);
+        if (lane == 0) s_share = s;
     }
+    if (threadIdx.x >= 32 && threadIdx.x < 34) a.meta[blockIdx.x * 2 + threadIdx.x - 32] = make_int4(-1, 0, 0, 0);
     __syncthreads();
-    const uint32_t u1 = s_u1;
-    uint32_t u = s_u0, before = s_before;
-    int b = s_b;
+    const uint32_t u1 = s_share.u1;
+    uint32_t u = s_share.u0, before = s_share.before;
+    int b = s_share.b;
     if (u >= u1) return;
     const Exponents expo;
     Seq sq = load_seq(a, b, R, false);
@@ -241,10 +251,10 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
         }
         const uint32_t off = u - before, item = off / (uint32_t)sq.cu;
         const int c0 = (int)(off - item * sq.cu), c1 = (int)min((uint32_t)sq.cu, c0 + (u1 - u));
-        const int kvh = (int)(item / (uint32_t)sq.nrt), rt = row_tile((int)(item - (uint32_t)kvh * sq.nrt), sq.nrt);
+        const int kvh = sq.nrt == 1 ? (int)item : (int)(item / (uint32_t)sq.nrt), rt = row_tile((int)(item - (uint32_t)kvh * sq.nrt), sq.nrt);
         const int rows = min(R, sq.nq * a.G - rt * R);                   // live rows of the tile
         const int first = sq.len - sq.nq;                               // position of token 0
-        const int nk = max(0, min(sq.len, first + (rt * R + rows - 1) / a.G + 1));   // positions the last row sees
+        const int nk = max(0, min(sq.len, first + div_g(a, rt * R + rows - 1) + 1));   // positions the last row sees
         const int t0 = c0 << (a.unit_shift - 4), t1 = min(c1 << (a.unit_shift - 4), (nk + kTile - 1) / kTile);
         // stage j of this warp: `tps` tiles from t0 + tps (warp + 8 j); one each where two would leave warps idle
         const int tps = t1 - t0 > kWarps ? 2 : 1, ts0 = t0 + tps * warp;
@@ -293,8 +303,9 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
             const int nr = e / (NB * 32), blk = e / 32 % NB, ln = e % 32, r = rt * R + nr * 8 + ln / 4;
             float x[8] = {};
             if (nr * 8 + ln / 4 < rows) {
-                const T *p = static_cast<const T *>(a.q) + (long)(sq.q0 + r / a.G) * a.qs +
-                             (long)(kvh * a.G + r % a.G) * D + blk * 32 + (ln & 3) * 8;
+                const int tok = div_g(a, r);
+                const T *p = static_cast<const T *>(a.q) + (long)(sq.q0 + tok) * a.qs +
+                             (long)(kvh * a.G + r - tok * a.G) * D + blk * 32 + (ln & 3) * 8;
                 if constexpr (HL) {
                     const float4 v0 = *reinterpret_cast<const float4 *>(p), v1 = *reinterpret_cast<const float4 *>(p + 4);
                     x[0] = v0.x, x[1] = v0.y, x[2] = v0.z, x[3] = v0.w, x[4] = v1.x, x[5] = v1.y, x[6] = v1.z, x[7] = v1.w;
@@ -332,7 +343,7 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
             for (int i = 0; i < 2; ++i) {
                 m[nr][i] = -INFINITY, nm[nr][i] = 0.f, l[nr][i] = 0.f;
                 const int r = nr * 8 + 2 * t + i;
-                lim[nr][i] = r < rows ? min(sq.len, first + (rt * R + r) / a.G + 1) : 0;
+                lim[nr][i] = r < rows ? min(sq.len, first + div_g(a, rt * R + r) + 1) : 0;
             }
 #pragma unroll
             for (int i = 0; i < MT; ++i) o[nr][i][0] = o[nr][i][1] = o[nr][i][2] = o[nr][i][3] = 0.f;
@@ -341,7 +352,7 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
 #pragma unroll
             for (int blk = 0; blk < NB; ++blk) qi[blk][0] = qb[blk * 8 + 2 * t], qi[blk][1] = qb[blk * 8 + 2 * t + 1];
         }
-        const int minlim = max(0, first + rt * R / a.G + 1);
+        const int minlim = max(0, first + div_g(a, rt * R) + 1);
         const int k0 = (g >> 1) + 4 * (g & 1);              // this lane's two positions of a tile: k0, k0 + 8
 
         // n <= TT tiles at position p0; EDGE: fewer than TT, masked positions, or missing pages.
@@ -596,8 +607,9 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
                             const int r = rt * R + rr;
                             const float inv = Ls[i] > 0.f ? 1.f / Ls[i] : 0.f;
                             const float y0 = (i ? x.y : x.x) * inv, y1 = (i ? x.w : x.z) * inv;
-                            T *p = static_cast<T *>(a.out) + (long)(sq.q0 + r / a.G) * a.os +
-                                   (long)(kvh * a.G + r % a.G) * D + dim;
+                            const int tok = div_g(a, r);
+                            T *p = static_cast<T *>(a.out) + (long)(sq.q0 + tok) * a.os +
+                                   (long)(kvh * a.G + r - tok * a.G) * D + dim;
                             if constexpr (HL) *reinterpret_cast<float2 *>(p) = make_float2(y0, y1);
                             else *reinterpret_cast<__half2 *>(p) = __floats2half2_rn(y0, y1);
                         }
@@ -606,10 +618,8 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
                     reinterpret_cast<float4 *>(a.part)[((long)slot * NR + nr) * MT * 32 + threadIdx.x] = x;
                     if (k == 0 && g == 0)
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            float *p = a.ml + ((long)slot * R + nr * 8 + 2 * t + i) * 2;
-                            p[0] = M[i], p[1] = Ls[i];
-                        }
+                        for (int i = 0; i < 2; ++i) a.ml[(long)slot * R + nr * 8 + 2 * t + i] = make_float2(M[i], Ls[i]);
+                    if (nr == 0 && threadIdx.x == 0) a.meta[slot] = make_int4((int)(before + item * sq.cu), b, kvh, rt | (c0 ? kInside : 0));
                 }
             }
             if (nr == NR - 1) fence_proxy_async_smem();   // the next copies into the ring come after these accesses
@@ -620,39 +630,46 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
     }
 }
 
-// One CTA per (cut between two runs, 8-row group, 16-dim fragment).  The first cut
-// inside an item joins the partials of all runs that share the item, each warp
-// every 8th run, in a fixed order.
-template <typename T, int D, int NR>
-__global__ void __launch_bounds__(kWarps * 32) merge_kernel(const AttnArgs a, uint32_t grid) {
-    constexpr int R = 8 * NR, MT = D / 16;
+// Joins at the first cut inside an item the partials of all runs that share the
+// item, in a fixed order.  What each run left is in its meta entries, so that the many cuts
+// with nothing to do leave after one round of loads.  PW warps share the runs of
+// one 16-dim fragment, 8 / PW fragments per CTA: with few items each is cut into
+// many parts and the loads of one warp would follow each other; with many items the CTAs would.
+template <typename T, int D, int NR, int PW>
+__global__ void __launch_bounds__(kWarps * 32) merge_kernel(const AttnArgs a, int grid) {
+    constexpr int R = 8 * NR, MT = D / 16, KC = kWarps / PW, NY = (MT + KC - 1) / KC;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int nr = blockIdx.y / MT, k = blockIdx.y % MT;
+    const int nr = blockIdx.y / NY, k = blockIdx.y % NY * KC + warp / PW, w = warp % PW;
     __shared__ float2 s_ml[kMaxCtas][8];
     __shared__ float4 s_o[kWarps][32];
     __shared__ float s_l[kWarps][8];
     pdl_launch_dependents();
     pdl_wait();
-    const Runs w = make_runs(a, R, grid, false);
-    const uint32_t c = blockIdx.x + 1;                       // the cut before run c
-    if (c >= w.nc) return;
-    const uint32_t u = w.start(c);
-    uint32_t before;
-    const int b = find_unit(a, R, u, before);
-    const Seq sq = load_seq(a, b, R, false);
-    const uint32_t item = (u - before) / (uint32_t)sq.cu, ua = before + item * sq.cu, ub = ua + sq.cu;
-    if (u == ua || w.start(c - 1) > ua) return;              // a whole item on each side, or not the item's first cut
-    const int kvh = (int)(item / (uint32_t)sq.nrt), rt = row_tile((int)(item - (uint32_t)kvh * sq.nrt), sq.nrt);
-    const int rows = min(R, sq.nq * a.G - rt * R);
-    if (nr * 8 >= rows) return;
-    const uint32_t last = (uint32_t)(((uint64_t)ub * w.nc - 1) / w.U);   // the run holding the item's last unit
-    const int np = (int)(last - c) + 2;                      // runs c - 1 .. last
-    const int slot0 = 2 * (int)(c - 1) + (w.start(c - 1) != ua ? 1 : 0);
-    for (int e = threadIdx.x; e < np * 8; e += kWarps * 32) {
-        const int slot = e < 8 ? slot0 : 2 * (int)(c - 1 + e / 8);
-        s_ml[e / 8][e % 8] = __ldcg(reinterpret_cast<const float2 *>(a.ml) + (long)slot * R + nr * 8 + e % 8);
+    const int c = blockIdx.x + 1;                            // the cut before run c
+    const int4 here = __ldcg(a.meta + 2 * c);
+    const int4 p0 = __ldcg(a.meta + 2 * c - 2), p1 = __ldcg(a.meta + 2 * c - 1);
+    if (here.x == -1 || !(here.w & kInside)) return;         // run c starts with an item of its own
+    int slot0 = 2 * c - 1;                                   // the item's first part, where it lies in run c - 1
+    if (p1.x != here.x) {
+        if (p0.x != here.x || (p0.w & kInside)) return;      // an earlier cut joins this item
+        slot0 = 2 * c - 2;
     }
+    int last = c;                                            // the last run with a part of the item
+    for (int i = c + 1; i < grid; i += 32) {
+        const int4 x = i + lane < grid ? __ldcg(a.meta + 2 * (i + lane)) : make_int4(-1, 0, 0, 0);
+        const uint32_t out = __ballot_sync(0xffffffffu, x.x != here.x || !(x.w & kInside));
+        last += out ? __ffs(out) - 1 : 32;
+        if (out) break;
+    }
+    const int b = here.y, kvh = here.z, rt = here.w & (kInside - 1), np = last - c + 2;
+    for (int e = threadIdx.x; e < np * 8; e += kWarps * 32) {
+        const int slot = e < 8 ? slot0 : 2 * (c - 1 + e / 8);
+        s_ml[e / 8][e % 8] = __ldcg(a.ml + (long)slot * R + nr * 8 + e % 8);
+    }
+    const int q0 = a.q_start ? a.q_start[b] : b;
+    const int rows = min(R, (a.q_start ? a.q_start[b + 1] - q0 : 1) * a.G - rt * R);
     __syncthreads();
+    if (nr * 8 >= rows) return;
     float M[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
     for (int p = g; p < np; p += 8)
 #pragma unroll
@@ -662,40 +679,43 @@ __global__ void __launch_bounds__(kWarps * 32) merge_kernel(const AttnArgs a, ui
 #pragma unroll
         for (int i = 0; i < 2; ++i) M[i] = fmaxf(M[i], __shfl_xor_sync(0xffffffffu, M[i], sh));
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (k < MT) {
 #pragma unroll 4
-    for (int p = warp; p < np; p += kWarps) {
-        const int slot = p == 0 ? slot0 : 2 * (int)(c - 1 + p);
-        const float4 y = __ldcg(reinterpret_cast<const float4 *>(a.part) + ((long)slot * NR + nr) * MT * 32 + k * 32 + lane);
-        float f[2];
+        for (int p = w; p < np; p += PW) {
+            const int slot = p == 0 ? slot0 : 2 * (c - 1 + p);
+            const float4 y = __ldcg(reinterpret_cast<const float4 *>(a.part) + ((long)slot * NR + nr) * MT * 32 + k * 32 + lane);
+            float f[2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const float2 ml = s_ml[p][2 * t + i];
-            f[i] = M[i] == -INFINITY ? 0.f : ex2(ml.x - M[i]);
-            l[i] = fmaf(ml.y, f[i], l[i]);
+            for (int i = 0; i < 2; ++i) {
+                const float2 ml = s_ml[p][2 * t + i];
+                f[i] = M[i] == -INFINITY ? 0.f : ex2(ml.x - M[i]);
+                l[i] = fmaf(ml.y, f[i], l[i]);
+            }
+            x.x = fmaf(y.x, f[0], x.x), x.y = fmaf(y.y, f[1], x.y);
+            x.z = fmaf(y.z, f[0], x.z), x.w = fmaf(y.w, f[1], x.w);
         }
-        x.x = fmaf(y.x, f[0], x.x), x.y = fmaf(y.y, f[1], x.y);
-        x.z = fmaf(y.z, f[0], x.z), x.w = fmaf(y.w, f[1], x.w);
     }
-    s_o[warp][lane] = x;
-    if (g == 0) s_l[warp][2 * t] = l[0], s_l[warp][2 * t + 1] = l[1];
-    __syncthreads();
-    if (warp) return;
+    if constexpr (PW > 1) {
+        s_o[warp][lane] = x;
+        if (g == 0) s_l[warp][2 * t] = l[0], s_l[warp][2 * t + 1] = l[1];
+        __syncthreads();
+        if (w) return;
 #pragma unroll
-    for (int i = 1; i < kWarps; ++i) {
-        const float4 y = s_o[i][lane];
-        x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+        for (int i = 1; i < PW; ++i) {
+            const float4 y = s_o[warp + i][lane];
+            x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+            l[0] += s_l[warp + i][2 * t], l[1] += s_l[warp + i][2 * t + 1];
+        }
     }
+    if (k >= MT) return;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int rr = nr * 8 + 2 * t + i;
         if (rr >= rows) continue;
-        float ls = 0.f;
-#pragma unroll
-        for (int j = 0; j < kWarps; ++j) ls += s_l[j][2 * t + i];
-        const int r = rt * R + rr;
-        const float inv = ls > 0.f ? 1.f / ls : 0.f;
+        const int r = rt * R + rr, tok = div_g(a, r);
+        const float inv = l[i] > 0.f ? 1.f / l[i] : 0.f;
         const float y0 = (i ? x.y : x.x) * inv, y1 = (i ? x.w : x.z) * inv;
-        T *p = static_cast<T *>(a.out) + (long)(sq.q0 + r / a.G) * a.os + (long)(kvh * a.G + r % a.G) * D + g * (D / 8) + 2 * k;
+        T *p = static_cast<T *>(a.out) + (long)(q0 + tok) * a.os + (long)(kvh * a.G + r - tok * a.G) * D + g * (D / 8) + 2 * k;
         if constexpr (sizeof(T) == 4) *reinterpret_cast<float2 *>(p) = make_float2(y0, y1);
         else *reinterpret_cast<__half2 *>(p) = __floats2half2_rn(y0, y1);
     }
@@ -715,10 +735,12 @@ static int launch(DevCtx *c, AttnArgs &a, cudaStream_t s) {
     while (items * ((cover >> a.unit_shift) + 1) > 0x7fffffffl) ++a.unit_shift;   // items <= 2^24: ends by 25
     const long most = std::min<long>(items, kMaxCtas) * ((cover >> a.unit_shift) + 1);
     const int grid = (int)std::min<long>(std::min(kMaxCtas, c->sm_count * (NR == 1 ? 2 : 1)), most);
-    a.ml = a.part + (size_t)kMaxCtas * 2 * R * D;
+    a.ml = reinterpret_cast<float2 *>(a.part + (size_t)kMaxCtas * 2 * R * D);
+    a.meta = reinterpret_cast<int4 *>(a.ml + kMaxCtas * 2 * R);
     int st = launch_pdl(attn_kernel<T, D, NR>, dim3(grid), dim3(kWarps * 32), Cfg<D, NR>::SMEM, s, a);
     if (st || grid == 1) return st;
-    return launch_pdl(merge_kernel<T, D, NR>, dim3(grid - 1, NR * (D / 16)), dim3(kWarps * 32), 0, s, a, (uint32_t)grid);
+    if (items * 8 >= grid) return launch_pdl(merge_kernel<T, D, NR, 1>, dim3(grid - 1, NR), dim3(kWarps * 32), 0, s, a, grid);
+    return launch_pdl(merge_kernel<T, D, NR, 8>, dim3(grid - 1, NR * (D / 16)), dim3(kWarps * 32), 0, s, a, grid);
 }
 
 template <typename T, int D>
@@ -744,7 +766,7 @@ extern "C" {
 
 size_t x100q_kv4_attn_work(const x100q_kv4 *kv, int n_tokens, int n_heads, int n_seqs) {
     if (!shape_ok(kv) || n_tokens < 0 || n_seqs < 1 || n_heads < 1 || n_heads % kv->n_kv_heads) return 0;
-    return (size_t)kMaxCtas * 2 * 32 * (kv->head_dim + 2) * sizeof(float);
+    return (size_t)kMaxCtas * 2 * (32 * (kv->head_dim + 2) * sizeof(float) + sizeof(int4));
 }
 
 int x100q_kv4_attn_dev(const x100q_kv4 *kv, const x100q_kv4_attn_args *a, void *stream) {
@@ -770,11 +792,12 @@ int x100q_kv4_attn_dev(const x100q_kv4 *kv, const x100q_kv4_attn_args *a, void *
     p.q_start = a->q_start, p.kv_len = a->kv_len;
     p.n_tokens = a->n_tokens, p.max_q = a->q_start ? std::min(a->max_q, a->n_tokens) : 1;
     p.nh = a->n_heads, p.G = a->n_heads / kv->n_kv_heads;
+    p.g_mul = (uint32_t)(((1ull << 32) + p.G - 1) / p.G);
     p.sl = a->scale * 1.4426950408889634f;
     p.part = static_cast<float *>(a->work);
     p.status = c->d_status;
     const long items = (long)a->n_seqs * kv->n_kv_heads * (((long)p.max_q * p.G + 7) / 8);
-    if (items > (1l << 24) || (long)p.max_q * p.G > (1l << 30)) return refuse(X100_E_TOO_LARGE);
+    if (items > (1l << 24) || (long)p.max_q * p.G > (1l << 20)) return refuse(X100_E_TOO_LARGE);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (a->dtype == X100Q_F32)
         return kv->head_dim == 128 ? launch_rows<float, 128>(c, p, s) : launch_rows<float, 64>(c, p, s);

@@ -513,38 +513,55 @@ def quantize_q8_0_dev(x, n: int, blocks, stream=None) -> None:
 
 
 # ---- paged 4-bit KV cache, residual RMS norm with 8-bit output (torch tensors) ---------------
-def _on_device(what: str, dtypes: dict) -> None:
-    """Every tensor of `dtypes` (name -> (tensor or None, dtype)) has its type and lies on the current device."""
+_DTYPE_ID: dict = {}   # torch dtype -> Q_F32 / Q_F16, filled with torch's first use here
+_raw_stream = None
+
+
+def _torch_types():
     import torch
-    dev = torch.cuda.current_device()
-    for name, (t, dt) in dtypes.items():
-        if t is not None and (t.dtype is not dt or t.get_device() != dev):
-            raise X100Error(X100_E_ARG, f"{what}: {name} has to be {dt} on the current device (cuda:{dev}), "
-                                        f"not {t.dtype} on {t.device}")
+    _DTYPE_ID.update({torch.float32: Q_F32, torch.float16: Q_F16})
 
 
 def _dtype_id(t, what: str) -> int:
+    if not _DTYPE_ID:
+        _torch_types()
+    i = _DTYPE_ID.get(t.dtype)
+    if i is None:
+        raise X100Error(X100_E_UNSUPPORTED, f"{what}: float32 or float16 is taken, not {t.dtype}")
+    return i
+
+
+def _here(stream):
+    """(current device, stream handle): the current device's current stream unless one is given."""
+    global _raw_stream
     import torch
-    if t.dtype is torch.float32:
-        return Q_F32
-    if t.dtype is torch.float16:
-        return Q_F16
-    raise X100Error(X100_E_UNSUPPORTED, f"{what}: float32 or float16 is taken, not {t.dtype}")
+    if _raw_stream is None:
+        _raw_stream = torch._C._cuda_getCurrentRawStream
+    dev = torch.cuda.current_device()
+    return dev, (_raw_stream(dev) if stream is None else _stream(stream))
 
 
-def _heads(t, name: str, what: str, dim: int):
+def _need(ok: bool, what: str, why: str) -> None:
+    if not ok:
+        raise X100Error(X100_E_ARG, f"{what}: {why}")
+
+
+def _take(t, name: str, what: str, dtype, dev: int) -> int:
+    """Pointer of a tensor of `dtype` on device `dev` (None: no pointer)."""
+    if t is None:
+        return 0
+    if t.dtype is not dtype or t.get_device() != dev:
+        raise X100Error(X100_E_ARG, f"{what}: {name} has to be {dtype} on the current device (cuda:{dev}), not {t.dtype} on {t.device}")
+    return t.data_ptr()
+
+
+def _heads(t, name: str, what: str, dim: int) -> int:
     """Token stride of [tokens, heads, dim] with the heads of a token side by side."""
+    if t.is_contiguous() and t.dim() == 3 and t.shape[2] == dim:
+        return t.shape[1] * dim
     if t.dim() != 3 or t.shape[2] != dim or t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != dim):
         raise X100Error(X100_E_ARG, f"{what}: {name} has to be [tokens, heads, {dim}], a token's heads side by side")
     return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1] * dim)
-
-
-def _ints(what: str, **named):
-    import torch
-    _on_device(what, {n: (t, torch.int32) for n, t in named.items()})
-    for n, t in named.items():
-        if t is not None and not t.is_contiguous():
-            raise X100Error(X100_E_ARG, f"{what}: {n} has to be contiguous")
 
 
 class Kv4Cache:
@@ -557,55 +574,66 @@ class Kv4Cache:
         self.kv = Kv4(None, n_pages, page_size, n_kv_heads, head_dim)
         self._ref = C.byref(self.kv)
         n = lib().x100q_kv4_bytes(self._ref)
-        if n == 0:
-            raise X100Error(X100_E_ARG, f"Kv4Cache: {n_pages} pages of {page_size} x {n_kv_heads} x {head_dim}")
+        _need(n > 0, "Kv4Cache", f"no pool of {n_pages} pages of {page_size} x {n_kv_heads} x {head_dim}")
         if pages is None:
             pages = torch.zeros(n, dtype=torch.uint8, device="cuda")
-        if pages.dtype is not torch.uint8 or not pages.is_cuda or not pages.is_contiguous() or pages.numel() < n:
-            raise X100Error(X100_E_ARG, f"Kv4Cache: pages has to be {n} contiguous uint8 on a GPU")
-        self.pages, self.kv.pages = pages, pages.data_ptr()
+        _need(pages.dtype is torch.uint8 and pages.is_cuda and pages.is_contiguous() and pages.numel() >= n, "Kv4Cache",
+              f"pages has to be {n} contiguous uint8 on a GPU")
+        self.pages, self.kv.pages, self.device = pages, pages.data_ptr(), pages.get_device()
         self.head_dim, self.n_kv_heads = head_dim, n_kv_heads
+
+    def _common(self, what, stream, table, **ints):
+        """Device, stream and the pointers of the int32 tensors (the page table's first)."""
+        import torch
+        dev, raw = _here(stream)
+        _need(dev == self.device, what, f"the pool is on cuda:{self.device}, the current device is cuda:{dev}")
+        _need(table.dim() == 2 and all(t is None or t.is_contiguous() for t in (table, *ints.values())), what,
+              "the page table has to be [sequences, entries], and it and the other integers contiguous")
+        return dev, raw, [_take(t, n, what, torch.int32, dev) for n, t in (("table", table), *ints.items())]
 
     def append(self, k, v, pos, table, seq=None, q=None, q_out=None, q_norm=None, k_norm=None, eps=1e-6, rope=None, stream=None):
         """x100q_kv4_append_dev: k, v [tokens, kv heads, dim] into the pages; returns q_out, the normed and rotated q."""
         import torch
-        what, D = "Kv4Cache.append", self.head_dim
-        dt = _dtype_id(k, what)
-        if q is not None and q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        _on_device(what, {"pages": (self.pages, torch.uint8), "k": (k, k.dtype), "v": (v, k.dtype), "q": (q, k.dtype), "q_out": (q_out, k.dtype),
-                          "q_norm": (q_norm, torch.float32), "k_norm": (k_norm, torch.float32), "rope": (rope, torch.float32)})
-        _ints(what, pos=pos, seq=seq, table=table)
-        n = pos.numel()
+        what, D, dt = "Kv4Cache.append", self.head_dim, k.dtype
+        kind = _dtype_id(k, what)
+        dev, raw, (tp, pp, sp) = self._common(what, stream, table, pos=pos, seq=seq)
+        n, kv = pos.numel(), self.n_kv_heads
         ks, vs = _heads(k, "k", what, D), _heads(v, "v", what, D)
+        _need(k.shape[0] == n and v.shape[0] == n and k.shape[1] == kv and v.shape[1] == kv and (seq is None or seq.numel() == n), what,
+              f"k and v have to be [{n}, {kv}, {D}], and seq as long as pos")
         qs = qos = nh = 0
         if q is not None:
+            if q_out is None:
+                q_out = torch.empty(q.shape, dtype=dt, device=q.device)
             qs, qos, nh = _heads(q, "q", what, D), _heads(q_out, "q_out", what, D), q.shape[1]
-        if (k.shape[0] != n or v.shape[0] != n or k.shape[1] != self.n_kv_heads or v.shape[1] != self.n_kv_heads or table.dim() != 2
-                or (seq is not None and seq.numel() != n) or (q is not None and (q.shape[0] != n or q_out.shape != q.shape))
-                or any(w is not None and (w.numel() != D or not w.is_contiguous()) for w in (q_norm, k_norm))
-                or (rope is not None and (rope.numel() % D or not rope.is_contiguous()))):
-            raise X100Error(X100_E_ARG, f"{what}: shapes do not agree")
-        a = Kv4AppendArgs(dt, n, nh, _p(q), k.data_ptr(), v.data_ptr(), _p(q_out), qs, ks, vs, qos, _p(q_norm), _p(k_norm), eps,
-                          _p(rope), rope.numel() // D if rope is not None else 0, pos.data_ptr(), _p(seq), table.data_ptr(),
-                          table.shape[1], table.shape[0])
-        check(lib().x100q_kv4_append_dev(self._ref, C.byref(a), _stream(stream)), "x100q_kv4_append_dev")
+            _need(q.shape[0] == n and q_out.shape == q.shape, what, f"q and q_out have to be [{n}, heads, {D}]")
+        f32 = torch.float32
+        for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
+            _need(w is None or (w.numel() == D and w.is_contiguous()), what, f"{name} has to be {D} contiguous values")
+        _need(rope is None or (rope.numel() % D == 0 and rope.is_contiguous()), what, f"rope has to be [positions, {D // 2}, 2]")
+        a = Kv4AppendArgs(kind, n, nh, _take(q, "q", what, dt, dev), _take(k, "k", what, dt, dev), _take(v, "v", what, dt, dev),
+                          _take(q_out, "q_out", what, dt, dev), qs, ks, vs, qos, _take(q_norm, "q_norm", what, f32, dev),
+                          _take(k_norm, "k_norm", what, f32, dev), eps, _take(rope, "rope", what, f32, dev),
+                          rope.numel() // D if rope is not None else 0, pp, sp, tp, table.shape[1], table.shape[0])
+        rc = lib().x100q_kv4_append_dev(self._ref, C.byref(a), raw)
+        if rc:
+            check(rc, "x100q_kv4_append_dev")
         return q_out
 
     def read(self, pos, table, seq=None, k_out=None, v_out=None, stream=None):
         """x100q_kv4_read_dev: the values (k, v) of the positions, fp16 [tokens, kv heads, dim]; both are made when neither is given."""
         import torch
-        what = "Kv4Cache.read"
-        n = pos.numel()
+        what, n, f16 = "Kv4Cache.read", pos.numel(), torch.float16
         if k_out is None and v_out is None:
-            k_out, v_out = (torch.zeros(n, self.n_kv_heads, self.head_dim, dtype=torch.float16, device=pos.device) for _ in range(2))
-        _on_device(what, {"pages": (self.pages, torch.uint8), "k_out": (k_out, torch.float16), "v_out": (v_out, torch.float16)})
-        _ints(what, pos=pos, seq=seq, table=table)
-        if (table.dim() != 2 or (seq is not None and seq.numel() != n)
-                or any(t is not None and (t.numel() != n * self.n_kv_heads * self.head_dim or not t.is_contiguous()) for t in (k_out, v_out))):
-            raise X100Error(X100_E_ARG, f"{what}: shapes do not agree")
-        check(lib().x100q_kv4_read_dev(self._ref, pos.data_ptr(), _p(seq), n, table.data_ptr(), table.shape[1], table.shape[0],
-                                       _p(k_out), _p(v_out), _stream(stream)), "x100q_kv4_read_dev")
+            k_out, v_out = (torch.zeros(n, self.n_kv_heads, self.head_dim, dtype=f16, device=pos.device) for _ in range(2))
+        dev, raw, (tp, pp, sp) = self._common(what, stream, table, pos=pos, seq=seq)
+        size = n * self.n_kv_heads * self.head_dim
+        _need((seq is None or seq.numel() == n) and all(t is None or (t.numel() == size and t.is_contiguous()) for t in (k_out, v_out)), what,
+              f"k_out and v_out have to be {size} contiguous values, and seq as long as pos")
+        rc = lib().x100q_kv4_read_dev(self._ref, pp, sp, n, tp, table.shape[1], table.shape[0], _take(k_out, "k_out", what, f16, dev),
+                                      _take(v_out, "v_out", what, f16, dev), raw)
+        if rc:
+            check(rc, "x100q_kv4_read_dev")
         return k_out, v_out
 
     def attend_work(self, n_tokens: int, n_heads: int, n_seqs: int):
@@ -616,21 +644,22 @@ class Kv4Cache:
     def attend(self, q, out, table, kv_len, q_start=None, max_q=1, scale=None, work=None, stream=None):
         """x100q_kv4_attn_dev: q [tokens, heads, dim] over the pages into out (made when None); q_start None: one token per sequence."""
         import torch
-        what, D = "Kv4Cache.attend", self.head_dim
-        dt = _dtype_id(q, what)
+        what, D, dt = "Kv4Cache.attend", self.head_dim, q.dtype
+        kind, n = _dtype_id(q, what), kv_len.numel()
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            out = torch.empty(q.shape, dtype=dt, device=q.device)
         if work is None:
-            work = self.attend_work(q.shape[0], q.shape[1], kv_len.numel())
-        _on_device(what, {"pages": (self.pages, torch.uint8), "q": (q, q.dtype), "out": (out, q.dtype), "work": (work, torch.uint8)})
-        _ints(what, q_start=q_start, kv_len=kv_len, table=table)
-        qs, os_, n = _heads(q, "q", what, D), _heads(out, "out", what, D), kv_len.numel()
-        if (out.shape != q.shape or table.dim() != 2 or table.shape[0] != n or (q_start is not None and q_start.numel() != n + 1)
-                or not work.is_contiguous()):
-            raise X100Error(X100_E_ARG, f"{what}: shapes do not agree")
-        a = Kv4AttnArgs(dt, q.shape[1], q.data_ptr(), out.data_ptr(), qs, os_, _p(q_start), q.shape[0], max_q, kv_len.data_ptr(),
-                        table.data_ptr(), table.shape[1], n, D ** -0.5 if scale is None else scale, work.data_ptr(), work.numel())
-        check(lib().x100q_kv4_attn_dev(self._ref, C.byref(a), _stream(stream)), "x100q_kv4_attn_dev")
+            work = self.attend_work(q.shape[0], q.shape[1], n)
+        dev, raw, (tp, lp, qp) = self._common(what, stream, table, kv_len=kv_len, q_start=q_start)
+        qs, os_ = _heads(q, "q", what, D), _heads(out, "out", what, D)
+        rows, heads = q.shape[0], q.shape[1]
+        _need(out.shape == q.shape and table.shape[0] == n and (q_start is None or q_start.numel() == n + 1) and work.is_contiguous(), what,
+              "out has to be as q, the page table and q_start as kv_len's sequences, and work contiguous")
+        a = Kv4AttnArgs(kind, heads, _take(q, "q", what, dt, dev), _take(out, "out", what, dt, dev), qs, os_, qp, rows, max_q, lp, tp,
+                        table.shape[1], n, D ** -0.5 if scale is None else scale, _take(work, "work", what, torch.uint8, dev), work.numel())
+        rc = lib().x100q_kv4_attn_dev(self._ref, C.byref(a), raw)
+        if rc:
+            check(rc, "x100q_kv4_attn_dev")
         return out
 
 
@@ -645,19 +674,28 @@ def rope_table(n_pos: int, head_dim: int, base: float, stream=None):
 def add_rmsnorm_q8(x, w, q, scales, residual=None, residual_out=None, eps=1e-6, group=0, stream=None):
     """x100q_add_rmsnorm_q8_dev: rows of x (+ residual, the sum to residual_out) RMS-normed with w into int8 q and its scales."""
     import torch
-    what = "add_rmsnorm_q8"
-    dt = _dtype_id(x, what)
-    _on_device(what, {"x": (x, x.dtype), "residual": (residual, x.dtype), "residual_out": (residual_out, x.dtype),
-                      "w": (w, torch.float32), "q": (q, torch.int8), "scales": (scales, torch.float32)})
-    rows, d = x.shape if x.dim() == 2 else (0, 0)
-    if (x.dim() != 2 or w.numel() != d or not w.is_contiguous() or not scales.is_contiguous()
-            or scales.numel() != rows * (d // group if group else 1)
-            or any(t is not None and (t.shape != x.shape or (d > 1 and t.stride(1) != 1)) for t in (x, q, residual, residual_out))):
-        raise X100Error(X100_E_ARG, f"{what}: shapes do not agree, or rows are not contiguous")
-    ld = lambda t: 0 if t is None else t.stride(0) if rows > 1 else d  # noqa: E731
-    a = NormQ8Args(dt, rows, d, group, x.data_ptr(), _p(residual), _p(residual_out), ld(x), ld(residual), ld(residual_out), ld(q),
-                   w.data_ptr(), eps, q.data_ptr(), scales.data_ptr())
-    check(lib().x100q_add_rmsnorm_q8_dev(C.byref(a), _stream(stream)), "x100q_add_rmsnorm_q8_dev")
+    what, dt, f32 = "add_rmsnorm_q8", x.dtype, torch.float32
+    kind = _dtype_id(x, what)
+    _need(x.dim() == 2, what, "x has to be [rows, elements]")
+    rows, d = x.shape
+    dev, raw = _here(stream)
+    _need(w.numel() == d and w.is_contiguous() and scales.is_contiguous() and scales.numel() == rows * (d // group if group else 1), what,
+          f"w has to be {d} and scales [{rows}, groups] contiguous values")
+    ld = []
+    for name, t in (("x", x), ("residual", residual), ("residual_out", residual_out), ("q", q)):
+        if t is None:
+            ld.append(0)
+        elif t.is_contiguous() and t.shape == x.shape:
+            ld.append(d)
+        else:
+            _need(t.shape == x.shape and (d == 1 or t.stride(1) == 1), what, f"{name} has to be [{rows}, {d}] with contiguous rows")
+            ld.append(t.stride(0) if rows > 1 else d)
+    a = NormQ8Args(kind, rows, d, group, _take(x, "x", what, dt, dev), _take(residual, "residual", what, dt, dev),
+                   _take(residual_out, "residual_out", what, dt, dev), *ld, _take(w, "w", what, f32, dev), eps,
+                   _take(q, "q", what, torch.int8, dev), _take(scales, "scales", what, f32, dev))
+    rc = lib().x100q_add_rmsnorm_q8_dev(C.byref(a), raw)
+    if rc:
+        check(rc, "x100q_add_rmsnorm_q8_dev")
 
 
 EP_HANDLE_BYTES = 64
