@@ -11,68 +11,13 @@
 #include <cmath>
 #include <type_traits>
 
-#include "kv4.cuh"
-#include "ptx.cuh"
-#include "qformats.cuh"
-#include "qgemv.h"
+#include "kv4_attn.cuh"
 
 namespace x100 {
 namespace kv4 {
 
-using q::pdl_launch_dependents;
-using q::pdl_wait;
-
 constexpr int kWarps = 8;
-constexpr int kMaxCtas = 320;           // bound of the grid, which sizes the workspace
 
-struct AttnArgs {
-    Pool pool;
-    Table tab;
-    const void *q;
-    void *out;
-    long qs, os;
-    const int *q_start, *kv_len;
-    int n_tokens, max_q, nh, G;
-    uint32_t g_mul;                      // ceil(2^32 / G): n / G = umulhi(n, g_mul) for n < 2^32 / G
-    int unit_shift;                      // positions per unit, a power of two (128 unless the list would pass 2^31 units)
-    float sl;                            // scale * log2(e)
-    // work: of the first (slot 0) and last (slot 1) item that a run has a part of only
-    float *part;                         // [kMaxCtas][2][8 NR * D] o in fragment order
-    float2 *ml;                          // [kMaxCtas][2][8 NR] running max (log2 units) and sum
-    int4 *meta;                          // [kMaxCtas][2] the item: first unit, sequence, kv head, row tile | kInside; or -1
-    int *status;
-};
-
-constexpr int kInside = 1 << 30;         // the run starts inside the item
-
-// Row number over the group's heads: rows of a sequence are at most 2^20 and G 4096 (the host checks), and the rounding of
-// g_mul, under 1 in 2^32 / G, reaches a quotient only from 2^32 / G on.
-__device__ __forceinline__ int div_g(const AttnArgs &a, int n) { return a.G == 1 ? n : (int)__umulhi((uint32_t)n, a.g_mul); }
-
-// ---- the work list -------------------------------------------------------------
-// Sequence b: first row of q, tokens, positions; `cu` units of every (kv head, row
-// tile) item, at least one so that rows without positions are written.
-struct Seq {
-    int q0, nq, len, nrt, cu;
-    uint32_t units;                      // of all its items
-};
-__device__ __forceinline__ Seq load_seq(const AttnArgs &a, int b, int R, bool report) {
-    Seq s;
-    s.q0 = a.q_start ? a.q_start[b] : b;
-    s.nq = a.q_start ? a.q_start[b + 1] - s.q0 : 1;
-    s.len = a.kv_len[b];
-    const int cover = a.tab.stride > (0x7fffffff >> a.pool.page_shift) ? 0x7fffffff : a.tab.stride << a.pool.page_shift;
-    const bool bad_q = s.q0 < 0 || s.nq < 0 || s.nq > a.max_q || s.q0 > a.n_tokens - s.nq;
-    if (bad_q) s.nq = 0;
-    if (bad_q || s.len < 0 || s.len > cover) {
-        if (report) atomicCAS(a.status, 0, X100_E_ARG);
-        s.len = s.len < 0 ? 0 : min(s.len, cover);
-    }
-    s.nrt = (int)((unsigned)(s.nq * a.G + R - 1) / (unsigned)R);
-    s.cu = max(1, (s.len >> a.unit_shift) + ((s.len & ((1 << a.unit_shift) - 1)) != 0));
-    s.units = (uint32_t)a.pool.nkv * s.nrt * s.cu;
-    return s;
-}
 // A run's share of the list, found by one whole warp: its units, and the
 // sequence holding the first with the units before it.
 struct Share {
@@ -134,8 +79,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-__device__ __forceinline__ uint32_t u32(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
-__device__ __forceinline__ __half2 h2(uint32_t u) { return *reinterpret_cast<__half2 *>(&u); }
 // D = A B + C with C apart (registers or zeros)
 __device__ __forceinline__ void mma_init(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1, float c0, float c1) {
@@ -144,45 +87,6 @@ __device__ __forceinline__ void mma_init(float (&d)[4], uint32_t a0, uint32_t a1
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
 }
-// Codes of both halves of a word as fp16 by placing them under an exponent:
-// bits 0-3 under 1024's read as 1024 + code, bits 4-7 as 1024 + 16 code, and bits
-// 4-7 under 64's as 64 + code.  The exponents come in registers that the
-// compiler cannot see through: with both as immediates each (w & mask) | exponent
-// would be two instructions instead of one.
-struct Exponents {
-    uint32_t e1024, e64;
-    __device__ Exponents() {
-        asm volatile("mov.b32 %0, 0x64006400;" : "=r"(e1024));
-        asm volatile("mov.b32 %0, 0x54005400;" : "=r"(e64));
-    }
-};
-__device__ __forceinline__ uint32_t field(uint32_t w, uint32_t mask, uint32_t expo) {
-    uint32_t r;
-    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(expo));
-    return r;
-}
-constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
-// code - 8, exactly
-__device__ __forceinline__ __half2 low_codes(uint32_t w, const Exponents &x) {
-    return __hsub2(h2(field(w, kLow, x.e1024)), __float2half2_rn(1032.f));
-}
-__device__ __forceinline__ __half2 high_codes(uint32_t w, const Exponents &x) {
-    return __hfma2(h2(field(w, kHigh, x.e1024)), __float2half2_rn(0.0625f), __float2half2_rn(-72.f));
-}
-// 2^x: x <= 8 here; results under 2^-126 are zeros
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-// x = hi + lo to 22 bits
-__device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t &lo) {
-    const __half2 h = __floats2half2_rn(x, y);
-    const float2 f = __half22float2(h);
-    hi = u32(h);
-    lo = u32(__floats2half2_rn(x - f.x, y - f.y));
-}
-
 template <int D, int NR>
 struct Cfg {
     static constexpr int ST = 3;                              // ring stages per warp, two tiles each
@@ -766,7 +670,9 @@ extern "C" {
 
 size_t x100q_kv4_attn_work(const x100q_kv4 *kv, int n_tokens, int n_heads, int n_seqs) {
     if (!shape_ok(kv) || n_tokens < 0 || n_seqs < 1 || n_heads < 1 || n_heads % kv->n_kv_heads) return 0;
-    return (size_t)kMaxCtas * 2 * (32 * (kv->head_dim + 2) * sizeof(float) + sizeof(int4));
+    const size_t few = (size_t)kMaxCtas * 2 * (32 * (kv->head_dim + 2) * sizeof(float) + sizeof(int4));
+    // no sequence can have more rows than the call
+    return (long)n_tokens * (n_heads / kv->n_kv_heads) < kPrefillRows ? few : std::max(few, prefill_work(kv->head_dim));
 }
 
 int x100q_kv4_attn_dev(const x100q_kv4 *kv, const x100q_kv4_attn_args *a, void *stream) {
@@ -799,6 +705,7 @@ int x100q_kv4_attn_dev(const x100q_kv4 *kv, const x100q_kv4_attn_args *a, void *
     const long items = (long)a->n_seqs * kv->n_kv_heads * (((long)p.max_q * p.G + 7) / 8);
     if (items > (1l << 24) || (long)p.max_q * p.G > (1l << 20)) return refuse(X100_E_TOO_LARGE);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if ((long)p.max_q * p.G >= kPrefillRows) return launch_prefill(c, p, a->dtype, kv->head_dim, s);
     if (a->dtype == X100Q_F32)
         return kv->head_dim == 128 ? launch_rows<float, 128>(c, p, s) : launch_rows<float, 64>(c, p, s);
     return kv->head_dim == 128 ? launch_rows<__half, 128>(c, p, s) : launch_rows<__half, 64>(c, p, s);

@@ -1,0 +1,711 @@
+// kv4_prefill.cu -- attention of many query rows (prompt chunks) over the paged
+// 4-bit KV cache on the 5th-generation tensor cores.
+//
+// Row tiles of 128 rows (token x head of the group, as in kv4_attn.cu) and key
+// tiles of 128 positions.  Per key tile and row tile S = Q K^T and O += P V, both
+// 128 x 128 x D tcgen05.mma with S, P (over S) and O in TMEM.  One CTA per SM:
+//   warps 0-3, 4-7   softmax of step X = 0, 1: a thread owns a row; S from TMEM, running max
+//                    (moved only when a score passes it by 2^8), P as fp16 back to TMEM
+//   warps 8-11       raw codes in shared memory -> fp16 K and V tiles in the 128-byte-swizzled
+//                    layouts the MMA reads; scale * (code - 8) is an fp16 value, so exact
+//   warp 12          issues the MMAs;  warp 13  copies the raw tiles (bulk copies)
+// fp16 q: the steps X are two row tiles over the same key tile (256 rows per item), so that
+// a key tile is unpacked once for both.  fp32 q: q and P are carried as hi + lo halves, two
+// products each, and the steps X are every other key tile of one row tile, joined at the end.
+// Either way one step's softmax runs beside the other's products.
+//
+// The work list is the one of kv4_attn.cu with units of 128 positions, each row
+// tile counted with the units that its last row sees.
+#include <algorithm>
+
+#include "kv4_attn.cuh"
+
+namespace x100 {
+namespace kv4 {
+
+constexpr int kPfThreads = 512, kDqWarps = 4, kRawStages = 3;
+constexpr int kKeys = 128;                 // positions per key tile
+constexpr int kPfCtas = 160;               // bound of the grid, which sizes the workspace
+constexpr int kPfRows = 256;               // rows per slot of the workspace
+
+template <int D>
+struct Pf {
+    static constexpr int QT = 128 * D * 2;                       // one Q tile, or half of fp32 q
+    static constexpr int KT = kKeys * D * 2;                     // a K or V tile
+    static constexpr int RAW = 4 * Lay<D>::BYTES;                // 64 positions
+    static constexpr int K0 = 2 * QT, V0 = K0 + 2 * KT, RAW0 = V0 + 2 * KT, SMEM = RAW0 + kRawStages * RAW + 1024;
+    static constexpr int SUB = 128 * 128;                        // 128 rows of 64 dims
+};
+
+// ---- tcgen05 pieces that ptx.cuh lacks --------------------------------------------
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void regs_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_less() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// ---- the work list ------------------------------------------------------------------
+// Positions that row tile rt of a sequence sees, and its units.
+template <int RT>
+__device__ __forceinline__ int seen(const AttnArgs &a, const Seq &s, int rt) {
+    const int rows = min(RT, s.nq * a.G - rt * RT);
+    return max(0, min(s.len, s.len - s.nq + div_g(a, rt * RT + rows - 1) + 1));
+}
+template <int RT>
+__device__ __forceinline__ int units_of(const AttnArgs &a, const Seq &s, int rt) { return max(1, (seen<RT>(a, s, rt) + kKeys - 1) / kKeys); }
+// Units of one kv head of a sequence; by one whole warp.
+template <int RT>
+__device__ __forceinline__ uint32_t head_units(const AttnArgs &a, const Seq &s) {
+    uint32_t n = 0;
+    for (int rt = threadIdx.x & 31; rt < s.nrt; rt += 32) n += units_of<RT>(a, s, rt);
+    return __reduce_add_sync(0xffffffffu, n);
+}
+// Where a run starts: unit u0 is unit `c` of (sequence b, kv head, row tile rt),
+// whose first unit is `item`.
+struct Start {
+    uint32_t u0, u1, item;
+    int b, kvh, rt;
+};
+template <int RT>
+__device__ __forceinline__ Start my_start(const AttnArgs &a) {
+    const int lane = threadIdx.x & 31;
+    Start r = {0, 0, 0, 0, 0, 0};
+    uint32_t U = 0;
+    for (int b = 0; b < a.tab.n_seqs; ++b) {
+        const Seq s = load_seq(a, b, RT, blockIdx.x == 0 && lane == 0);
+        if (s.nrt) U += a.pool.nkv * head_units<RT>(a, s);
+    }
+    const uint32_t per = (U + gridDim.x - 1) / gridDim.x;
+    if (per * blockIdx.x >= U) return r;
+    r.u0 = per * blockIdx.x, r.u1 = min(U, r.u0 + per);
+    uint32_t base = 0;
+    for (;; ++r.b) {                       // ends: u0 < U
+        const Seq s = load_seq(a, r.b, RT, false);
+        if (!s.nrt) continue;
+        const uint32_t hu = head_units<RT>(a, s);
+        if (r.u0 - base >= hu * a.pool.nkv) {
+            base += hu * a.pool.nkv;
+            continue;
+        }
+        r.kvh = (int)((r.u0 - base) / hu);
+        base += r.kvh * hu;
+        for (int r0 = 0;; r0 += 32) {
+            const uint32_t mine = r0 + lane < s.nrt ? units_of<RT>(a, s, r0 + lane) : 0;
+            uint32_t incl = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t up = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += up;
+            }
+            const uint32_t hit = __ballot_sync(0xffffffffu, base + incl > r.u0);
+            if (hit) {
+                const int l = __ffs(hit) - 1;
+                r.item = base + __shfl_sync(0xffffffffu, incl - mine, l);
+                r.rt = r0 + l;
+                return r;
+            }
+            base += __shfl_sync(0xffffffffu, incl, 31);
+        }
+    }
+}
+// The segments of a run, one item (or a part of one) after the other.  Every role walks them by itself.
+template <int RT>
+struct Walk {
+    Start at;
+    Seq sq;
+    uint32_t u;
+    int cu, c0, c1, n;                     // units of the item; those of this segment; their number
+    __device__ Walk(const AttnArgs &a, const Start &s) : at(s), u(s.u0) {
+        if (u < at.u1) {
+            sq = load_seq(a, at.b, RT, false);
+            set(a);
+        }
+    }
+    __device__ bool more() const { return u < at.u1; }
+    __device__ void set(const AttnArgs &a) {
+        cu = units_of<RT>(a, sq, at.rt);
+        c0 = (int)(u - at.item);
+        c1 = (int)min((uint32_t)cu, (uint32_t)c0 + (at.u1 - u));
+        n = c1 - c0;
+    }
+    __device__ void next(const AttnArgs &a) {
+        u += n;
+        if (u >= at.u1) return;
+        at.item += cu;
+        if (++at.rt == sq.nrt) {
+            at.rt = 0;
+            if (++at.kvh == a.pool.nkv) {
+                at.kvh = 0;
+                do sq = load_seq(a, ++at.b, RT, false);
+                while (!sq.nrt);
+            }
+        }
+        set(a);
+    }
+};
+
+struct PfBars {
+    uint64_t raw_full[kRawStages], raw_empty[kRawStages], k_full[2], k_empty[2], v_full[2], v_empty[2];
+    uint64_t s_full[2], p_ready[2], o_done[2], q_full, joined, drain;
+    uint32_t raw_ok[kRawStages];           // bit i: 16-position tile i of the raw stage was copied
+    uint32_t tmem;
+    int abort_flag;
+    Start start;
+    float2 ml[2][128];
+};
+
+// 8 codes of a word times their scale, as fp16 in the order 0, 4, 1, 5, 2, 6, 3, 7
+__device__ __forceinline__ uint4 eight(uint32_t w, __half2 d, const Exponents &x) {
+    const uint32_t w8 = w >> 8;
+    return make_uint4(u32(__hmul2(low_codes(w, x), d)), u32(__hmul2(high_codes(w, x), d)), u32(__hmul2(low_codes(w8, x), d)),
+                      u32(__hmul2(high_codes(w8, x), d)));
+}
+
+// The query order that goes with it: the halves of 8 dims (a.x = dims 0, 1 ..) as 0, 4, 1, 5, 2, 6, 3, 7
+__device__ __forceinline__ uint4 as_eight(uint4 a) {
+    return make_uint4(__byte_perm(a.x, a.z, 0x5410), __byte_perm(a.x, a.z, 0x7632), __byte_perm(a.y, a.w, 0x5410), __byte_perm(a.y, a.w, 0x7632));
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const AttnArgs a) {
+    using L = Lay<D>;
+    using P = Pf<D>;
+    constexpr bool HL = sizeof(T) == 4;
+    constexpr int RT = HL ? 128 : 256;      // rows per item
+    constexpr int KS = D / 16, VS = kKeys / 16;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    __shared__ PfBars bars;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wg = warp >> 2;
+    if (threadIdx.x == 0) {
+        bars.abort_flag = 0;
+        for (int i = 0; i < kRawStages; ++i) mbar_init(&bars.raw_full[i], 1), mbar_init(&bars.raw_empty[i], kDqWarps);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bars.k_full[i], kDqWarps), mbar_init(&bars.k_empty[i], 1);
+            mbar_init(&bars.v_full[i], kDqWarps), mbar_init(&bars.v_empty[i], 1);
+            mbar_init(&bars.s_full[i], 1), mbar_init(&bars.p_ready[i], 4), mbar_init(&bars.o_done[i], 1);
+        }
+        mbar_init(&bars.q_full, 8), mbar_init(&bars.joined, 8), mbar_init(&bars.drain, 1);
+        fence_barrier_init();
+    }
+    if (warp == 12) {
+        tmem_alloc(&bars.tmem, 512);
+        tmem_relinquish();
+    }
+    pdl_launch_dependents();
+    pdl_wait();
+    if (warp == 0) {
+        const Start s = my_start<RT>(a);
+        if (lane == 0) bars.start = s;
+    }
+    if (threadIdx.x >= 32 && threadIdx.x < 34) a.meta[blockIdx.x * 2 + threadIdx.x - 32] = make_int4(-1, 0, 0, 0);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = bars.tmem, tS = tmem, tO = tmem + 256;   // S, O of step X: + 128 X columns
+    Walk<RT> w(a, bars.start);
+    volatile int *abort_flag = &bars.abort_flag;
+    if (wg < 2) {
+        // ================================ softmax ================================
+        regs_more<184>();
+        const int X = wg, row = threadIdx.x & 127, lanebase = (warp & 3) * 32;
+        const uint32_t toff = (uint32_t)lanebase << 16, sx = tS + 128 * X + toff, ox = tO + 128 * X + toff;
+        uint32_t step = 0, joins = 0;            // steps of this X, meetings of the two groups so far
+        bool ok = true;
+        auto meet = [&]() {                      // both groups (bounded, unlike a named barrier)
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.joined);
+            return __all_sync(0xffffffffu, mbar_wait(&bars.joined, joins++ & 1, abort_flag, a.status));
+        };
+        int nseg = 0;
+        for (; w.more() && ok; w.next(a), ++nseg) {
+            const int r = w.at.rt * RT + (HL ? 0 : 128 * X) + row, live_rows = w.sq.nq * a.G;
+            const bool live = r < live_rows;
+            const int tok = live ? div_g(a, r) : 0, head = w.at.kvh * a.G + r - tok * a.G;
+            const int lim = live ? min(w.sq.len, w.sq.len - w.sq.nq + tok + 1) : 0;
+            // ---- q: this row's halves into the swizzled K-major tiles (HL: both groups, half of the dims each) ----
+            {
+                const T *qp = static_cast<const T *>(a.q) + (long)(w.sq.q0 + tok) * a.qs + (long)head * D;
+                uint8_t *qs = sm + (HL ? 0 : X * P::QT) + row * 128;
+#pragma unroll
+                for (int i = 0; i < (HL ? D / 16 : D / 8); ++i) {
+                    const int ch = HL ? X * (D / 16) + i : i;    // 8 dims
+                    uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
+                    if (live) {
+                        if constexpr (HL) {
+                            const float4 x = *reinterpret_cast<const float4 *>(qp + ch * 8), y = *reinterpret_cast<const float4 *>(qp + ch * 8 + 4);
+                            split2(x.x, x.y, hi.x, lo.x), split2(x.z, x.w, hi.y, lo.y);
+                            split2(y.x, y.y, hi.z, lo.z), split2(y.z, y.w, hi.w, lo.w);
+                        } else {
+                            hi = *reinterpret_cast<const uint4 *>(qp + ch * 8);
+                        }
+                    }
+                    uint8_t *at = qs + (ch >> 3) * P::SUB + (((ch & 7) ^ (row & 7)) << 4);
+                    *reinterpret_cast<uint4 *>(at) = as_eight(hi);
+                    if constexpr (HL) *reinterpret_cast<uint4 *>(at + P::QT) = as_eight(lo);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars.q_full);
+            }
+            const int *trow = a.tab.page + (long)w.at.b * a.tab.stride;
+            bool hole = false;                   // pages out of range among the segment's
+            {
+                const int ps = a.pool.page_shift, e0 = (w.c0 * kKeys) >> ps, e1 = (min(w.c1 * kKeys, w.sq.len) + (1 << ps) - 1) >> ps;
+                for (int i = e0 + lane; i < e1; i += 32) hole = hole || (unsigned)__ldg(trow + i) >= (unsigned)a.pool.n_pages;
+                hole = __any_sync(0xffffffffu, hole);
+                if (hole && lane == 0) atomicCAS(a.status, 0, X100_E_ARG);
+            }
+            float m = -INFINITY, nm = 0.f, l = 0.f;
+            bool any = false;                    // O holds sums
+            for (int c = w.c0 + (HL ? X : 0); c < w.c1; c += HL ? 2 : 1, ++step) {
+                const int p0 = c * kKeys;
+                ok = __all_sync(0xffffffffu, mbar_wait(&bars.s_full[X], step & 1, abort_flag, a.status));
+                if (!ok) break;
+                tc_fence_after();
+                float s[128];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) tmem_ld32(sx + 32 * i, *reinterpret_cast<uint32_t(*)[32]>(s + 32 * i));
+                tmem_wait_ld();
+                if (__any_sync(0xffffffffu, p0 + kKeys > lim) || hole) {
+                    const int cut = lim - p0;
+#pragma unroll
+                    for (int i = 0; i < 128; ++i)
+                        if (i >= cut) s[i] = -INFINITY;
+                    if (hole) {
+                        uint32_t gone = 0;
+                        for (int i = 0; i < 8 && p0 + 16 * i < w.sq.len; ++i)
+                            if ((unsigned)__ldg(trow + ((p0 + 16 * i) >> a.pool.page_shift)) >= (unsigned)a.pool.n_pages) gone |= 1u << i;
+#pragma unroll
+                        for (int i = 0; i < 128; ++i)
+                            if (gone >> (i / 16) & 1) s[i] = -INFINITY;
+                    }
+                }
+                float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                for (int i = 4; i < 128; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.sl;
+                if (__any_sync(0xffffffffu, top > m + 8.f)) {
+                    const float mn = fmaxf(m, top), f = mn == -INFINITY ? 1.f : ex2(m - mn);
+                    m = mn;
+                    nm = mn == -INFINITY ? 0.f : -mn;
+                    l *= f;
+                    if (any) {
+                        ok = __all_sync(0xffffffffu, mbar_wait(&bars.o_done[X], (step - 1) & 1, abort_flag, a.status));
+                        if (!ok) break;
+                        tc_fence_after();
+#pragma unroll
+                        for (int i = 0; i < D / 16; ++i) {
+                            uint32_t v[16];
+                            tmem_ld16(ox + 16 * i, v);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * f);
+                            tmem_st16(ox + 16 * i, v);
+                        }
+                    }
+                }
+                any = true;
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t hi[16], lo[16];
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        const float x = ex2(fmaf(s[32 * i + 2 * k], a.sl, nm)), y = ex2(fmaf(s[32 * i + 2 * k + 1], a.sl, nm));
+                        sum[k & 3] += x + y;
+                        if constexpr (HL) split2(x, y, hi[k], lo[k]);
+                        else hi[k] = u32(__floats2half2_rn(x, y));
+                    }
+                    tmem_st16(sx + 16 * i, hi);
+                    if constexpr (HL) tmem_st16(sx + 64 + 16 * i, lo);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars.p_ready[X]);
+            }
+            if (!ok) break;
+            // ---- out ----
+            if (any) {
+                ok = __all_sync(0xffffffffu, mbar_wait(&bars.o_done[X], (step - 1) & 1, abort_flag, a.status));
+                if (!ok) break;
+                tc_fence_after();
+            }
+            float f = 1.f;
+            if constexpr (HL) {
+                // join the two groups: group 1 leaves its scaled sums where q was (the products that read q are done
+                // when both groups' last step is), group 0 adds them to its own
+                bars.ml[X][row] = make_float2(m, l);
+                ok = meet();
+                if (!ok) break;
+                const float2 other = bars.ml[X ^ 1][row];
+                const float M = fmaxf(m, other.x);
+                f = M == -INFINITY ? 0.f : ex2(m - M);
+                l = l * f + (M == -INFINITY ? 0.f : other.y * ex2(other.x - M));
+                m = M;
+                float4 *sums = reinterpret_cast<float4 *>(sm) + row;
+                if (X == 1) {
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) {
+                        uint32_t v[16];
+                        if (any) {
+                            tmem_ld16(ox + 16 * i, v);
+                            tmem_wait_ld();
+                        }
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            sums[(4 * i + k) * 128] = any ? make_float4(__uint_as_float(v[4 * k]) * f, __uint_as_float(v[4 * k + 1]) * f,
+                                                                        __uint_as_float(v[4 * k + 2]) * f, __uint_as_float(v[4 * k + 3]) * f)
+                                                          : make_float4(0.f, 0.f, 0.f, 0.f);
+                    }
+                }
+                ok = meet();
+                if (!ok) break;
+            }
+            const bool whole = w.c0 == 0 && w.c1 == w.cu;
+            if (!HL || X == 0) {
+                const int slot = (int)blockIdx.x * 2 + (nseg ? 1 : 0), prow = HL ? row : 128 * X + row;
+                const float inv = whole ? (l > 0.f ? 1.f / l : 0.f) : 1.f;
+                const float4 *sums = reinterpret_cast<const float4 *>(sm) + row;
+                T *op = static_cast<T *>(a.out) + (long)(w.sq.q0 + tok) * a.os + (long)head * D;
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    uint32_t v[16];
+                    tmem_ld16(ox + 16 * i, v);
+                    tmem_wait_ld();
+                    float o[16];
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) o[k] = __uint_as_float(v[k]) * f;
+                    if constexpr (HL) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const float4 x = sums[(4 * i + k) * 128];
+                            o[4 * k] += x.x, o[4 * k + 1] += x.y, o[4 * k + 2] += x.z, o[4 * k + 3] += x.w;
+                        }
+                    }
+                    if (!whole) {
+                        float4 *pp = reinterpret_cast<float4 *>(a.part) + (long)slot * kPfRows * (D / 4) + prow;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) pp[(4 * i + k) * kPfRows] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+                    } else if (live) {
+                        // columns 0 .. 7 of a group of 8 are its dims 0, 4, 1, 5, 2, 6, 3, 7
+#pragma unroll
+                        for (int h = 0; h < 16; h += 8) {
+                            const float y[8] = {o[h] * inv, o[h + 2] * inv, o[h + 4] * inv, o[h + 6] * inv,
+                                                o[h + 1] * inv, o[h + 3] * inv, o[h + 5] * inv, o[h + 7] * inv};
+                            if constexpr (HL) {
+                                *reinterpret_cast<float4 *>(op + 16 * i + h) = make_float4(y[0], y[1], y[2], y[3]);
+                                *reinterpret_cast<float4 *>(op + 16 * i + h + 4) = make_float4(y[4], y[5], y[6], y[7]);
+                            } else {
+                                *reinterpret_cast<uint4 *>(op + 16 * i + h) =
+                                    make_uint4(u32(__floats2half2_rn(y[0], y[1])), u32(__floats2half2_rn(y[2], y[3])),
+                                               u32(__floats2half2_rn(y[4], y[5])), u32(__floats2half2_rn(y[6], y[7])));
+                            }
+                        }
+                    }
+                }
+                if (!whole) {
+                    a.ml[(long)slot * kPfRows + prow] = make_float2(m, l);
+                    if (X == 0 && row == 0) a.meta[slot] = make_int4((int)w.at.item, w.at.b, w.at.kvh, w.at.rt | (w.c0 ? kInside : 0));
+                }
+            }
+            if constexpr (HL) ok = meet();          // group 0 has read the sums: q may come again
+            tc_fence_before();                      // the next step's products overwrite S and O
+        }
+        if (!ok) *abort_flag = 1;
+    } else if (wg == 2) {
+        // ================================ codes -> fp16 tiles ================================
+        regs_less<96>();
+        const Exponents expo;
+        const int th = threadIdx.x - 256;
+        uint32_t tile = 0, raw = 0;                // key tiles, raw stages so far
+        bool ok = true;
+        for (; w.more() && ok; w.next(a)) {
+            for (int c = w.c0; c < w.c1 && ok; ++c, ++tile) {
+                const uint32_t st = tile & 1, par = (tile >> 1 & 1) ^ 1;
+                uint8_t *kt = sm + P::K0 + st * P::KT, *vt = sm + P::V0 + st * P::KT;
+                // all of K first: its products come a step ahead of V's
+                ok = __all_sync(0xffffffffu, mbar_wait(&bars.k_empty[st], par, abort_flag, a.status));
+                if (!ok) break;
+                for (int half = 0; half < 2; ++half) {
+                    const uint32_t rs = (raw + half) % kRawStages;
+                    ok = __all_sync(0xffffffffu, mbar_wait(&bars.raw_full[rs], (raw + half) / kRawStages & 1, abort_flag, a.status));
+                    if (!ok) break;
+                    const uint8_t *rp = sm + P::RAW0 + rs * P::RAW;
+                    const uint32_t have = bars.raw_ok[rs];
+                    const int left = w.sq.len - c * kKeys - half * 64;   // positions of the sequence from here
+                    // 4 lanes per position, a word of every block each
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int key = i * 32 + (th >> 2), t = th & 3, in = key & 15, kk = half * 64 + key;
+                        const uint8_t *tp = rp + (key >> 4) * L::BYTES;
+                        const bool on = (have >> (key >> 4) & 1) && key < left;
+                        uint32_t kw[L::NB];
+                        __half kd[L::NB];
+                        if constexpr (D == 128) {
+                            *reinterpret_cast<uint4 *>(kw) = *reinterpret_cast<const uint4 *>(tp + L::k_word(in, 0, t));
+                            *reinterpret_cast<uint2 *>(kd) = *reinterpret_cast<const uint2 *>(tp + L::k_scale(in, 0));
+                        } else {
+                            *reinterpret_cast<uint2 *>(kw) = *reinterpret_cast<const uint2 *>(tp + L::k_word(in, 0, t));
+                            *reinterpret_cast<uint32_t *>(kd) = *reinterpret_cast<const uint32_t *>(tp + L::k_scale(in, 0));
+                        }
+#pragma unroll
+                        for (int b = 0; b < L::NB; ++b) {
+                            const __half2 d = __half2half2(on ? kd[b] : __ushort_as_half(0));
+                            *reinterpret_cast<uint4 *>(kt + (b >> 1) * P::SUB + kk * 128 + ((((b & 1) * 4 + t) ^ (kk & 7)) << 4)) = eight(kw[b], d, expo);
+                        }
+                    }
+                }
+                if (!ok) break;
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars.k_full[st]);
+                ok = __all_sync(0xffffffffu, mbar_wait(&bars.v_empty[st], par, abort_flag, a.status));
+                if (!ok) break;
+                for (int half = 0; half < 2; ++half, ++raw) {
+                    const uint32_t rs = raw % kRawStages;
+                    const uint8_t *rp = sm + P::RAW0 + rs * P::RAW;
+                    const uint32_t have = bars.raw_ok[rs];
+                    const int left = w.sq.len - c * kKeys - half * 64;
+                    // a lane has the D / 8 dims from g * D / 8 of positions t + 4 m
+#pragma unroll
+                    for (int i = 0; i < (D == 128 ? 2 : 1); ++i) {
+                        const int tl = th >> 5, g = lane >> 2, t = lane & 3;
+                        const uint8_t *tp = rp + tl * L::BYTES;
+                        const bool on = have >> tl & 1;
+                        const uint4 x = *reinterpret_cast<const uint4 *>(tp + L::V0 + i * 512 + lane * 16);
+                        const uint32_t vw[4] = {x.x, x.y, x.z, x.w};
+                        __half vd[4];
+                        *reinterpret_cast<uint2 *>(vd) = *reinterpret_cast<const uint2 *>(tp + L::v_scale(t, g * (D / 8) / 32));
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            // D = 128: words 2 q, 2 q + 1 of position t + 4 (2 i + q); D = 64: word q of position t + 4 q
+                            const int m = D == 128 ? 2 * i + (k >> 1) : k, key = tl * 16 + 4 * m + t, kk = half * 64 + key;
+                            const int dim = g * (D / 8) + (D == 128 ? (k & 1) * 8 : 0);
+                            const __half2 d = __half2half2(on && key < left ? vd[m] : __ushort_as_half(0));
+                            *reinterpret_cast<uint4 *>(vt + (dim >> 6) * P::SUB + kk * 128 + ((((dim & 63) >> 3) ^ (kk & 7)) << 4)) = eight(vw[k], d, expo);
+                        }
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bars.raw_empty[rs]);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars.v_full[st]);
+            }
+        }
+        if (!ok) *abort_flag = 1;
+    } else {
+        regs_less<40>();
+        if (warp == 12 && lane == 0) {
+            // ================================ products ================================
+            const uint32_t idS = idesc_make(1, 0, 0, 128, 128), idO = idesc_make(1, 0, 1, 128, D);
+            // matrix descriptors; tiles and slices of them differ in the address field (16-byte steps) alone
+            const uint64_t descQ = smem_desc_sw128(smem_u32(sm), 16, 1024), descK = smem_desc_sw128(smem_u32(sm + P::K0), 16, 1024);
+            const uint64_t descV = smem_desc_sw128(smem_u32(sm + P::V0), P::SUB, 1024);
+            uint32_t tile = 0, step[2] = {0, 0}, seg = 0;
+            bool ok = true;
+            for (; w.more() && ok; w.next(a), ++seg) {
+                const int S = HL ? w.n : 2 * w.n;
+                ok = mbar_wait(&bars.q_full, seg & 1, abort_flag, a.status);
+                if (!ok) break;
+                tc_fence_after();
+                auto scores = [&](int s) {
+                    const int X = s & 1;
+                    const uint32_t tl = tile + (HL ? s : s >> 1), st = tl & 1;
+                    if (HL || X == 0) {
+                        if (!mbar_wait(&bars.k_full[st], tl >> 1 & 1, abort_flag, a.status)) return false;
+                        tc_fence_after();
+                    }
+                    const uint64_t qd = descQ + (HL ? 0 : X * (P::QT >> 4)), kd = descK + st * (P::KT >> 4);
+#pragma unroll
+                    for (int p = 0; p < (HL ? 2 : 1); ++p)
+#pragma unroll
+                        for (int k = 0; k < KS; ++k) {
+                            const uint32_t off = ((k >> 2) * P::SUB + (k & 3) * 32) >> 4;
+                            umma_f16(tS + 128 * X, qd + p * (P::QT >> 4) + off, kd + off, idS, (p | k) ? 1u : 0u);
+                        }
+                    umma_commit(&bars.s_full[X]);
+                    if (HL || X == 1) umma_commit(&bars.k_empty[st]);
+                    return true;
+                };
+                for (int s = 0; s < 2 && s < S && ok; ++s) ok = scores(s);
+                uint32_t first = 3;                 // bit X: O of X has no sums yet
+                for (int s = 0; s < S && ok; ++s) {
+                    const int X = s & 1;
+                    const uint32_t tl = tile + (HL ? s : s >> 1), st = tl & 1;
+                    ok = mbar_wait(&bars.p_ready[X], step[X] & 1, abort_flag, a.status);
+                    if (ok && (HL || X == 0)) ok = mbar_wait(&bars.v_full[st], tl >> 1 & 1, abort_flag, a.status);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint64_t vd = descV + st * (P::KT >> 4);
+                    const uint32_t more = first >> X & 1 ? 0u : 1u;
+#pragma unroll
+                    for (int p = 0; p < (HL ? 2 : 1); ++p)
+#pragma unroll
+                        for (int k = 0; k < VS; ++k)
+                            umma_f16_ts(tO + 128 * X, tS + 128 * X + 64 * p + 8 * k, vd + k * (2048 >> 4), idO, (p | k) ? 1u : more);
+                    first &= ~(1u << X);
+                    ++step[X];
+                    umma_commit(&bars.o_done[X]);
+                    if (HL || X == 1) umma_commit(&bars.v_empty[st]);
+                    if (s + 2 < S) ok = scores(s + 2);
+                }
+                tile += w.n;
+            }
+            if (!ok) *abort_flag = 1;
+            umma_commit(&bars.drain);               // every product issued has ended when this completes
+            mbar_wait_drain(&bars.drain, 0, kWaitLimitNs);
+        } else if (warp == 13) {
+            // ================================ raw tiles ================================
+            uint32_t raw = 0;
+            bool ok = true;
+            const int ps = a.pool.page_shift;
+            const long page_step = a.pool.page_bytes * a.pool.nkv;
+            for (; w.more() && ok; w.next(a)) {
+                const int *trow = a.tab.page + (long)w.at.b * a.tab.stride;
+                const uint8_t *base = a.pool.pages + (long)w.at.kvh * a.pool.page_bytes;
+                for (int h = 2 * w.c0; h < 2 * w.c1 && ok; ++h, ++raw) {
+                    const uint32_t rs = raw % kRawStages;
+                    const int pos = h * 64 + lane * 16;
+                    const int page = lane < 4 && pos < w.sq.len ? __ldg(trow + (pos >> ps)) : -1;
+                    const bool on = (unsigned)page < (unsigned)a.pool.n_pages;
+                    const uint32_t have = __ballot_sync(0xffffffffu, on);
+                    ok = __all_sync(0xffffffffu, mbar_wait(&bars.raw_empty[rs], (raw / kRawStages & 1) ^ 1, abort_flag, a.status));
+                    if (!ok) break;
+                    if (lane == 0) {
+                        bars.raw_ok[rs] = have;
+                        mbar_arrive_expect_tx(&bars.raw_full[rs], __popc(have) * L::BYTES);
+                    }
+                    __syncwarp();
+                    if (on)
+                        bulk_load(sm + P::RAW0 + rs * P::RAW + lane * L::BYTES, base + page * page_step + ((pos & ((1 << ps) - 1)) >> 4) * L::BYTES, L::BYTES,
+                                  &bars.raw_full[rs]);
+                }
+            }
+            if (!ok) {                              // let the copies in flight land before the CTA ends
+                *abort_flag = 1;
+                if (lane == 0)
+                    for (uint32_t i = raw > kRawStages ? raw - kRawStages : 0; i < raw; ++i)
+                        mbar_wait_drain(&bars.raw_full[i % kRawStages], i / kRawStages & 1, kWaitLimitNs);
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12) tmem_dealloc(tmem, 512);
+}
+
+// Joins the parts of an item at the first cut inside it (as merge_kernel in kv4_attn.cu): a thread per row, 16 columns per CTA.
+template <typename T, int D>
+__global__ void __launch_bounds__(kPfRows) prefill_merge_kernel(const AttnArgs a, int grid) {
+    constexpr int RT = sizeof(T) == 4 ? 128 : 256;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int c = blockIdx.x + 1, col = blockIdx.y * 16, row = threadIdx.x;
+    const int4 here = __ldcg(a.meta + 2 * c), p0 = __ldcg(a.meta + 2 * c - 2), p1 = __ldcg(a.meta + 2 * c - 1);
+    if (here.x == -1 || !(here.w & kInside)) return;
+    int slot0 = 2 * c - 1;
+    if (p1.x != here.x) {
+        if (p0.x != here.x || (p0.w & kInside)) return;
+        slot0 = 2 * c - 2;
+    }
+    const int b = here.y, rt = here.w & (kInside - 1), r = rt * RT + row;
+    const int q0 = a.q_start ? a.q_start[b] : b, nq = a.q_start ? a.q_start[b + 1] - q0 : 1;
+    if (row >= RT || r >= nq * a.G) return;
+    float m = -INFINITY, l = 0.f, o[16] = {};
+    for (int i = c - 1; i < grid; ++i) {
+        if (i > c) {
+            const int4 x = __ldcg(a.meta + 2 * i);
+            if (x.x != here.x || !(x.w & kInside)) break;
+        }
+        const long slot = i == c - 1 ? slot0 : 2 * i;
+        const float2 ml = __ldcg(a.ml + slot * kPfRows + row);
+        const float4 *pp = reinterpret_cast<const float4 *>(a.part) + (slot * (D / 4) + col / 4) * kPfRows + row;
+        float4 v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = __ldcg(pp + k * kPfRows);
+        const float mn = fmaxf(m, ml.x), f = mn == -INFINITY ? 0.f : ex2(m - mn), g = mn == -INFINITY ? 0.f : ex2(ml.x - mn);
+        m = mn;
+        l = l * f + ml.y * g;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            o[4 * k] = o[4 * k] * f + v[k].x * g, o[4 * k + 1] = o[4 * k + 1] * f + v[k].y * g;
+            o[4 * k + 2] = o[4 * k + 2] * f + v[k].z * g, o[4 * k + 3] = o[4 * k + 3] * f + v[k].w * g;
+        }
+    }
+    const int tok = div_g(a, r);
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    T *op = static_cast<T *>(a.out) + (long)(q0 + tok) * a.os + (long)(here.z * a.G + r - tok * a.G) * D + col;
+#pragma unroll
+    for (int h = 0; h < 16; h += 8) {
+        const float y[8] = {o[h] * inv, o[h + 2] * inv, o[h + 4] * inv, o[h + 6] * inv, o[h + 1] * inv, o[h + 3] * inv, o[h + 5] * inv, o[h + 7] * inv};
+        if constexpr (sizeof(T) == 4) {
+            *reinterpret_cast<float4 *>(op + h) = make_float4(y[0], y[1], y[2], y[3]);
+            *reinterpret_cast<float4 *>(op + h + 4) = make_float4(y[4], y[5], y[6], y[7]);
+        } else {
+            *reinterpret_cast<uint4 *>(op + h) = make_uint4(u32(__floats2half2_rn(y[0], y[1])), u32(__floats2half2_rn(y[2], y[3])),
+                                                            u32(__floats2half2_rn(y[4], y[5])), u32(__floats2half2_rn(y[6], y[7])));
+        }
+    }
+}
+
+size_t prefill_work(int head_dim) {
+    return (size_t)kPfCtas * 2 * (kPfRows * (head_dim + 2) * sizeof(float) + sizeof(int4));
+}
+
+template <typename T, int D>
+static int launch_pf(DevCtx *c, AttnArgs &a, cudaStream_t s) {
+    constexpr int RT = sizeof(T) == 4 ? 128 : 256;
+    static bool attr[64];
+    if (!attr[c->device]) {
+        set_qkernel_attrs(prefill_kernel<T, D>, Pf<D>::SMEM);
+        attr[c->device] = true;
+    }
+    const long items = (long)a.tab.n_seqs * a.pool.nkv * (((long)a.max_q * a.G + RT - 1) / RT);
+    const long cover = std::min(0x7fffffffl, (long)a.tab.stride << a.pool.page_shift);
+    const long most = std::min<long>(items, kPfCtas) * (cover / kKeys + 1);
+    const int grid = (int)std::min<long>(std::min(kPfCtas, c->sm_count), most);
+    a.ml = reinterpret_cast<float2 *>(a.part + (size_t)kPfCtas * 2 * kPfRows * D);
+    a.meta = reinterpret_cast<int4 *>(a.ml + kPfCtas * 2 * kPfRows);
+    a.unit_shift = 7;
+    int st = launch_pdl(prefill_kernel<T, D>, dim3(grid), dim3(kPfThreads), Pf<D>::SMEM, s, a);
+    if (st || grid == 1) return st;
+    return launch_pdl(prefill_merge_kernel<T, D>, dim3(grid - 1, D / 16), dim3(kPfRows), 0, s, a, grid);
+}
+
+int launch_prefill(DevCtx *c, AttnArgs &a, int dtype, int head_dim, cudaStream_t s) {
+    if (dtype == X100Q_F32) return head_dim == 128 ? launch_pf<float, 128>(c, a, s) : launch_pf<float, 64>(c, a, s);
+    return head_dim == 128 ? launch_pf<__half, 128>(c, a, s) : launch_pf<__half, 64>(c, a, s);
+}
+
+}  // namespace kv4
+}  // namespace x100
