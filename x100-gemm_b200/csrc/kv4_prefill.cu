@@ -9,6 +9,7 @@
 //   warps 8-11       raw codes in shared memory -> fp16 K and V tiles in the 128-byte-swizzled
 //                    layouts the MMA reads; scale * (code - 8) is an fp16 value, so exact
 //   warp 12          issues the MMAs;  warp 13  copies the raw tiles (bulk copies)
+//   warp 14          walks the work list and hands every role its segments through shared memory
 // fp16 q: the steps X are two row tiles over the same key tile (256 rows per item), so that
 // a key tile is unpacked once for both.  fp32 q: q and P are carried as hi + lo halves, two
 // products each, and the steps X are every other key tile of one row tile, joined at the end.
@@ -38,22 +39,29 @@ struct Pf {
 };
 
 // ---- tcgen05 pieces that ptx.cuh lacks --------------------------------------------
-__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
+// Issued by the lane whose `lead` is not zero, from code that the whole warp runs: the descriptors then are
+// warp-uniform values in uniform registers.  (With one lane in a branch of its own each of them is moved there
+// for every instruction, and the products waited for their issue: 140 cycles per 128 x 128 x 16 instead of 64.)
+__device__ __forceinline__ void umma_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t acc, uint32_t lead) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(acc)
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc), "r"(lead)
         : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *r) {
+// A from tensor memory
+__device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t acc, uint32_t lead) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(acc), "r"(lead)
+        : "memory");
+}
+__device__ __forceinline__ void umma_commit_lead(uint64_t *bar, uint32_t lead) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+        "r"(lead)
         : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r) {
@@ -77,8 +85,11 @@ __device__ __forceinline__ int seen(const AttnArgs &a, const Seq &s, int rt) {
     const int rows = min(RT, s.nq * a.G - rt * RT);
     return max(0, min(s.len, s.len - s.nq + div_g(a, rt * RT + rows - 1) + 1));
 }
+// Units of a row tile in the list: its key tiles, and kLead more for what an item costs besides (q in, sums out),
+// so that runs of many short items do not take longer than the others.
+constexpr int kLead = 2;
 template <int RT>
-__device__ __forceinline__ int units_of(const AttnArgs &a, const Seq &s, int rt) { return max(1, (seen<RT>(a, s, rt) + kKeys - 1) / kKeys); }
+__device__ __forceinline__ int units_of(const AttnArgs &a, const Seq &s, int rt) { return kLead + max(1, (seen<RT>(a, s, rt) + kKeys - 1) / kKeys); }
 // Units of one kv head of a sequence; by one whole warp.
 template <int RT>
 __device__ __forceinline__ uint32_t head_units(const AttnArgs &a, const Seq &s) {
@@ -134,49 +145,23 @@ __device__ __forceinline__ Start my_start(const AttnArgs &a) {
         }
     }
 }
-// The segments of a run, one item (or a part of one) after the other.  Every role walks them by itself.
-template <int RT>
-struct Walk {
-    Start at;
-    Seq sq;
-    uint32_t u;
-    int cu, c0, c1, n;                     // units of the item; those of this segment; their number
-    __device__ Walk(const AttnArgs &a, const Start &s) : at(s), u(s.u0) {
-        if (u < at.u1) {
-            sq = load_seq(a, at.b, RT, false);
-            set(a);
-        }
-    }
-    __device__ bool more() const { return u < at.u1; }
-    __device__ void set(const AttnArgs &a) {
-        cu = units_of<RT>(a, sq, at.rt);
-        c0 = (int)(u - at.item);
-        c1 = (int)min((uint32_t)cu, (uint32_t)c0 + (at.u1 - u));
-        n = c1 - c0;
-    }
-    __device__ void next(const AttnArgs &a) {
-        u += n;
-        if (u >= at.u1) return;
-        at.item += cu;
-        if (++at.rt == sq.nrt) {
-            at.rt = 0;
-            if (++at.kvh == a.pool.nkv) {
-                at.kvh = 0;
-                do sq = load_seq(a, ++at.b, RT, false);
-                while (!sq.nrt);
-            }
-        }
-        set(a);
-    }
+// A segment: key tiles c0 .. c1 - 1 of an item (all cu of them, or a part).
+struct Seg {
+    int n;                                 // c1 - c0; 0: the run is over
+    int c0, cu, b, kvh, rt, q0, nq, len;
+    uint32_t item;                         // the item's first unit
 };
+constexpr int kSegs = 4, kRoles = 14;      // ring of segments; warps that read one
 
+// Barriers that a step's MMAs signal come in pairs, the step's parity choosing one, so that the one for key tile k is
+// also what frees that tile's stage (fp16 q, X = 1) and the issuing warp commits only twice a step.
 struct PfBars {
     uint64_t raw_full[kRawStages], raw_empty[kRawStages], k_full[2], k_empty[2], v_full[2], v_empty[2];
-    uint64_t s_full[2], p_ready[2], o_done[2], q_full, joined, drain;
+    uint64_t s_full[2][2], p_ready[2], o_done[2][2], q_full, q_empty, joined, drain, seg_full[kSegs], seg_empty[kSegs];
     uint32_t raw_ok[kRawStages];           // bit i: 16-position tile i of the raw stage was copied
     uint32_t tmem;
     int abort_flag;
-    Start start;
+    Seg seg[kSegs];
     float2 ml[2][128];
 };
 
@@ -190,6 +175,20 @@ __device__ __forceinline__ uint4 eight(uint32_t w, __half2 d, const Exponents &x
 // The query order that goes with it: the halves of 8 dims (a.x = dims 0, 1 ..) as 0, 4, 1, 5, 2, 6, 3, 7
 __device__ __forceinline__ uint4 as_eight(uint4 a) {
     return make_uint4(__byte_perm(a.x, a.z, 0x5410), __byte_perm(a.x, a.z, 0x7632), __byte_perm(a.y, a.w, 0x5410), __byte_perm(a.y, a.w, 0x7632));
+}
+
+// x * a + b for two floats at once
+__device__ __forceinline__ void fma2(float &x, float &y, uint64_t a, uint64_t b) {
+    asm("{\n\t.reg .b64 t;\n\tmov.b64 t, {%0, %1};\n\tfma.rn.f32x2 t, t, %2, %3;\n\tmov.b64 {%0, %1}, t;\n\t}" : "+f"(x), "+f"(y) : "l"(a), "l"(b));
+}
+__device__ __forceinline__ uint64_t both(float x) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %1};" : "=l"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t s, float x, float y) {
+    asm("{\n\t.reg .b64 t;\n\tmov.b64 t, {%1, %2};\n\tadd.rn.f32x2 %0, %0, t;\n\t}" : "+l"(s) : "f"(x), "f"(y));
+    return s;
 }
 
 template <typename T, int D>
@@ -206,12 +205,14 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const AttnArgs a
     if (threadIdx.x == 0) {
         bars.abort_flag = 0;
         for (int i = 0; i < kRawStages; ++i) mbar_init(&bars.raw_full[i], 1), mbar_init(&bars.raw_empty[i], kDqWarps);
+        for (int i = 0; i < kSegs; ++i) mbar_init(&bars.seg_full[i], 1), mbar_init(&bars.seg_empty[i], kRoles);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bars.k_full[i], kDqWarps), mbar_init(&bars.k_empty[i], 1);
             mbar_init(&bars.v_full[i], kDqWarps), mbar_init(&bars.v_empty[i], 1);
-            mbar_init(&bars.s_full[i], 1), mbar_init(&bars.p_ready[i], 4), mbar_init(&bars.o_done[i], 1);
+            mbar_init(&bars.p_ready[i], 4);
+            for (int k = 0; k < 2; ++k) mbar_init(&bars.s_full[i][k], 1), mbar_init(&bars.o_done[i][k], 1);
         }
-        mbar_init(&bars.q_full, 8), mbar_init(&bars.joined, 8), mbar_init(&bars.drain, 1);
+        mbar_init(&bars.q_full, 8), mbar_init(&bars.q_empty, 1), mbar_init(&bars.joined, 8), mbar_init(&bars.drain, 1);
         fence_barrier_init();
     }
     if (warp == 12) {
@@ -220,73 +221,86 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const AttnArgs a
     }
     pdl_launch_dependents();
     pdl_wait();
-    if (warp == 0) {
-        const Start s = my_start<RT>(a);
-        if (lane == 0) bars.start = s;
-    }
     if (threadIdx.x >= 32 && threadIdx.x < 34) a.meta[blockIdx.x * 2 + threadIdx.x - 32] = make_int4(-1, 0, 0, 0);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = bars.tmem, tS = tmem, tO = tmem + 256;   // S, O of step X: + 128 X columns
-    Walk<RT> w(a, bars.start);
     volatile int *abort_flag = &bars.abort_flag;
+    auto wait = [&](uint64_t *bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, a.status)); };
+    // the i-th segment; a role reads what it needs of it before release(i)
+    auto segment = [&](uint32_t i) { return wait(&bars.seg_full[i % kSegs], i / kSegs & 1); };
+    auto release = [&](uint32_t i) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.seg_empty[i % kSegs]);
+    };
+    bool ok = true;
     if (wg < 2) {
         // ================================ softmax ================================
-        regs_more<184>();
-        const int X = wg, row = threadIdx.x & 127, lanebase = (warp & 3) * 32;
-        const uint32_t toff = (uint32_t)lanebase << 16, sx = tS + 128 * X + toff, ox = tO + 128 * X + toff;
+        regs_more<176>();
+        const int X = wg, row = threadIdx.x & 127;
+        const uint32_t toff = (uint32_t)((warp & 3) * 32) << 16, sx = tS + 128 * X + toff, ox = tO + 128 * X + toff;
         uint32_t step = 0, joins = 0;            // steps of this X, meetings of the two groups so far
-        bool ok = true;
         auto meet = [&]() {                      // both groups (bounded, unlike a named barrier)
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars.joined);
-            return __all_sync(0xffffffffu, mbar_wait(&bars.joined, joins++ & 1, abort_flag, a.status));
+            return wait(&bars.joined, joins++ & 1);
         };
-        int nseg = 0;
-        for (; w.more() && ok; w.next(a), ++nseg) {
-            const int r = w.at.rt * RT + (HL ? 0 : 128 * X) + row, live_rows = w.sq.nq * a.G;
-            const bool live = r < live_rows;
-            const int tok = live ? div_g(a, r) : 0, head = w.at.kvh * a.G + r - tok * a.G;
-            const int lim = live ? min(w.sq.len, w.sq.len - w.sq.nq + tok + 1) : 0;
-            // ---- q: this row's halves into the swizzled K-major tiles (HL: both groups, half of the dims each) ----
-            {
-                const T *qp = static_cast<const T *>(a.q) + (long)(w.sq.q0 + tok) * a.qs + (long)head * D;
-                uint8_t *qs = sm + (HL ? 0 : X * P::QT) + row * 128;
+        // q of a segment: this row's halves into the swizzled K-major tiles (HL: both groups, half of the dims each)
+        auto put_q = [&](const Seg &v) {
+            const int r = v.rt * RT + (HL ? 0 : 128 * X) + row;
+            const bool on = r < v.nq * a.G;
+            const int tok = on ? div_g(a, r) : 0;
+            const T *qp = static_cast<const T *>(a.q) + (long)(v.q0 + tok) * a.qs + (long)(v.kvh * a.G + r - tok * a.G) * D;
+            uint8_t *qs = sm + (HL ? 0 : X * P::QT) + row * 128;
 #pragma unroll
-                for (int i = 0; i < (HL ? D / 16 : D / 8); ++i) {
-                    const int ch = HL ? X * (D / 16) + i : i;    // 8 dims
-                    uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
-                    if (live) {
-                        if constexpr (HL) {
-                            const float4 x = *reinterpret_cast<const float4 *>(qp + ch * 8), y = *reinterpret_cast<const float4 *>(qp + ch * 8 + 4);
-                            split2(x.x, x.y, hi.x, lo.x), split2(x.z, x.w, hi.y, lo.y);
-                            split2(y.x, y.y, hi.z, lo.z), split2(y.z, y.w, hi.w, lo.w);
-                        } else {
-                            hi = *reinterpret_cast<const uint4 *>(qp + ch * 8);
-                        }
+            for (int i = 0; i < (HL ? D / 16 : D / 8); ++i) {
+                const int ch = HL ? X * (D / 16) + i : i;    // 8 dims
+                uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
+                if (on) {
+                    if constexpr (HL) {
+                        const float4 x = *reinterpret_cast<const float4 *>(qp + ch * 8), y = *reinterpret_cast<const float4 *>(qp + ch * 8 + 4);
+                        split2(x.x, x.y, hi.x, lo.x), split2(x.z, x.w, hi.y, lo.y);
+                        split2(y.x, y.y, hi.z, lo.z), split2(y.z, y.w, hi.w, lo.w);
+                    } else {
+                        hi = *reinterpret_cast<const uint4 *>(qp + ch * 8);
                     }
-                    uint8_t *at = qs + (ch >> 3) * P::SUB + (((ch & 7) ^ (row & 7)) << 4);
-                    *reinterpret_cast<uint4 *>(at) = as_eight(hi);
-                    if constexpr (HL) *reinterpret_cast<uint4 *>(at + P::QT) = as_eight(lo);
                 }
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bars.q_full);
+                uint8_t *at = qs + (ch >> 3) * P::SUB + (((ch & 7) ^ (row & 7)) << 4);
+                *reinterpret_cast<uint4 *>(at) = as_eight(hi);
+                if constexpr (HL) *reinterpret_cast<uint4 *>(at + P::QT) = as_eight(lo);
             }
-            const int *trow = a.tab.page + (long)w.at.b * a.tab.stride;
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.q_full);
+        };
+        uint32_t nseg = 0;
+        ok = segment(0);
+        if (ok && bars.seg[0].n) put_q(bars.seg[0]);
+        for (; ok; ++nseg) {
+            const Seg &w = bars.seg[nseg % kSegs];
+            const int n = w.n;
+            if (n == 0) break;
+            const int *trow = a.tab.page + (long)w.b * a.tab.stride;
+            const int c0 = w.c0, len = w.len;
+            int lim;                             // positions the row sees
+            {
+                const int r = w.rt * RT + (HL ? 0 : 128 * X) + row;
+                lim = r < w.nq * a.G ? min(len, len - w.nq + div_g(a, r) + 1) : 0;
+            }
             bool hole = false;                   // pages out of range among the segment's
             {
-                const int ps = a.pool.page_shift, e0 = (w.c0 * kKeys) >> ps, e1 = (min(w.c1 * kKeys, w.sq.len) + (1 << ps) - 1) >> ps;
+                const int ps = a.pool.page_shift, e0 = (c0 * kKeys) >> ps, e1 = (min((c0 + n) * kKeys, len) + (1 << ps) - 1) >> ps;
                 for (int i = e0 + lane; i < e1; i += 32) hole = hole || (unsigned)__ldg(trow + i) >= (unsigned)a.pool.n_pages;
                 hole = __any_sync(0xffffffffu, hole);
                 if (hole && lane == 0) atomicCAS(a.status, 0, X100_E_ARG);
             }
             float m = -INFINITY, nm = 0.f, l = 0.f;
-            bool any = false;                    // O holds sums
-            for (int c = w.c0 + (HL ? X : 0); c < w.c1; c += HL ? 2 : 1, ++step) {
-                const int p0 = c * kKeys;
-                ok = __all_sync(0xffffffffu, mbar_wait(&bars.s_full[X], step & 1, abort_flag, a.status));
+            const bool any = !HL || X < n;       // this group has steps
+            const uint64_t sl2 = both(a.sl);
+            for (int c = HL ? X : 0; c < n; c += HL ? 2 : 1, ++step) {
+                const int p0 = (c0 + c) * kKeys;
+                ok = wait(&bars.s_full[X][step & 1], step >> 1 & 1);
                 if (!ok) break;
                 tc_fence_after();
                 float s[128];
@@ -300,7 +314,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const AttnArgs a
                         if (i >= cut) s[i] = -INFINITY;
                     if (hole) {
                         uint32_t gone = 0;
-                        for (int i = 0; i < 8 && p0 + 16 * i < w.sq.len; ++i)
+                        for (int i = 0; i < 8 && p0 + 16 * i < len; ++i)
                             if ((unsigned)__ldg(trow + ((p0 + 16 * i) >> a.pool.page_shift)) >= (unsigned)a.pool.n_pages) gone |= 1u << i;
 #pragma unroll
                         for (int i = 0; i < 128; ++i)
@@ -309,15 +323,19 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const AttnArgs a
                 }
                 float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                for (int i = 4; i < 128; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
+                for (int i = 4; i < 124; i += 8)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) mx[k] = fmaxf(fmaxf(mx[k], s[i + k]), s[i + 4 + k]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], s[124 + k]);
                 const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.sl;
                 if (__any_sync(0xffffffffu, top > m + 8.f)) {
                     const float mn = fmaxf(m, top), f = mn == -INFINITY ? 1.f : ex2(m - mn);
                     m = mn;
                     nm = mn == -INFINITY ? 0.f : -mn;
                     l *= f;
-                    if (any) {
-                        ok = __all_sync(0xffffffffu, mbar_wait(&bars.o_done[X], (step - 1) & 1, abort_flag, a.status));
+                    if (c >= (HL ? 2 : 1)) {     // O holds sums
+                        ok = wait(&bars.o_done[X][(step - 1) & 1], (step - 1) >> 1 & 1);
                         if (!ok) break;
                         tc_fence_after();
 #pragma unroll
@@ -331,137 +349,139 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const AttnArgs a
                         }
                     }
                 }
-                any = true;
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                const uint64_t nm2 = both(nm);
+                uint64_t sum[2] = {0ull, 0ull};   // two floats each
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     uint32_t hi[16], lo[16];
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
-                        const float x = ex2(fmaf(s[32 * i + 2 * k], a.sl, nm)), y = ex2(fmaf(s[32 * i + 2 * k + 1], a.sl, nm));
-                        sum[k & 3] += x + y;
+                        float x = s[32 * i + 2 * k], y = s[32 * i + 2 * k + 1];
+                        fma2(x, y, sl2, nm2);
+                        x = ex2(x), y = ex2(y);
+                        sum[k & 1] = add2(sum[k & 1], x, y);
                         if constexpr (HL) split2(x, y, hi[k], lo[k]);
                         else hi[k] = u32(__floats2half2_rn(x, y));
                     }
                     tmem_st16(sx + 16 * i, hi);
                     if constexpr (HL) tmem_st16(sx + 64 + 16 * i, lo);
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                {
+                    float s0, s1, s2, s3;
+                    asm("mov.b64 {%0, %1}, %2;" : "=f"(s0), "=f"(s1) : "l"(sum[0]));
+                    asm("mov.b64 {%0, %1}, %2;" : "=f"(s2), "=f"(s3) : "l"(sum[1]));
+                    l += (s0 + s1) + (s2 + s3);
+                }
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bars.p_ready[X]);
             }
             if (!ok) break;
-            // ---- out ----
-            if (any) {
-                ok = __all_sync(0xffffffffu, mbar_wait(&bars.o_done[X], (step - 1) & 1, abort_flag, a.status));
-                if (!ok) break;
-                tc_fence_after();
+            // ---- the next segment's q, as soon as the products have read this one's: its first scores then come
+            // while the sums go out ----
+            ok = segment(nseg + 1);
+            if (ok && bars.seg[(nseg + 1) % kSegs].n) {
+                ok = wait(&bars.q_empty, nseg & 1);
+                if (ok) put_q(bars.seg[(nseg + 1) % kSegs]);
             }
-            float f = 1.f;
+            // ---- out ----
+            if (ok && any) ok = wait(&bars.o_done[X][(step - 1) & 1], (step - 1) >> 1 & 1);
+            // HL: each group puts half of the dims out, of its own sums and of the other's (the same lanes of tensor memory)
+            float f = 1.f, fo = 0.f;
             if constexpr (HL) {
-                // join the two groups: group 1 leaves its scaled sums where q was (the products that read q are done
-                // when both groups' last step is), group 0 adds them to its own
-                bars.ml[X][row] = make_float2(m, l);
-                ok = meet();
-                if (!ok) break;
+                if (ok) {
+                    bars.ml[X][row] = make_float2(m, l);
+                    ok = meet();
+                }
                 const float2 other = bars.ml[X ^ 1][row];
                 const float M = fmaxf(m, other.x);
                 f = M == -INFINITY ? 0.f : ex2(m - M);
-                l = l * f + (M == -INFINITY ? 0.f : other.y * ex2(other.x - M));
+                fo = M == -INFINITY ? 0.f : ex2(other.x - M);
+                l = l * f + other.y * fo;
                 m = M;
-                float4 *sums = reinterpret_cast<float4 *>(sm) + row;
-                if (X == 1) {
-#pragma unroll
-                    for (int i = 0; i < D / 16; ++i) {
-                        uint32_t v[16];
-                        if (any) {
-                            tmem_ld16(ox + 16 * i, v);
-                            tmem_wait_ld();
-                        }
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            sums[(4 * i + k) * 128] = any ? make_float4(__uint_as_float(v[4 * k]) * f, __uint_as_float(v[4 * k + 1]) * f,
-                                                                        __uint_as_float(v[4 * k + 2]) * f, __uint_as_float(v[4 * k + 3]) * f)
-                                                          : make_float4(0.f, 0.f, 0.f, 0.f);
-                    }
-                }
-                ok = meet();
-                if (!ok) break;
             }
-            const bool whole = w.c0 == 0 && w.c1 == w.cu;
-            if (!HL || X == 0) {
-                const int slot = (int)blockIdx.x * 2 + (nseg ? 1 : 0), prow = HL ? row : 128 * X + row;
-                const float inv = whole ? (l > 0.f ? 1.f / l : 0.f) : 1.f;
-                const float4 *sums = reinterpret_cast<const float4 *>(sm) + row;
-                T *op = static_cast<T *>(a.out) + (long)(w.sq.q0 + tok) * a.os + (long)head * D;
+            if (!ok) break;
+            tc_fence_after();
+            const int r = w.rt * RT + (HL ? 0 : 128 * X) + row;
+            const bool live = r < w.nq * a.G, whole = n == w.cu, two = HL && n > 1;   // one key tile: step 1 has no sums
+            const int tok = live ? div_g(a, r) : 0;
+            const int slot = (int)blockIdx.x * 2 + (nseg ? 1 : 0), prow = HL ? row : 128 * X + row;
+            const float inv = whole ? (l > 0.f ? 1.f / l : 0.f) : 1.f;
+            const float f0 = HL ? (X ? fo : f) : 1.f, f1 = HL ? (X ? f : fo) : 0.f;
+            T *op = static_cast<T *>(a.out) + (long)(w.q0 + tok) * a.os + (long)(w.kvh * a.G + r - tok * a.G) * D;
 #pragma unroll
-                for (int i = 0; i < D / 16; ++i) {
-                    uint32_t v[16];
-                    tmem_ld16(ox + 16 * i, v);
-                    tmem_wait_ld();
-                    float o[16];
+            for (int j = 0; j < (HL ? D / 32 : D / 16); ++j) {
+                const int i = HL ? X * (D / 32) + j : j;
+                uint32_t v[16], v1[HL ? 16 : 1];
+                tmem_ld16((HL ? tO + toff : ox) + 16 * i, v);
+                if constexpr (HL) {
+                    if (two) tmem_ld16(tO + 128 + toff + 16 * i, v1);
+                }
+                tmem_wait_ld();
+                float o[16];
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) o[k] = __uint_as_float(v[k]) * f;
+                for (int k = 0; k < 16; ++k) {
+                    o[k] = __uint_as_float(v[k]) * f0;
                     if constexpr (HL) {
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const float4 x = sums[(4 * i + k) * 128];
-                            o[4 * k] += x.x, o[4 * k + 1] += x.y, o[4 * k + 2] += x.z, o[4 * k + 3] += x.w;
-                        }
-                    }
-                    if (!whole) {
-                        float4 *pp = reinterpret_cast<float4 *>(a.part) + (long)slot * kPfRows * (D / 4) + prow;
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) pp[(4 * i + k) * kPfRows] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
-                    } else if (live) {
-                        // columns 0 .. 7 of a group of 8 are its dims 0, 4, 1, 5, 2, 6, 3, 7
-#pragma unroll
-                        for (int h = 0; h < 16; h += 8) {
-                            const float y[8] = {o[h] * inv, o[h + 2] * inv, o[h + 4] * inv, o[h + 6] * inv,
-                                                o[h + 1] * inv, o[h + 3] * inv, o[h + 5] * inv, o[h + 7] * inv};
-                            if constexpr (HL) {
-                                *reinterpret_cast<float4 *>(op + 16 * i + h) = make_float4(y[0], y[1], y[2], y[3]);
-                                *reinterpret_cast<float4 *>(op + 16 * i + h + 4) = make_float4(y[4], y[5], y[6], y[7]);
-                            } else {
-                                *reinterpret_cast<uint4 *>(op + 16 * i + h) =
-                                    make_uint4(u32(__floats2half2_rn(y[0], y[1])), u32(__floats2half2_rn(y[2], y[3])),
-                                               u32(__floats2half2_rn(y[4], y[5])), u32(__floats2half2_rn(y[6], y[7])));
-                            }
-                        }
+                        if (two) o[k] = fmaf(__uint_as_float(v1[k]), f1, o[k]);
                     }
                 }
                 if (!whole) {
-                    a.ml[(long)slot * kPfRows + prow] = make_float2(m, l);
-                    if (X == 0 && row == 0) a.meta[slot] = make_int4((int)w.at.item, w.at.b, w.at.kvh, w.at.rt | (w.c0 ? kInside : 0));
+                    float4 *pp = reinterpret_cast<float4 *>(a.part) + (long)slot * kPfRows * (D / 4) + prow;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) pp[(4 * i + k) * kPfRows] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+                } else if (live) {
+                    // columns 0 .. 7 of a group of 8 are its dims 0, 4, 1, 5, 2, 6, 3, 7
+#pragma unroll
+                    for (int h = 0; h < 16; h += 8) {
+                        const float y[8] = {o[h] * inv, o[h + 2] * inv, o[h + 4] * inv, o[h + 6] * inv,
+                                            o[h + 1] * inv, o[h + 3] * inv, o[h + 5] * inv, o[h + 7] * inv};
+                        if constexpr (HL) {
+                            *reinterpret_cast<float4 *>(op + 16 * i + h) = make_float4(y[0], y[1], y[2], y[3]);
+                            *reinterpret_cast<float4 *>(op + 16 * i + h + 4) = make_float4(y[4], y[5], y[6], y[7]);
+                        } else {
+                            *reinterpret_cast<uint4 *>(op + 16 * i + h) =
+                                make_uint4(u32(__floats2half2_rn(y[0], y[1])), u32(__floats2half2_rn(y[2], y[3])),
+                                           u32(__floats2half2_rn(y[4], y[5])), u32(__floats2half2_rn(y[6], y[7])));
+                        }
+                    }
                 }
             }
-            if constexpr (HL) ok = meet();          // group 0 has read the sums: q may come again
-            tc_fence_before();                      // the next step's products overwrite S and O
+            if (!whole && (!HL || X == 0)) {
+                a.ml[(long)slot * kPfRows + prow] = make_float2(m, l);
+                if (X == 0 && row == 0) a.meta[slot] = make_int4((int)w.item, w.b, w.kvh, w.rt | (c0 ? kInside : 0));
+            }
+            tc_fence_before();                      // the next step's products overwrite the sums
+            if constexpr (HL) ok = meet();          // both groups have read them
+            release(nseg);
         }
-        if (!ok) *abort_flag = 1;
     } else if (wg == 2) {
         // ================================ codes -> fp16 tiles ================================
         regs_less<96>();
         const Exponents expo;
         const int th = threadIdx.x - 256;
         uint32_t tile = 0, raw = 0;                // key tiles, raw stages so far
-        bool ok = true;
-        for (; w.more() && ok; w.next(a)) {
-            for (int c = w.c0; c < w.c1 && ok; ++c, ++tile) {
+        for (uint32_t nseg = 0; ok; ++nseg) {
+            ok = segment(nseg);
+            if (!ok) break;
+            const Seg &w = bars.seg[nseg % kSegs];
+            const int n = w.n, c0 = w.c0, len = w.len;
+            release(nseg);
+            if (n == 0) break;
+            for (int c = c0; c < c0 + n && ok; ++c, ++tile) {
                 const uint32_t st = tile & 1, par = (tile >> 1 & 1) ^ 1;
                 uint8_t *kt = sm + P::K0 + st * P::KT, *vt = sm + P::V0 + st * P::KT;
                 // all of K first: its products come a step ahead of V's
-                ok = __all_sync(0xffffffffu, mbar_wait(&bars.k_empty[st], par, abort_flag, a.status));
+                ok = wait(HL ? &bars.k_empty[st] : &bars.s_full[1][st], par);
                 if (!ok) break;
                 for (int half = 0; half < 2; ++half) {
                     const uint32_t rs = (raw + half) % kRawStages;
-                    ok = __all_sync(0xffffffffu, mbar_wait(&bars.raw_full[rs], (raw + half) / kRawStages & 1, abort_flag, a.status));
+                    ok = wait(&bars.raw_full[rs], (raw + half) / kRawStages & 1);
                     if (!ok) break;
                     const uint8_t *rp = sm + P::RAW0 + rs * P::RAW;
                     const uint32_t have = bars.raw_ok[rs];
-                    const int left = w.sq.len - c * kKeys - half * 64;   // positions of the sequence from here
+                    const int left = len - c * kKeys - half * 64;   // positions of the sequence from here
                     // 4 lanes per position, a word of every block each
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
@@ -488,13 +508,13 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const AttnArgs a
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bars.k_full[st]);
-                ok = __all_sync(0xffffffffu, mbar_wait(&bars.v_empty[st], par, abort_flag, a.status));
+                ok = wait(HL ? &bars.v_empty[st] : &bars.o_done[1][st], par);
                 if (!ok) break;
                 for (int half = 0; half < 2; ++half, ++raw) {
                     const uint32_t rs = raw % kRawStages;
                     const uint8_t *rp = sm + P::RAW0 + rs * P::RAW;
                     const uint32_t have = bars.raw_ok[rs];
-                    const int left = w.sq.len - c * kKeys - half * 64;
+                    const int left = len - c * kKeys - half * 64;
                     // a lane has the D / 8 dims from g * D / 8 of positions t + 4 m
 #pragma unroll
                     for (int i = 0; i < (D == 128 ? 2 : 1); ++i) {
@@ -522,84 +542,91 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const AttnArgs a
                 if (lane == 0) mbar_arrive(&bars.v_full[st]);
             }
         }
-        if (!ok) *abort_flag = 1;
     } else {
-        regs_less<40>();
-        if (warp == 12 && lane == 0) {
+        regs_less<64>();
+        if (warp == 12) {
             // ================================ products ================================
-            const uint32_t idS = idesc_make(1, 0, 0, 128, 128), idO = idesc_make(1, 0, 1, 128, D);
+            const uint32_t lead = lane == 0 ? 1u : 0u;
+            constexpr uint32_t idS = idesc_make(1, 0, 0, 128, 128), idO = idesc_make(1, 0, 1, 128, D);
             // matrix descriptors; tiles and slices of them differ in the address field (16-byte steps) alone
             const uint64_t descQ = smem_desc_sw128(smem_u32(sm), 16, 1024), descK = smem_desc_sw128(smem_u32(sm + P::K0), 16, 1024);
             const uint64_t descV = smem_desc_sw128(smem_u32(sm + P::V0), P::SUB, 1024);
-            uint32_t tile = 0, step[2] = {0, 0}, seg = 0;
-            bool ok = true;
-            for (; w.more() && ok; w.next(a), ++seg) {
-                const int S = HL ? w.n : 2 * w.n;
-                ok = mbar_wait(&bars.q_full, seg & 1, abort_flag, a.status);
+            uint32_t tile = 0, sdone = 0, pdone = 0;   // key tiles; scores and sums issued so far, X = 1's in the high half
+            for (uint32_t nseg = 0; ok; ++nseg) {
+                ok = segment(nseg);
                 if (!ok) break;
-                tc_fence_after();
+                const int n = bars.seg[nseg % kSegs].n;
+                release(nseg);
+                if (n == 0) break;
+                const int S = HL ? n : 2 * n;
+                ok = wait(&bars.q_full, nseg & 1);
+                if (!ok) break;
                 auto scores = [&](int s) {
                     const int X = s & 1;
                     const uint32_t tl = tile + (HL ? s : s >> 1), st = tl & 1;
                     if (HL || X == 0) {
-                        if (!mbar_wait(&bars.k_full[st], tl >> 1 & 1, abort_flag, a.status)) return false;
-                        tc_fence_after();
+                        if (!wait(&bars.k_full[st], tl >> 1 & 1)) return false;
                     }
+                    tc_fence_after();
                     const uint64_t qd = descQ + (HL ? 0 : X * (P::QT >> 4)), kd = descK + st * (P::KT >> 4);
 #pragma unroll
                     for (int p = 0; p < (HL ? 2 : 1); ++p)
 #pragma unroll
                         for (int k = 0; k < KS; ++k) {
                             const uint32_t off = ((k >> 2) * P::SUB + (k & 3) * 32) >> 4;
-                            umma_f16(tS + 128 * X, qd + p * (P::QT >> 4) + off, kd + off, idS, (p | k) ? 1u : 0u);
+                            umma_ss(tS + 128 * X, qd + p * (P::QT >> 4) + off, kd + off, idS, (p | k) ? 1u : 0u, lead);
                         }
-                    umma_commit(&bars.s_full[X]);
-                    if (HL || X == 1) umma_commit(&bars.k_empty[st]);
+                    umma_commit_lead(&bars.s_full[X][sdone >> (16 * X) & 1], lead);
+                    sdone += 1u << (16 * X);
+                    if (HL) umma_commit_lead(&bars.k_empty[st], lead);
+                    if (s == S - 1) umma_commit_lead(&bars.q_empty, lead);
                     return true;
                 };
                 for (int s = 0; s < 2 && s < S && ok; ++s) ok = scores(s);
-                uint32_t first = 3;                 // bit X: O of X has no sums yet
                 for (int s = 0; s < S && ok; ++s) {
                     const int X = s & 1;
-                    const uint32_t tl = tile + (HL ? s : s >> 1), st = tl & 1;
-                    ok = mbar_wait(&bars.p_ready[X], step[X] & 1, abort_flag, a.status);
-                    if (ok && (HL || X == 0)) ok = mbar_wait(&bars.v_full[st], tl >> 1 & 1, abort_flag, a.status);
+                    const uint32_t tl = tile + (HL ? s : s >> 1), st = tl & 1, done = pdone >> (16 * X);
+                    ok = wait(&bars.p_ready[X], done & 1);
+                    if (ok && (HL || X == 0)) ok = wait(&bars.v_full[st], tl >> 1 & 1);
                     if (!ok) break;
                     tc_fence_after();
                     const uint64_t vd = descV + st * (P::KT >> 4);
-                    const uint32_t more = first >> X & 1 ? 0u : 1u;
+                    const uint32_t more = s >= 2 ? 1u : 0u;      // O of X holds sums of the segment
 #pragma unroll
                     for (int p = 0; p < (HL ? 2 : 1); ++p)
 #pragma unroll
                         for (int k = 0; k < VS; ++k)
-                            umma_f16_ts(tO + 128 * X, tS + 128 * X + 64 * p + 8 * k, vd + k * (2048 >> 4), idO, (p | k) ? 1u : more);
-                    first &= ~(1u << X);
-                    ++step[X];
-                    umma_commit(&bars.o_done[X]);
-                    if (HL || X == 1) umma_commit(&bars.v_empty[st]);
+                            umma_ts(tO + 128 * X, tS + 128 * X + 64 * p + 8 * k, vd + k * (2048 >> 4), idO, (p | k) ? 1u : more, lead);
+                    umma_commit_lead(&bars.o_done[X][done & 1], lead);
+                    pdone += 1u << (16 * X);
+                    if (HL) umma_commit_lead(&bars.v_empty[st], lead);
                     if (s + 2 < S) ok = scores(s + 2);
                 }
-                tile += w.n;
+                tile += n;
             }
-            if (!ok) *abort_flag = 1;
-            umma_commit(&bars.drain);               // every product issued has ended when this completes
+            umma_commit_lead(&bars.drain, lead);    // every product issued has ended when this completes
             mbar_wait_drain(&bars.drain, 0, kWaitLimitNs);
         } else if (warp == 13) {
             // ================================ raw tiles ================================
             uint32_t raw = 0;
-            bool ok = true;
             const int ps = a.pool.page_shift;
             const long page_step = a.pool.page_bytes * a.pool.nkv;
-            for (; w.more() && ok; w.next(a)) {
-                const int *trow = a.tab.page + (long)w.at.b * a.tab.stride;
-                const uint8_t *base = a.pool.pages + (long)w.at.kvh * a.pool.page_bytes;
-                for (int h = 2 * w.c0; h < 2 * w.c1 && ok; ++h, ++raw) {
+            for (uint32_t nseg = 0; ok; ++nseg) {
+                ok = segment(nseg);
+                if (!ok) break;
+                const Seg &w = bars.seg[nseg % kSegs];
+                const int n = w.n, c0 = w.c0, len = w.len;
+                const int *trow = a.tab.page + (long)w.b * a.tab.stride;
+                const uint8_t *base = a.pool.pages + (long)w.kvh * a.pool.page_bytes;
+                release(nseg);
+                if (n == 0) break;
+                for (int h = 2 * c0; h < 2 * (c0 + n) && ok; ++h, ++raw) {
                     const uint32_t rs = raw % kRawStages;
                     const int pos = h * 64 + lane * 16;
-                    const int page = lane < 4 && pos < w.sq.len ? __ldg(trow + (pos >> ps)) : -1;
+                    const int page = lane < 4 && pos < len ? __ldg(trow + (pos >> ps)) : -1;
                     const bool on = (unsigned)page < (unsigned)a.pool.n_pages;
                     const uint32_t have = __ballot_sync(0xffffffffu, on);
-                    ok = __all_sync(0xffffffffu, mbar_wait(&bars.raw_empty[rs], (raw / kRawStages & 1) ^ 1, abort_flag, a.status));
+                    ok = wait(&bars.raw_empty[rs], (raw / kRawStages & 1) ^ 1);
                     if (!ok) break;
                     if (lane == 0) {
                         bars.raw_ok[rs] = have;
@@ -617,8 +644,45 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const AttnArgs a
                     for (uint32_t i = raw > kRawStages ? raw - kRawStages : 0; i < raw; ++i)
                         mbar_wait_drain(&bars.raw_full[i % kRawStages], i / kRawStages & 1, kWaitLimitNs);
             }
+        } else if (warp == 14) {
+            // ================================ work list ================================
+            const Start at = my_start<RT>(a);
+            uint32_t u = at.u0, item = at.item, nseg = 0;
+            int b = at.b, kvh = at.kvh, rt = at.rt;
+            Seq sq;
+            if (u < at.u1) sq = load_seq(a, b, RT, false);
+            for (bool more = true; more && ok;) {
+                Seg g = {};
+                more = u < at.u1;
+                if (more) {
+                    // a run that ends within an item's kLead units has none of its key tiles, and one that starts there has all
+                    const int cu = units_of<RT>(a, sq, rt) - kLead, k0 = (int)(u - item), k1 = (int)min((uint32_t)(cu + kLead), k0 + (at.u1 - u));
+                    g.c0 = max(0, k0 - kLead);
+                    g.n = max(0, k1 - kLead) - g.c0;
+                    g.cu = cu, g.b = b, g.kvh = kvh, g.rt = rt, g.q0 = sq.q0, g.nq = sq.nq, g.len = sq.len, g.item = item;
+                    item += cu + kLead;
+                    u = item;
+                    if (u < at.u1 && ++rt == sq.nrt) {
+                        rt = 0;
+                        if (++kvh == a.pool.nkv) {
+                            kvh = 0;
+                            do sq = load_seq(a, ++b, RT, false);
+                            while (!sq.nrt);
+                        }
+                    }
+                    if (g.n == 0) continue;
+                }
+                ok = wait(&bars.seg_empty[nseg % kSegs], (nseg / kSegs & 1) ^ 1);
+                if (!ok) break;
+                if (lane == 0) {
+                    bars.seg[nseg % kSegs] = g;
+                    mbar_arrive(&bars.seg_full[nseg % kSegs]);
+                }
+                ++nseg;
+            }
         }
     }
+    if (!ok) *abort_flag = 1;
     tc_fence_before();
     __syncthreads();
     if (warp == 12) tmem_dealloc(tmem, 512);
