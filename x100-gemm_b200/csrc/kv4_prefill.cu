@@ -201,7 +201,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const AttnArgs a
     extern __shared__ uint8_t smem_raw[];
     uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     __shared__ PfBars bars;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wg = warp >> 2;
+    // broadcast, so that the compiler knows it for a warp-uniform value and the branches on it for uniform ones
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, wg = warp >> 2;
     if (threadIdx.x == 0) {
         bars.abort_flag = 0;
         for (int i = 0; i < kRawStages; ++i) mbar_init(&bars.raw_full[i], 1), mbar_init(&bars.raw_empty[i], kDqWarps);
@@ -225,7 +226,9 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const AttnArgs a
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = bars.tmem, tS = tmem, tO = tmem + 256;   // S, O of step X: + 128 X columns
+    // S, O of step X: + 128 X columns.  All 512 columns are this CTA's, so they start at column 0.
+    constexpr uint32_t tS = 0, tO = 256;
+    const uint32_t tmem = bars.tmem;
     volatile int *abort_flag = &bars.abort_flag;
     auto wait = [&](uint64_t *bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, a.status)); };
     // the i-th segment; a role reads what it needs of it before release(i)
@@ -234,7 +237,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const AttnArgs a
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.seg_empty[i % kSegs]);
     };
-    bool ok = true;
+    bool ok = __all_sync(0xffffffffu, tmem == 0);
+    if (!ok && threadIdx.x == 0) atomicCAS(a.status, 0, X100_E_LAUNCH);
     if (wg < 2) {
         // ================================ softmax ================================
         regs_more<176>();
@@ -555,7 +559,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const AttnArgs a
             for (uint32_t nseg = 0; ok; ++nseg) {
                 ok = segment(nseg);
                 if (!ok) break;
-                const int n = bars.seg[nseg % kSegs].n;
+                const int n = __shfl_sync(0xffffffffu, bars.seg[nseg % kSegs].n, 0);   // uniform for the compiler too
                 release(nseg);
                 if (n == 0) break;
                 const int S = HL ? n : 2 * n;
