@@ -6,10 +6,10 @@
 // 128 x 128 x D tcgen05.mma with S, P (over S) and O in TMEM.  One CTA per SM:
 //   warps 0-3, 4-7   softmax of step X = 0, 1: a thread owns a row; S from TMEM, running max
 //                    (moved only when a score passes it by 2^8), P as fp16 back to TMEM
-//   warps 8-11       raw codes in shared memory -> fp16 K and V tiles in the 128-byte-swizzled
+//   4 or 8 warps     raw codes in shared memory -> fp16 K and V tiles in the 128-byte-swizzled
 //                    layouts the MMA reads; scale * (code - 8) is an fp16 value, so exact
-//   warp 12          issues the MMAs;  warp 13  copies the raw tiles (bulk copies)
-//   warp 14          walks the work list and hands every role its segments through shared memory
+//   a warp each      issues the MMAs; copies the raw tiles (bulk copies);
+//                    walks the work list and hands every role its segments through shared memory
 // fp16 q: the steps X are two row tiles over the same key tile (256 rows per item), so that
 // a key tile is unpacked once for both.  fp32 q: q and P are carried as hi + lo halves, two
 // products each, and the steps X are every other key tile of one row tile, joined at the end.
@@ -24,17 +24,24 @@
 namespace x100 {
 namespace kv4 {
 
-constexpr int kPfThreads = 512, kDqWarps = 4, kRawStages = 3;
+constexpr int kRawStages = 3;
 constexpr int kKeys = 128;                 // positions per key tile
 constexpr int kPfCtas = 160;               // bound of the grid, which sizes the workspace
 constexpr int kPfRows = 256;               // rows per slot of the workspace
+
+// Warps that unpack: four feed two row tiles per key tile (fp16 q; more of them only take issue slots from the
+// softmax: 488 against 509 us for 2048 tokens over 16384 positions), eight feed a key tile per step (fp32 q).
+template <typename T>
+struct Roles {
+    static constexpr int DQ = sizeof(T) == 4 ? 8 : 4, kMma = 8 + DQ, THREADS = (8 + DQ + 4) * 32, SEGS = 8 + DQ + 2;   // SEGS: warps that read segments
+};
 
 template <int D>
 struct Pf {
     static constexpr int QT = 128 * D * 2;                       // one Q tile, or half of fp32 q
     static constexpr int KT = kKeys * D * 2;                     // a K or V tile
     static constexpr int RAW = 4 * Lay<D>::BYTES;                // 64 positions
-    static constexpr int K0 = 2 * QT, V0 = K0 + 2 * KT, RAW0 = V0 + 2 * KT, SMEM = RAW0 + kRawStages * RAW + 1024;
+    static constexpr int K0 = 2 * QT, V0 = K0 + 2 * KT, RAW0 = V0 + 2 * KT, SMEM = RAW0 + kRawStages * RAW;
     static constexpr int SUB = 128 * 128;                        // 128 rows of 64 dims
 };
 
@@ -151,7 +158,7 @@ struct Seg {
     int c0, cu, b, kvh, rt, q0, nq, len;
     uint32_t item;                         // the item's first unit
 };
-constexpr int kSegs = 4, kRoles = 14;      // ring of segments; warps that read one
+constexpr int kSegs = 4;                   // ring of segments
 
 // Barriers that a step's MMAs signal come in pairs, the step's parity choosing one, so that the one for key tile k is
 // also what frees that tile's stage (fp16 q, X = 1) and the issuing warp commits only twice a step.
@@ -192,21 +199,21 @@ __device__ __forceinline__ uint64_t add2(uint64_t s, float x, float y) {
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(Roles<T>::THREADS, 1) prefill_kernel(const AttnArgs a) {
     using L = Lay<D>;
     using P = Pf<D>;
     constexpr bool HL = sizeof(T) == 4;
     constexpr int RT = HL ? 128 : 256;      // rows per item
-    constexpr int KS = D / 16, VS = kKeys / 16;
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    using W = Roles<T>;
+    constexpr int KS = D / 16, VS = kKeys / 16, kDqWarps = W::DQ;
+    extern __shared__ __align__(1024) uint8_t sm[];
     __shared__ PfBars bars;
     // broadcast, so that the compiler knows it for a warp-uniform value and the branches on it for uniform ones
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, wg = warp >> 2;
     if (threadIdx.x == 0) {
         bars.abort_flag = 0;
         for (int i = 0; i < kRawStages; ++i) mbar_init(&bars.raw_full[i], 1), mbar_init(&bars.raw_empty[i], kDqWarps);
-        for (int i = 0; i < kSegs; ++i) mbar_init(&bars.seg_full[i], 1), mbar_init(&bars.seg_empty[i], kRoles);
+        for (int i = 0; i < kSegs; ++i) mbar_init(&bars.seg_full[i], 1), mbar_init(&bars.seg_empty[i], W::SEGS);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bars.k_full[i], kDqWarps), mbar_init(&bars.k_empty[i], 1);
             mbar_init(&bars.v_full[i], kDqWarps), mbar_init(&bars.v_empty[i], 1);
@@ -216,7 +223,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const AttnArgs a
         mbar_init(&bars.q_full, 8), mbar_init(&bars.q_empty, 1), mbar_init(&bars.joined, 8), mbar_init(&bars.drain, 1);
         fence_barrier_init();
     }
-    if (warp == 12) {
+    if (warp == W::kMma) {
         tmem_alloc(&bars.tmem, 512);
         tmem_relinquish();
     }
@@ -230,18 +237,19 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const AttnArgs a
     constexpr uint32_t tS = 0, tO = 256;
     const uint32_t tmem = bars.tmem;
     volatile int *abort_flag = &bars.abort_flag;
-    auto wait = [&](uint64_t *bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, a.status)); };
+    auto wait = [&](uint64_t *bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait_quiet(bar, parity, abort_flag, a.status)); };
     // the i-th segment; a role reads what it needs of it before release(i)
     auto segment = [&](uint32_t i) { return wait(&bars.seg_full[i % kSegs], i / kSegs & 1); };
     auto release = [&](uint32_t i) {
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.seg_empty[i % kSegs]);
     };
-    bool ok = __all_sync(0xffffffffu, tmem == 0);
+    bool ok = __all_sync(0xffffffffu, tmem == 0 && (smem_u32(sm) & 1023) == 0);
     if (!ok && threadIdx.x == 0) atomicCAS(a.status, 0, X100_E_LAUNCH);
     if (wg < 2) {
         // ================================ softmax ================================
-        regs_more<176>();
+        // registers: the launch's 65536 (512 threads of 128) or 61440 (640 of 96) shared out anew
+        regs_more<HL ? 160 : 176>();
         const int X = wg, row = threadIdx.x & 127;
         const uint32_t toff = (uint32_t)((warp & 3) * 32) << 16, sx = tS + 128 * X + toff, ox = tO + 128 * X + toff;
         uint32_t step = 0, joins = 0;            // steps of this X, meetings of the two groups so far
@@ -460,9 +468,9 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const AttnArgs a
             if constexpr (HL) ok = meet();          // both groups have read them
             release(nseg);
         }
-    } else if (wg == 2) {
+    } else if (warp < W::kMma) {
         // ================================ codes -> fp16 tiles ================================
-        regs_less<96>();
+        regs_less<HL ? 56 : 96>();
         const Exponents expo;
         const int th = threadIdx.x - 256;
         uint32_t tile = 0, raw = 0;                // key tiles, raw stages so far
@@ -479,19 +487,19 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const AttnArgs a
                 // all of K first: its products come a step ahead of V's
                 ok = wait(HL ? &bars.k_empty[st] : &bars.s_full[1][st], par);
                 if (!ok) break;
+#pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     const uint32_t rs = (raw + half) % kRawStages;
                     ok = wait(&bars.raw_full[rs], (raw + half) / kRawStages & 1);
                     if (!ok) break;
                     const uint8_t *rp = sm + P::RAW0 + rs * P::RAW;
                     const uint32_t have = bars.raw_ok[rs];
-                    const int left = len - c * kKeys - half * 64;   // positions of the sequence from here
                     // 4 lanes per position, a word of every block each
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int key = i * 32 + (th >> 2), t = th & 3, in = key & 15, kk = half * 64 + key;
+                    for (int u = 0; u < 8 / kDqWarps; ++u) {
+                        const int key = u * (8 * kDqWarps) + (th >> 2), t = th & 3, in = key & 15, kk = half * 64 + key;
                         const uint8_t *tp = rp + (key >> 4) * L::BYTES;
-                        const bool on = (have >> (key >> 4) & 1) && key < left;
+                        const bool on = (have >> (key >> 4) & 1) && c * kKeys + kk < len;
                         uint32_t kw[L::NB];
                         __half kd[L::NB];
                         if constexpr (D == 128) {
@@ -514,41 +522,42 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const AttnArgs a
                 if (lane == 0) mbar_arrive(&bars.k_full[st]);
                 ok = wait(HL ? &bars.v_empty[st] : &bars.o_done[1][st], par);
                 if (!ok) break;
-                for (int half = 0; half < 2; ++half, ++raw) {
-                    const uint32_t rs = raw % kRawStages;
-                    const uint8_t *rp = sm + P::RAW0 + rs * P::RAW;
-                    const uint32_t have = bars.raw_ok[rs];
-                    const int left = len - c * kKeys - half * 64;
-                    // a lane has the D / 8 dims from g * D / 8 of positions t + 4 m
+#pragma unroll
+                for (int u = 0; u < 8 / kDqWarps; ++u) {
+                    // a warp has a 16-position tile; a lane the D / 8 dims from g * D / 8 of positions t + 4 m
+                    const int tl = u * kDqWarps + warp - 8, g = lane >> 2, t = lane & 3;
+                    const uint32_t rs = (raw + (tl >> 2)) % kRawStages;
+                    const uint8_t *tp = sm + P::RAW0 + rs * P::RAW + (tl & 3) * L::BYTES;
+                    const int left = bars.raw_ok[rs] >> (tl & 3) & 1 ? len - c * kKeys : 0;   // positions of the sequence from the key tile on
+                    __half vd[4];
+                    *reinterpret_cast<uint2 *>(vd) = *reinterpret_cast<const uint2 *>(tp + L::v_scale(t, g * (D / 8) / 32));
 #pragma unroll
                     for (int i = 0; i < (D == 128 ? 2 : 1); ++i) {
-                        const int tl = th >> 5, g = lane >> 2, t = lane & 3;
-                        const uint8_t *tp = rp + tl * L::BYTES;
-                        const bool on = have >> tl & 1;
                         const uint4 x = *reinterpret_cast<const uint4 *>(tp + L::V0 + i * 512 + lane * 16);
                         const uint32_t vw[4] = {x.x, x.y, x.z, x.w};
-                        __half vd[4];
-                        *reinterpret_cast<uint2 *>(vd) = *reinterpret_cast<const uint2 *>(tp + L::v_scale(t, g * (D / 8) / 32));
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
                             // D = 128: words 2 q, 2 q + 1 of position t + 4 (2 i + q); D = 64: word q of position t + 4 q
-                            const int m = D == 128 ? 2 * i + (k >> 1) : k, key = tl * 16 + 4 * m + t, kk = half * 64 + key;
+                            const int m = D == 128 ? 2 * i + (k >> 1) : k, kk = tl * 16 + 4 * m + t;
                             const int dim = g * (D / 8) + (D == 128 ? (k & 1) * 8 : 0);
-                            const __half2 d = __half2half2(on && key < left ? vd[m] : __ushort_as_half(0));
+                            const __half2 d = __half2half2(kk < left ? vd[m] : __ushort_as_half(0));
                             *reinterpret_cast<uint4 *>(vt + (dim >> 6) * P::SUB + kk * 128 + ((((dim & 63) >> 3) ^ (kk & 7)) << 4)) = eight(vw[k], d, expo);
                         }
                     }
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&bars.raw_empty[rs]);
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&bars.v_full[st]);
+                if (lane == 0) {
+                    mbar_arrive(&bars.raw_empty[raw % kRawStages]);
+                    mbar_arrive(&bars.raw_empty[(raw + 1) % kRawStages]);
+                    mbar_arrive(&bars.v_full[st]);
+                }
+                raw += 2;
             }
         }
     } else {
-        regs_less<64>();
-        if (warp == 12) {
+        regs_less<HL ? 48 : 64>();
+        if (warp == W::kMma) {
             // ================================ products ================================
             const uint32_t lead = lane == 0 ? 1u : 0u;
             constexpr uint32_t idS = idesc_make(1, 0, 0, 128, 128), idO = idesc_make(1, 0, 1, 128, D);
@@ -610,7 +619,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const AttnArgs a
             }
             umma_commit_lead(&bars.drain, lead);    // every product issued has ended when this completes
             mbar_wait_drain(&bars.drain, 0, kWaitLimitNs);
-        } else if (warp == 13) {
+        } else if (warp == W::kMma + 1) {
             // ================================ raw tiles ================================
             uint32_t raw = 0;
             const int ps = a.pool.page_shift;
@@ -648,7 +657,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const AttnArgs a
                     for (uint32_t i = raw > kRawStages ? raw - kRawStages : 0; i < raw; ++i)
                         mbar_wait_drain(&bars.raw_full[i % kRawStages], i / kRawStages & 1, kWaitLimitNs);
             }
-        } else if (warp == 14) {
+        } else if (warp == W::kMma + 2) {
             // ================================ work list ================================
             const Start at = my_start<RT>(a);
             uint32_t u = at.u0, item = at.item, nseg = 0;
@@ -689,7 +698,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const AttnArgs a
     if (!ok) *abort_flag = 1;
     tc_fence_before();
     __syncthreads();
-    if (warp == 12) tmem_dealloc(tmem, 512);
+    if (warp == W::kMma) tmem_dealloc(tmem, 512);
 }
 
 // Joins the parts of an item at the first cut inside it (as merge_kernel in kv4_attn.cu): a thread per row, 16 columns per CTA.
@@ -765,7 +774,7 @@ static int launch_pf(DevCtx *c, AttnArgs &a, cudaStream_t s) {
     a.ml = reinterpret_cast<float2 *>(a.part + (size_t)kPfCtas * 2 * kPfRows * D);
     a.meta = reinterpret_cast<int4 *>(a.ml + kPfCtas * 2 * kPfRows);
     a.unit_shift = 7;
-    int st = launch_pdl(prefill_kernel<T, D>, dim3(grid), dim3(kPfThreads), Pf<D>::SMEM, s, a);
+    int st = launch_pdl(prefill_kernel<T, D>, dim3(grid), dim3(Roles<T>::THREADS), Pf<D>::SMEM, s, a);
     if (st || grid == 1) return st;
     return launch_pdl(prefill_merge_kernel<T, D>, dim3(grid - 1, D / 16), dim3(kPfRows), 0, s, a, grid);
 }

@@ -82,6 +82,34 @@ __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, volati
     }
 }
 
+// The same wait for kernels whose waiting warps share the schedulers with busy
+// ones: each try may suspend the warp for up to kWaitHintNs, so that it does not
+// spend its neighbours' issue slots on polling.
+constexpr uint32_t kWaitHintNs = 20000;
+__device__ __forceinline__ bool mbar_wait_quiet(uint64_t *bar, uint32_t parity, volatile int *abort_flag, int *err) {
+    const uint32_t a = smem_u32(bar);
+    unsigned long long t0 = 0;
+    for (;;) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+            "selp.b32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(a), "r"(parity), "r"(kWaitHintNs)
+            : "memory");
+        if (ok) return true;
+        if (*abort_flag) return false;
+        const unsigned long long t = globaltimer_ns();
+        if (t0 == 0) t0 = t;
+        if (t - t0 > kWaitLimitNs) {
+            *abort_flag = 1;
+            if (err) atomicExch(err, 7);
+            return false;
+        }
+    }
+}
+
 // Short bounded wait used only while unwinding after an abort.
 __device__ __forceinline__ bool mbar_wait_drain(uint64_t *bar, uint32_t parity, unsigned long long limit_ns) {
     const uint32_t a = smem_u32(bar);
