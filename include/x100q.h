@@ -171,7 +171,7 @@ typedef struct {
     const float *q_norm, *k_norm; /* [head_dim] or NULL                      */
     float eps;
     const float *rope;            /* [rope_len][head_dim / 2][cos, sin] or NULL */
-    int rope_len;                 /* a position past it is out of range      */
+    int rope_len;                 /* a position past it is out of range; the table is 16-byte aligned */
     const int *pos, *seq;         /* [n_tokens]                              */
     const int *page_table;
     int table_stride, n_seqs;

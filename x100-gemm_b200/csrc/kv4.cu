@@ -24,201 +24,223 @@ struct AppendArgs {
     const float *qn, *kn;
     float eps;
     const float2 *rope;
-    int rope_len, n_tokens, nh;
+    int rope_len, n_tokens, nh, slices;
     const int *pos, *seq;
     int *status;
 };
 
-// The E consecutive elements of a lane (E = D / 32: lane l holds E l ..), in fp32.
+// 16 bytes of a head in fp32.
 template <typename T, int E>
-__device__ __forceinline__ void load_lane(const T *p, int lane, float (&x)[E]) {
+__device__ __forceinline__ void unpack(uint4 v, float (&x)[E]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
     if constexpr (sizeof(T) == 4) {
-        if constexpr (E == 4) {
-            const float4 v = *(reinterpret_cast<const float4 *>(p) + lane);
-            x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
-        } else {
-            const float2 v = *(reinterpret_cast<const float2 *>(p) + lane);
-            x[0] = v.x, x[1] = v.y;
-        }
-    } else {
-        __half2 h[E / 2];
-        if constexpr (E == 4) *reinterpret_cast<uint2 *>(h) = *(reinterpret_cast<const uint2 *>(p) + lane);
-        else *reinterpret_cast<uint32_t *>(h) = *(reinterpret_cast<const uint32_t *>(p) + lane);
 #pragma unroll
-        for (int i = 0; i < E / 2; ++i) {
-            const float2 f = __half22float2(h[i]);
+        for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(w[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(w + i));
             x[2 * i] = f.x, x[2 * i + 1] = f.y;
         }
     }
 }
 template <typename T, int E>
-__device__ __forceinline__ void store_lane(T *p, int lane, const float (&x)[E]) {
-    if constexpr (sizeof(T) == 4) {
-        if constexpr (E == 4) *(reinterpret_cast<float4 *>(p) + lane) = make_float4(x[0], x[1], x[2], x[3]);
-        else *(reinterpret_cast<float2 *>(p) + lane) = make_float2(x[0], x[1]);
-    } else {
-        __half2 h[E / 2];
+__device__ __forceinline__ uint4 pack(const float (&x)[E]) {
+    uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < E / 2; ++i) h[i] = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
-        if constexpr (E == 4) *(reinterpret_cast<uint2 *>(p) + lane) = *reinterpret_cast<uint2 *>(h);
-        else *(reinterpret_cast<uint32_t *>(p) + lane) = *reinterpret_cast<uint32_t *>(h);
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(x[i]);
+        else {
+            const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t *>(&h);
+        }
     }
+    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// One head of q, k or v of one token per warp; a lane holds E = D / 32
-// consecutive elements, so an element's rotation partner (j + D / 2) is lane ^ 16's
-// same element and a block of 32 is 32 / E neighbouring lanes.  Every product, sum and
-// quotient up to the code is rounded by itself (no contraction), which makes the codes
-// the same on any machine that follows the formula.  Codes are taken before
-// the factor 1 / rms, which a block's scale carries: rounding of the sum of squares
-// cannot move a value over a code's border.
+// A lane holds 16 bytes (E elements) of a head, so LH = D / E lanes have a head and a warp HW = 32 / LH
+// heads side by side.  An element's rotation partner (j + D / 2) is the same element of lane ^ LH / 2, and a block
+// of 32 is 32 / E neighbouring lanes.  A warp takes the groups of HW heads of one token that are its slice's
+// (slice, slice + slices, ..), the next group's bytes on their way while one is worked on; the rotation's row is
+// loaded once.  Every product, sum and quotient up to the code is rounded by itself (no contraction), which
+// makes the codes the same on any machine that follows the formula.  Codes are taken before the factor
+// 1 / rms, which a block's scale carries: rounding of the sum of squares cannot move a value over a code's
+// border.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
     using L = Lay<D>;
-    constexpr int E = D / 32, LB = 32 / E;   // LB lanes per block
-    const int lane = threadIdx.x & 31;
-    const int heads = a.nh + 2 * a.pool.nkv;
+    constexpr int E = 16 / sizeof(T), LH = D / E, HW = 32 / LH, LB = 32 / E;   // LB lanes per block
+    const int lane = threadIdx.x & 31, in = lane % LH, hl = lane / LH;          // place in the head, head of the group
+    const int nkv = a.pool.nkv, gq = (a.nh + HW - 1) / HW, gk = (nkv + HW - 1) / HW, groups = gq + 2 * gk;
     const long item = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
     pdl_launch_dependents();
     pdl_wait();
-    if (item >= (long)a.n_tokens * heads) return;
-    const int i = (int)(item / heads), h = (int)(item % heads);
+    if (item >= (long)a.n_tokens * a.slices) return;
+    const int i = (int)(item / a.slices), slice = (int)(item % a.slices);
     const int pos = a.pos[i];
     if (pos < 0) return;                                  // padding
-    const bool is_q = h < a.nh, is_k = !is_q && h < a.nh + a.pool.nkv;
     const int seq = a.seq ? a.seq[i] : i;
-    const bool rotate = a.rope && (is_q || is_k);
-    uint8_t *tile = nullptr;
-    bool bad = rotate && pos >= a.rope_len;
-    if (!is_q && !bad) {
-        tile = tile_of(a.pool, a.tab, seq, pos, is_k ? h - a.nh : h - a.nh - a.pool.nkv);
-        bad = tile == nullptr;
-    }
-    if (bad) {
-        if (lane == 0) atomicCAS(a.status, 0, X100_E_ARG);
-        return;
-    }
-    float x[E], t[E];
-    const T *src = is_q ? static_cast<const T *>(a.q) + i * a.qs + (long)h * D
-                        : is_k ? static_cast<const T *>(a.k) + i * a.ks + (long)(h - a.nh) * D
-                               : static_cast<const T *>(a.v) + i * a.vs + (long)(h - a.nh - a.pool.nkv) * D;
-    load_lane<T, E>(src, lane, x);
-    float s = 1.f;
-    const float *w = is_q ? a.qn : is_k ? a.kn : nullptr;
-    if (w) {
-        float ss = 0.f;
+    // bytes of group g for this lane; heads past the last one load nothing
+    auto fetch = [&](int g) {
+        const T *p;
+        int h;
+        if (g < gq) h = g * HW + hl, p = h < a.nh ? static_cast<const T *>(a.q) + i * a.qs : nullptr;
+        else if (g < gq + gk) h = (g - gq) * HW + hl, p = h < nkv ? static_cast<const T *>(a.k) + i * a.ks : nullptr;
+        else h = (g - gq - gk) * HW + hl, p = h < nkv ? static_cast<const T *>(a.v) + i * a.vs : nullptr;
+        return p ? *reinterpret_cast<const uint4 *>(p + (long)h * D + in * E) : make_uint4(0, 0, 0, 0);
+    };
+    int g = slice;
+    if (g >= groups) return;
+    uint4 next = fetch(g);
+    // the rotation's row and the token's page: a bad position or page is left out and reported
+    const bool turn = a.rope != nullptr, far = turn && pos >= a.rope_len;
+    float2 cs[E];
+    if (turn && !far) {
+        const float4 *row = reinterpret_cast<const float4 *>(a.rope + (long)pos * (D / 2) + (in * E & (D / 2 - 1)));
 #pragma unroll
-        for (int e = 0; e < E; ++e) ss += x[e] * x[e];
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        s = 1.f / sqrtf(ss / (float)D + a.eps);
-#pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = __fmul_rn(x[e], __ldg(w + E * lane + e));
+        for (int e = 0; e < E / 2; ++e) {
+            const float4 r = __ldg(row + e);
+            cs[2 * e] = make_float2(r.x, r.y), cs[2 * e + 1] = make_float2(r.z, r.w);
+        }
     }
-    if (rotate) {
-        const float2 *row = a.rope + (long)pos * (D / 2) + ((E * lane) & (D / 2 - 1));
+    uint8_t *tile = nullptr;                              // of kv head 0
+    if (g + (groups - 1 - g) / a.slices * a.slices >= gq) tile = tile_of(a.pool, a.tab, seq, pos, 0);   // the slice has k or v
+    bool bad = false;
+    for (; g < groups; g += a.slices) {
+        float x[E], t[E];
+        unpack<T, E>(next, x);
+        if (g + a.slices < groups) next = fetch(g + a.slices);
+        const bool is_q = g < gq, is_k = !is_q && g < gq + gk;
+        const int h = (is_q ? g : is_k ? g - gq : g - gq - gk) * HW + hl;
+        const bool rotate = turn && (is_q || is_k);
+        if (far || (!is_q && !tile)) {
+            bad = true;
+            continue;
+        }
+        float s = 1.f;
+        const float *w = is_q ? a.qn : is_k ? a.kn : nullptr;
+        if (w) {
+            float ss = 0.f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) ss += x[e] * x[e];
+#pragma unroll
+            for (int o = LH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            s = 1.f / sqrtf(ss / (float)D + a.eps);
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[e] = __fmul_rn(x[e], __ldg(w + in * E + e));
+        }
+        if (rotate) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float o = __shfl_xor_sync(0xffffffffu, x[e], LH / 2);
+                t[e] = in < LH / 2 ? __fsub_rn(__fmul_rn(x[e], cs[e].x), __fmul_rn(o, cs[e].y))
+                                   : __fadd_rn(__fmul_rn(x[e], cs[e].x), __fmul_rn(o, cs[e].y));
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) t[e] = x[e];
+        }
+        if (is_q) {
+            if (w) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) t[e] *= s;
+            }
+            if (h < a.nh) *reinterpret_cast<uint4 *>(static_cast<T *>(a.qo) + i * a.qos + (long)h * D + in * E) = pack<T, E>(t);
+            continue;
+        }
+        float top = t[0], low = t[0], z = 0.f;            // z: 0, or NaN where a value is not finite
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const float2 cs = __ldg(row + e);
-            const float o = __shfl_xor_sync(0xffffffffu, x[e], 16);
-            t[e] = lane < 16 ? __fsub_rn(__fmul_rn(x[e], cs.x), __fmul_rn(o, cs.y))
-                             : __fadd_rn(__fmul_rn(x[e], cs.x), __fmul_rn(o, cs.y));
+            top = fmaxf(top, t[e]);
+            low = fminf(low, t[e]);
+            z = fmaf(t[e], 0.f, z);
         }
-    } else {
 #pragma unroll
-        for (int e = 0; e < E; ++e) t[e] = x[e];
-    }
-    if (is_q) {
+        for (int o = 1; o < LB; o <<= 1) {
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+        }
+        const float m = top >= -low ? top : low;
+        float inv = fabsf(m) < kTinyBlock ? 0.f : __fdiv_rn(-8.f, m);
+        float d = __fmul_rn(__fmul_rn(m, -0.125f), s);
+        const uint32_t fine = __ballot_sync(0xffffffffu, z == 0.f && fabsf(d) < INFINITY);
+        const uint32_t mine = ((1u << LB) - 1u) << (lane & ~(LB - 1));
+        if (h >= nkv) continue;
+        if ((fine & mine) != mine) {                      // a NaN or an infinity in the block
+            inv = 0.f, d = 0.f;
+            bad = true;
 #pragma unroll
-        for (int e = 0; e < E; ++e) t[e] *= s;
-        store_lane<T, E>(static_cast<T *>(a.qo) + i * a.qos + (long)h * D, lane, t);
-        return;
-    }
-    float top = t[0], low = t[0];
-    bool fin = true;
+            for (int e = 0; e < E; ++e) t[e] = 0.f;
+        }
+        // x * inv + 8.5 lies in (0, 17): added to 2^23 rounding down, its floor is the low bits (8 where inv is 0)
+        uint32_t codes = 0;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        top = fmaxf(top, t[e]);
-        low = fminf(low, t[e]);
-        fin = fin && fabsf(t[e]) < INFINITY;
-    }
-#pragma unroll
-    for (int o = 1; o < LB; o <<= 1) {
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
-    }
-    const float m = top >= -low ? top : low;
-    float inv = fabsf(m) < kTinyBlock ? 0.f : __fdiv_rn(-8.f, m);
-    float d = __fmul_rn(__fmul_rn(m, -0.125f), s);
-    const uint32_t mask = __ballot_sync(0xffffffffu, fin && fabsf(d) < INFINITY) | 0u;
-    const uint32_t mine = (LB == 32 ? 0xffffffffu : ((1u << LB) - 1u)) << (lane & ~(LB - 1));
-    if ((mask & mine) != mine) {                          // a NaN or an infinity in the block
-        inv = 0.f, d = 0.f;
-        if (lane % LB == 0) atomicCAS(a.status, 0, X100_E_ARG);
-    }
-    uint32_t codes = 0;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const float c = inv == 0.f ? 8.f : floorf(__fadd_rn(__fmul_rn(t[e], inv), 8.5f));
-        codes |= (uint32_t)fminf(fmaxf(c, 0.f), 15.f) << (4 * e);
-    }
-    const __half dh = __float2half_rn(__bfloat162float(__float2bfloat16_rn(fminf(fmaxf(d, -kMostScale), kMostScale))));
-    const int sp = pos & 15, b = E * lane / 32;
-    if (is_k) {
-        const int in = E * lane & 31;                     // first dim of the lane in its block
-        uint8_t *at = tile + L::k_word(sp, b, in >> 3) + (in & 7) / 2;
+        for (int e = 0; e < E; ++e) {
+            const uint32_t c = __float_as_uint(__fadd_rd(__fadd_rn(__fmul_rn(t[e], inv), 8.5f), 8388608.f)) - 0x4b000000u;
+            codes |= min(c, 15u) << (4 * e);
+        }
+        const __half dh = __float2half_rn(__bfloat162float(__float2bfloat16_rn(fminf(fmaxf(d, -kMostScale), kMostScale))));
+        uint8_t *th = tile + h * a.pool.page_bytes;
+        const int sp = pos & 15, b = in * E / 32;
+        uint8_t *at = is_k ? th + L::k_word(sp, b, in * E % 32 / 8) + in * E % 8 / 2
+                           : th + L::v_piece(sp, in * E / (D / 8)) + in * E % (D / 8) / 2;
         if constexpr (E == 4) *reinterpret_cast<uint16_t *>(at) = (uint16_t)codes;
-        else *at = (uint8_t)codes;
-        if (lane % LB == 0) *reinterpret_cast<__half *>(tile + L::k_scale(sp, b)) = dh;
-    } else {
-        const int g = E * lane / (D / 8);
-        uint8_t *at = tile + L::v_piece(sp, g) + (E * lane % (D / 8)) / 2;
-        if constexpr (E == 4) *reinterpret_cast<uint16_t *>(at) = (uint16_t)codes;
-        else *at = (uint8_t)codes;
-        if (lane % LB == 0) *reinterpret_cast<__half *>(tile + L::v_scale(sp, b)) = dh;
+        else *reinterpret_cast<uint32_t *>(at) = codes;
+        if (lane % LB == 0) *reinterpret_cast<__half *>(th + (is_k ? L::k_scale(sp, b) : L::v_scale(sp, b))) = dh;
     }
+    if (bad) atomicCAS(a.status, 0, X100_E_ARG);
 }
 
 struct ReadArgs {
     Pool pool;
     Table tab;
     const int *pos, *seq;
-    int n_tokens;
+    int n_tokens, slices;
     __half *k, *v;
     int *status;
 };
 
-// The inverse: one head of k or v of one token per warp, d * (code - 8) in fp16 (exact).
+// The inverse: a lane has 8 dims of a head (a word of codes, 16 bytes out), d * (code - 8) in fp16 (exact); warps and
+// slices as in append_kernel.
 template <int D>
 __global__ void __launch_bounds__(256) read_kernel(const ReadArgs a) {
     using L = Lay<D>;
-    constexpr int E = D / 32;
-    const int lane = threadIdx.x & 31;
-    const int kinds = (a.k ? 1 : 0) + (a.v ? 1 : 0), heads = kinds * a.pool.nkv;
+    constexpr int LH = D / 8, HW = 32 / LH;
+    const int lane = threadIdx.x & 31, in = lane % LH, hl = lane / LH, nkv = a.pool.nkv;
+    const int gk = (nkv + HW - 1) / HW, groups = gk * ((a.k ? 1 : 0) + (a.v ? 1 : 0));
     const long item = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
     pdl_launch_dependents();
     pdl_wait();
-    if (item >= (long)a.n_tokens * heads) return;
-    const int i = (int)(item / heads), r = (int)(item % heads), h = r % a.pool.nkv;
-    const bool is_k = a.k && r < a.pool.nkv;
+    if (item >= (long)a.n_tokens * a.slices) return;
+    const int i = (int)(item / a.slices), slice = (int)(item % a.slices);
     const int pos = a.pos[i];
     if (pos < 0) return;
-    const uint8_t *tile = tile_of(a.pool, a.tab, a.seq ? a.seq[i] : i, pos, h);
+    const uint8_t *tile = tile_of(a.pool, a.tab, a.seq ? a.seq[i] : i, pos, 0);
     if (!tile) {
         if (lane == 0) atomicCAS(a.status, 0, X100_E_ARG);
         return;
     }
-    const int sp = pos & 15, b = E * lane / 32, in = E * lane & 31, g = E * lane / (D / 8);
-    const uint8_t *at = is_k ? tile + L::k_word(sp, b, in >> 3) + (in & 7) / 2
-                             : tile + L::v_piece(sp, g) + (E * lane % (D / 8)) / 2;
-    const float d = __half2float(*reinterpret_cast<const __half *>(tile + (is_k ? L::k_scale(sp, b) : L::v_scale(sp, b))));
-    uint32_t codes;
-    if constexpr (E == 4) codes = *reinterpret_cast<const uint16_t *>(at);
-    else codes = *at;
-    float x[E];
+    const int sp = pos & 15, b = in / 4;
+#pragma unroll 2
+    for (int g = slice; g < groups; g += a.slices) {
+        const bool is_k = a.k && g < gk;
+        const int h = (a.k && !is_k ? g - gk : g) * HW + hl;
+        if (h >= nkv) continue;
+        const uint8_t *th = tile + h * a.pool.page_bytes;
+        const uint8_t *at = is_k ? th + L::k_word(sp, b, in & 3) : th + L::v_piece(sp, in * 8 / (D / 8)) + in * 8 % (D / 8) / 2;
+        const uint32_t codes = *reinterpret_cast<const uint32_t *>(at);
+        const float d = __half2float(*reinterpret_cast<const __half *>(th + (is_k ? L::k_scale(sp, b) : L::v_scale(sp, b))));
+        float x[8];
 #pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = d * ((int)(codes >> (4 * e) & 15) - 8);
-    store_lane<__half, E>((is_k ? a.k : a.v) + ((long)i * a.pool.nkv + h) * D, lane, x);
+        for (int e = 0; e < 8; ++e) x[e] = d * ((int)(codes >> (4 * e) & 15) - 8);
+        *reinterpret_cast<uint4 *>((is_k ? a.k : a.v) + ((long)i * nkv + h) * D + in * 8) = pack<__half, 8>(x);
+    }
+}
+
+// Warps per token: enough to fill the card when there are few tokens, one when there are many.
+inline int slices_for(const DevCtx *c, int n_tokens, int groups) {
+    const long want = ((long)c->sm_count * 32 + n_tokens - 1) / n_tokens;
+    return (int)std::max<long>(1, std::min<long>(want, groups));
 }
 
 __global__ void rope64_kernel(float2 *rope, long n, int half, double step) {
@@ -256,7 +278,7 @@ int x100q_kv4_append_dev(const x100q_kv4 *kv, const x100q_kv4_append_args *a, vo
     if (!kv->pages || !aligned16(kv->pages) || !a->k || !a->v || !a->pos || !a->page_table || a->table_stride < 1 ||
         a->n_seqs < 1 || (!a->seq && a->n_tokens > a->n_seqs) || !aligned16(a->k) || !aligned16(a->v) ||
         !pitch_ok(a->k_stride, kw, es) || !pitch_ok(a->v_stride, kw, es) || (a->rope && a->rope_len < 1) ||
-        (reinterpret_cast<uintptr_t>(a->rope) & 7) || ((a->q_norm || a->k_norm) && !(a->eps >= 0.f)))
+        !aligned16(a->rope) || ((a->q_norm || a->k_norm) && !(a->eps >= 0.f)))
         return refuse(X100_E_ARG);
     if (a->q && (a->n_heads < 1 || a->n_heads > 4096 || !a->q_out || !aligned16(a->q) || !aligned16(a->q_out) ||
                  !pitch_ok(a->q_stride, a->n_heads * kv->head_dim, es) ||
@@ -273,8 +295,9 @@ int x100q_kv4_append_dev(const x100q_kv4 *kv, const x100q_kv4_append_args *a, vo
     p.rope = reinterpret_cast<const float2 *>(a->rope), p.rope_len = a->rope_len;
     p.n_tokens = a->n_tokens, p.nh = a->q ? a->n_heads : 0;
     p.pos = a->pos, p.seq = a->seq, p.status = c->d_status;
-    const long warps = (long)p.n_tokens * (p.nh + 2 * p.pool.nkv), ctas = (warps + 7) / 8;
-    if (ctas > 0x7fffffffl) return refuse(X100_E_TOO_LARGE);
+    const int hw = 512 / (kv->head_dim * es), kvg = (p.pool.nkv + hw - 1) / hw;   // heads per warp, groups of k or v
+    p.slices = slices_for(c, p.n_tokens, (p.nh + hw - 1) / hw + 2 * kvg);
+    const long ctas = ((long)p.n_tokens * p.slices + 7) / 8;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const dim3 grid((unsigned)ctas), blk(256);
     int st;
@@ -297,10 +320,10 @@ int x100q_kv4_read_dev(const x100q_kv4 *kv, const int *pos, const int *seq, int 
         return refuse(X100_E_ARG);
     DevCtx *c = ctx();
     if (!c) return get_error();
-    ReadArgs p = {make_pool(kv), {page_table, table_stride, n_seqs}, pos, seq, n_tokens, static_cast<__half *>(k_out),
+    const int hw = 256 / kv->head_dim, groups = (kv->n_kv_heads + hw - 1) / hw * ((k_out ? 1 : 0) + (v_out ? 1 : 0));
+    ReadArgs p = {make_pool(kv), {page_table, table_stride, n_seqs}, pos, seq, n_tokens, slices_for(c, n_tokens, groups), static_cast<__half *>(k_out),
                   static_cast<__half *>(v_out), c->d_status};
-    const long warps = (long)n_tokens * kv->n_kv_heads * ((k_out ? 1 : 0) + (v_out ? 1 : 0)), ctas = (warps + 7) / 8;
-    if (ctas > 0x7fffffffl) return refuse(X100_E_TOO_LARGE);
+    const long ctas = ((long)n_tokens * p.slices + 7) / 8;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     return kv->head_dim == 128 ? launch_pdl(read_kernel<128>, dim3((unsigned)ctas), dim3(256), 0, s, p)
                                : launch_pdl(read_kernel<64>, dim3((unsigned)ctas), dim3(256), 0, s, p);

@@ -642,7 +642,7 @@ static int launch(DevCtx *c, AttnArgs &a, cudaStream_t s) {
     a.ml = reinterpret_cast<float2 *>(a.part + (size_t)kMaxCtas * 2 * R * D);
     a.meta = reinterpret_cast<int4 *>(a.ml + kMaxCtas * 2 * R);
     int st = launch_pdl(attn_kernel<T, D, NR>, dim3(grid), dim3(kWarps * 32), Cfg<D, NR>::SMEM, s, a);
-    if (st || grid == 1) return st;
+    if (st || grid == 1 || cover <= 1l << a.unit_shift) return st;   // items of one unit are never cut
     if (items * 8 >= grid) return launch_pdl(merge_kernel<T, D, NR, 1>, dim3(grid - 1, NR), dim3(kWarps * 32), 0, s, a, grid);
     return launch_pdl(merge_kernel<T, D, NR, 8>, dim3(grid - 1, NR * (D / 16)), dim3(kWarps * 32), 0, s, a, grid);
 }

@@ -513,54 +513,39 @@ def quantize_q8_0_dev(x, n: int, blocks, stream=None) -> None:
 
 
 # ---- paged 4-bit KV cache, residual RMS norm with 8-bit output (torch tensors) ---------------
-_DTYPE_ID: dict = {}   # torch dtype -> Q_F32 / Q_F16, filled with torch's first use here
-_raw_stream = None
+# A decode step calls these for every layer, so the checks are plain expressions
+# on the way through and only a failed one goes looking for its reason.
+_TORCH = None   # (torch, {dtype: Q_F32 / Q_F16}, float16, float32, int32, int8, uint8, current device, its current stream)
 
 
-def _torch_types():
-    import torch
-    _DTYPE_ID.update({torch.float32: Q_F32, torch.float16: Q_F16})
+def _torch():
+    global _TORCH
+    if _TORCH is None:
+        import torch
+        torch.cuda.current_device()   # initialises CUDA
+        _TORCH = (torch, {torch.float32: Q_F32, torch.float16: Q_F16}, torch.float16, torch.float32, torch.int32, torch.int8, torch.uint8,
+                  torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream)
+    return _TORCH
 
 
-def _dtype_id(t, what: str) -> int:
-    if not _DTYPE_ID:
-        _torch_types()
-    i = _DTYPE_ID.get(t.dtype)
-    if i is None:
-        raise X100Error(X100_E_UNSUPPORTED, f"{what}: float32 or float16 is taken, not {t.dtype}")
-    return i
+def _refuse(what: str, why: str, code: int = X100_E_ARG):
+    raise X100Error(code, f"{what}: {why}")
 
 
-def _here(stream):
-    """(current device, stream handle): the current device's current stream unless one is given."""
-    global _raw_stream
-    import torch
-    if _raw_stream is None:
-        _raw_stream = torch._C._cuda_getCurrentRawStream
-    dev = torch.cuda.current_device()
-    return dev, (_raw_stream(dev) if stream is None else _stream(stream))
+def _placed(what: str, dev: int, **named) -> None:
+    """Raise for the first of name = (tensor or None, dtype) of another type or device; integers have to be contiguous too."""
+    torch = _torch()[0]
+    for name, (t, dt) in named.items():
+        if t is not None and (t.dtype is not dt or t.get_device() != dev):
+            _refuse(what, f"{name} has to be {dt} on the current device (cuda:{dev}), not {t.dtype} on {t.device}")
+        if t is not None and dt is torch.int32 and not t.is_contiguous():
+            _refuse(what, f"{name} has to be contiguous")
 
 
-def _need(ok: bool, what: str, why: str) -> None:
-    if not ok:
-        raise X100Error(X100_E_ARG, f"{what}: {why}")
-
-
-def _take(t, name: str, what: str, dtype, dev: int) -> int:
-    """Pointer of a tensor of `dtype` on device `dev` (None: no pointer)."""
-    if t is None:
-        return 0
-    if t.dtype is not dtype or t.get_device() != dev:
-        raise X100Error(X100_E_ARG, f"{what}: {name} has to be {dtype} on the current device (cuda:{dev}), not {t.dtype} on {t.device}")
-    return t.data_ptr()
-
-
-def _heads(t, name: str, what: str, dim: int) -> int:
-    """Token stride of [tokens, heads, dim] with the heads of a token side by side."""
-    if t.is_contiguous() and t.dim() == 3 and t.shape[2] == dim:
-        return t.shape[1] * dim
+def _token_stride(t, name: str, what: str, dim: int) -> int:
+    """Token stride of [tokens, heads, dim] that is not contiguous: the heads of a token have to lie side by side."""
     if t.dim() != 3 or t.shape[2] != dim or t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != dim):
-        raise X100Error(X100_E_ARG, f"{what}: {name} has to be [tokens, heads, {dim}], a token's heads side by side")
+        _refuse(what, f"{name} has to be [tokens, heads, {dim}], a token's heads side by side")
     return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1] * dim)
 
 
@@ -570,94 +555,123 @@ class Kv4Cache:
     layout, the masks and what is out of range.  Methods allocate nothing unless an output or the scratch is left out."""
 
     def __init__(self, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, pages=None):
-        import torch
+        torch = _torch()[0]
         self.kv = Kv4(None, n_pages, page_size, n_kv_heads, head_dim)
         self._ref = C.byref(self.kv)
         n = lib().x100q_kv4_bytes(self._ref)
-        _need(n > 0, "Kv4Cache", f"no pool of {n_pages} pages of {page_size} x {n_kv_heads} x {head_dim}")
+        if n == 0:
+            _refuse("Kv4Cache", f"no pool of {n_pages} pages of {page_size} x {n_kv_heads} x {head_dim}")
         if pages is None:
             pages = torch.zeros(n, dtype=torch.uint8, device="cuda")
-        _need(pages.dtype is torch.uint8 and pages.is_cuda and pages.is_contiguous() and pages.numel() >= n, "Kv4Cache",
-              f"pages has to be {n} contiguous uint8 on a GPU")
+        if pages.dtype is not torch.uint8 or not pages.is_cuda or not pages.is_contiguous() or pages.numel() < n:
+            _refuse("Kv4Cache", f"pages has to be {n} contiguous uint8 on a GPU")
         self.pages, self.kv.pages, self.device = pages, pages.data_ptr(), pages.get_device()
         self.head_dim, self.n_kv_heads = head_dim, n_kv_heads
+        self._append, self._read, self._attn = lib().x100q_kv4_append_dev, lib().x100q_kv4_read_dev, lib().x100q_kv4_attn_dev
 
-    def _common(self, what, stream, table, **ints):
-        """Device, stream and the pointers of the int32 tensors (the page table's first)."""
-        import torch
-        dev, raw = _here(stream)
-        _need(dev == self.device, what, f"the pool is on cuda:{self.device}, the current device is cuda:{dev}")
-        _need(table.dim() == 2 and all(t is None or t.is_contiguous() for t in (table, *ints.values())), what,
-              "the page table has to be [sequences, entries], and it and the other integers contiguous")
-        return dev, raw, [_take(t, n, what, torch.int32, dev) for n, t in (("table", table), *ints.items())]
+    def _elsewhere(self, what, dev):
+        _refuse(what, f"the pool is on cuda:{self.device}, the current device is cuda:{dev}")
 
     def append(self, k, v, pos, table, seq=None, q=None, q_out=None, q_norm=None, k_norm=None, eps=1e-6, rope=None, stream=None):
         """x100q_kv4_append_dev: k, v [tokens, kv heads, dim] into the pages; returns q_out, the normed and rotated q."""
-        import torch
-        what, D, dt = "Kv4Cache.append", self.head_dim, k.dtype
-        kind = _dtype_id(k, what)
-        dev, raw, (tp, pp, sp) = self._common(what, stream, table, pos=pos, seq=seq)
-        n, kv = pos.numel(), self.n_kv_heads
-        ks, vs = _heads(k, "k", what, D), _heads(v, "v", what, D)
-        _need(k.shape[0] == n and v.shape[0] == n and k.shape[1] == kv and v.shape[1] == kv and (seq is None or seq.numel() == n), what,
-              f"k and v have to be [{n}, {kv}, {D}], and seq as long as pos")
-        qs = qos = nh = 0
+        torch, kinds, _, f32, i32_, _, _, device, current = _torch()
+        what, dev, D, KV, dt = "Kv4Cache.append", device(), self.head_dim, self.n_kv_heads, k.dtype
+        if dev != self.device:
+            self._elsewhere(what, dev)
+        kind = kinds.get(dt)
+        if kind is None:
+            _refuse(what, f"float32 or float16 is taken, not {dt}", X100_E_UNSUPPORTED)
+        if q is not None and q_out is None:
+            q_out = torch.empty(q.shape, dtype=dt, device=q.device)
+        if not (k.get_device() == dev and v.get_device() == dev and v.dtype is dt and pos.dtype is i32_ and pos.get_device() == dev and pos.is_contiguous()
+                and table.dtype is i32_ and table.get_device() == dev and table.is_contiguous()
+                and (seq is None or (seq.dtype is i32_ and seq.get_device() == dev and seq.is_contiguous()))
+                and (q is None or (q.dtype is dt and q.get_device() == dev and q_out.dtype is dt and q_out.get_device() == dev))
+                and (q_norm is None or (q_norm.dtype is f32 and q_norm.get_device() == dev)) and (k_norm is None or (k_norm.dtype is f32 and k_norm.get_device() == dev))
+                and (rope is None or (rope.dtype is f32 and rope.get_device() == dev))):
+            _placed(what, dev, k=(k, dt), v=(v, dt), q=(q, dt), q_out=(q_out, dt), q_norm=(q_norm, f32), k_norm=(k_norm, f32), rope=(rope, f32), pos=(pos, i32_),
+                    seq=(seq, i32_), table=(table, i32_))
+        n, want = pos.numel(), (pos.numel(), KV, D)
+        if not (k.shape == want and v.shape == want and table.dim() == 2 and (seq is None or seq.numel() == n)):
+            _refuse(what, f"k and v have to be {want}, the page table [sequences, entries], and seq as long as pos")
+        ks = KV * D if k.is_contiguous() else _token_stride(k, "k", what, D)
+        vs = KV * D if v.is_contiguous() else _token_stride(v, "v", what, D)
+        qp = op = qs = os_ = heads = 0
         if q is not None:
-            if q_out is None:
-                q_out = torch.empty(q.shape, dtype=dt, device=q.device)
-            qs, qos, nh = _heads(q, "q", what, D), _heads(q_out, "q_out", what, D), q.shape[1]
-            _need(q.shape[0] == n and q_out.shape == q.shape, what, f"q and q_out have to be [{n}, heads, {D}]")
-        f32 = torch.float32
-        for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
-            _need(w is None or (w.numel() == D and w.is_contiguous()), what, f"{name} has to be {D} contiguous values")
-        _need(rope is None or (rope.numel() % D == 0 and rope.is_contiguous()), what, f"rope has to be [positions, {D // 2}, 2]")
-        a = Kv4AppendArgs(kind, n, nh, _take(q, "q", what, dt, dev), _take(k, "k", what, dt, dev), _take(v, "v", what, dt, dev),
-                          _take(q_out, "q_out", what, dt, dev), qs, ks, vs, qos, _take(q_norm, "q_norm", what, f32, dev),
-                          _take(k_norm, "k_norm", what, f32, dev), eps, _take(rope, "rope", what, f32, dev),
-                          rope.numel() // D if rope is not None else 0, pp, sp, tp, table.shape[1], table.shape[0])
-        rc = lib().x100q_kv4_append_dev(self._ref, C.byref(a), raw)
+            if q.dim() != 3 or q.shape[0] != n or q.shape[2] != D or q_out.shape != q.shape:
+                _refuse(what, f"q and q_out have to be [{n}, heads, {D}]")
+            heads = q.shape[1]
+            qs = heads * D if q.is_contiguous() else _token_stride(q, "q", what, D)
+            os_ = heads * D if q_out.is_contiguous() else _token_stride(q_out, "q_out", what, D)
+            qp, op = q.data_ptr(), q_out.data_ptr()
+        if not ((q_norm is None or (q_norm.numel() == D and q_norm.is_contiguous())) and (k_norm is None or (k_norm.numel() == D and k_norm.is_contiguous()))
+                and (rope is None or (rope.numel() % D == 0 and rope.is_contiguous()))):
+            _refuse(what, f"q_norm and k_norm have to be {D} contiguous values and rope [positions, {D // 2}, 2]")
+        tn, ts = table.shape
+        a = Kv4AppendArgs(kind, n, heads, qp, k.data_ptr(), v.data_ptr(), op, qs, ks, vs, os_, 0 if q_norm is None else q_norm.data_ptr(),
+                          0 if k_norm is None else k_norm.data_ptr(), eps, 0 if rope is None else rope.data_ptr(), 0 if rope is None else rope.numel() // D,
+                          pos.data_ptr(), 0 if seq is None else seq.data_ptr(), table.data_ptr(), ts, tn)
+        rc = self._append(self._ref, C.byref(a), current(dev) if stream is None else _stream(stream))
         if rc:
             check(rc, "x100q_kv4_append_dev")
         return q_out
 
     def read(self, pos, table, seq=None, k_out=None, v_out=None, stream=None):
         """x100q_kv4_read_dev: the values (k, v) of the positions, fp16 [tokens, kv heads, dim]; both are made when neither is given."""
-        import torch
-        what, n, f16 = "Kv4Cache.read", pos.numel(), torch.float16
+        torch, _, f16, _, i32_, _, _, device, current = _torch()
+        what, dev, n = "Kv4Cache.read", device(), pos.numel()
+        if dev != self.device:
+            self._elsewhere(what, dev)
         if k_out is None and v_out is None:
             k_out, v_out = (torch.zeros(n, self.n_kv_heads, self.head_dim, dtype=f16, device=pos.device) for _ in range(2))
-        dev, raw, (tp, pp, sp) = self._common(what, stream, table, pos=pos, seq=seq)
+        if not (pos.dtype is i32_ and pos.get_device() == dev and pos.is_contiguous() and table.dtype is i32_ and table.get_device() == dev and table.is_contiguous()
+                and (seq is None or (seq.dtype is i32_ and seq.get_device() == dev and seq.is_contiguous()))
+                and (k_out is None or (k_out.dtype is f16 and k_out.get_device() == dev)) and (v_out is None or (v_out.dtype is f16 and v_out.get_device() == dev))):
+            _placed(what, dev, k_out=(k_out, f16), v_out=(v_out, f16), pos=(pos, i32_), seq=(seq, i32_), table=(table, i32_))
         size = n * self.n_kv_heads * self.head_dim
-        _need((seq is None or seq.numel() == n) and all(t is None or (t.numel() == size and t.is_contiguous()) for t in (k_out, v_out)), what,
-              f"k_out and v_out have to be {size} contiguous values, and seq as long as pos")
-        rc = lib().x100q_kv4_read_dev(self._ref, pp, sp, n, tp, table.shape[1], table.shape[0], _take(k_out, "k_out", what, f16, dev),
-                                      _take(v_out, "v_out", what, f16, dev), raw)
+        if not (table.dim() == 2 and (seq is None or seq.numel() == n) and (k_out is None or (k_out.numel() == size and k_out.is_contiguous()))
+                and (v_out is None or (v_out.numel() == size and v_out.is_contiguous()))):
+            _refuse(what, f"k_out and v_out have to be {size} contiguous values, the page table [sequences, entries], and seq as long as pos")
+        tn, ts = table.shape
+        rc = self._read(self._ref, pos.data_ptr(), 0 if seq is None else seq.data_ptr(), n, table.data_ptr(), ts, tn, 0 if k_out is None else k_out.data_ptr(),
+                        0 if v_out is None else v_out.data_ptr(), current(dev) if stream is None else _stream(stream))
         if rc:
             check(rc, "x100q_kv4_read_dev")
         return k_out, v_out
 
     def attend_work(self, n_tokens: int, n_heads: int, n_seqs: int):
         """Scratch for attend(); calls that overlap on the GPU need one each."""
-        import torch
+        torch = _torch()[0]
         return torch.empty(lib().x100q_kv4_attn_work(self._ref, n_tokens, n_heads, n_seqs), dtype=torch.uint8, device=self.pages.device)
 
     def attend(self, q, out, table, kv_len, q_start=None, max_q=1, scale=None, work=None, stream=None):
         """x100q_kv4_attn_dev: q [tokens, heads, dim] over the pages into out (made when None); q_start None: one token per sequence."""
-        import torch
-        what, D, dt = "Kv4Cache.attend", self.head_dim, q.dtype
-        kind, n = _dtype_id(q, what), kv_len.numel()
+        torch, kinds, _, _, i32_, _, u8, device, current = _torch()
+        what, dev, D, dt, n = "Kv4Cache.attend", device(), self.head_dim, q.dtype, kv_len.numel()
+        if dev != self.device:
+            self._elsewhere(what, dev)
+        kind = kinds.get(dt)
+        if kind is None:
+            _refuse(what, f"float32 or float16 is taken, not {dt}", X100_E_UNSUPPORTED)
+        if q.dim() != 3 or q.shape[2] != D:
+            _refuse(what, f"q has to be [tokens, heads, {D}]")
+        rows, heads, _ = q.shape
         if out is None:
             out = torch.empty(q.shape, dtype=dt, device=q.device)
         if work is None:
-            work = self.attend_work(q.shape[0], q.shape[1], n)
-        dev, raw, (tp, lp, qp) = self._common(what, stream, table, kv_len=kv_len, q_start=q_start)
-        qs, os_ = _heads(q, "q", what, D), _heads(out, "out", what, D)
-        rows, heads = q.shape[0], q.shape[1]
-        _need(out.shape == q.shape and table.shape[0] == n and (q_start is None or q_start.numel() == n + 1) and work.is_contiguous(), what,
-              "out has to be as q, the page table and q_start as kv_len's sequences, and work contiguous")
-        a = Kv4AttnArgs(kind, heads, _take(q, "q", what, dt, dev), _take(out, "out", what, dt, dev), qs, os_, qp, rows, max_q, lp, tp,
-                        table.shape[1], n, D ** -0.5 if scale is None else scale, _take(work, "work", what, torch.uint8, dev), work.numel())
-        rc = lib().x100q_kv4_attn_dev(self._ref, C.byref(a), raw)
+            work = self.attend_work(rows, heads, n)
+        if not (q.get_device() == dev and out.dtype is dt and out.get_device() == dev and work.dtype is u8 and work.get_device() == dev and work.is_contiguous()
+                and kv_len.dtype is i32_ and kv_len.get_device() == dev and kv_len.is_contiguous() and table.dtype is i32_ and table.get_device() == dev
+                and table.is_contiguous() and (q_start is None or (q_start.dtype is i32_ and q_start.get_device() == dev and q_start.is_contiguous()))):
+            _placed(what, dev, q=(q, dt), out=(out, dt), work=(work, u8), kv_len=(kv_len, i32_), table=(table, i32_), q_start=(q_start, i32_))
+            _refuse(what, "work has to be contiguous")
+        if not (out.shape == q.shape and table.dim() == 2 and table.shape[0] == n and (q_start is None or q_start.numel() == n + 1)):
+            _refuse(what, "out has to be as q, the page table [sequences, entries] and q_start as long as kv_len, and one more")
+        qs = heads * D if q.is_contiguous() else _token_stride(q, "q", what, D)
+        os_ = heads * D if out.is_contiguous() else _token_stride(out, "out", what, D)
+        a = Kv4AttnArgs(kind, heads, q.data_ptr(), out.data_ptr(), qs, os_, 0 if q_start is None else q_start.data_ptr(), rows, max_q, kv_len.data_ptr(),
+                        table.data_ptr(), table.shape[1], n, D ** -0.5 if scale is None else scale, work.data_ptr(), work.numel())
+        rc = self._attn(self._ref, C.byref(a), current(dev) if stream is None else _stream(stream))
         if rc:
             check(rc, "x100q_kv4_attn_dev")
         return out
@@ -665,7 +679,7 @@ class Kv4Cache:
 
 def rope_table(n_pos: int, head_dim: int, base: float, stream=None):
     """x100q_rope_table_dev: (cos, sin) [n_pos, head_dim / 2, 2] for Kv4Cache.append."""
-    import torch
+    torch = _torch()[0]
     t = torch.empty(n_pos, head_dim // 2, 2, dtype=torch.float32, device="cuda")
     check(lib().x100q_rope_table_dev(t.data_ptr(), n_pos, head_dim, base, _stream(stream)), "x100q_rope_table_dev")
     return t
@@ -673,27 +687,33 @@ def rope_table(n_pos: int, head_dim: int, base: float, stream=None):
 
 def add_rmsnorm_q8(x, w, q, scales, residual=None, residual_out=None, eps=1e-6, group=0, stream=None):
     """x100q_add_rmsnorm_q8_dev: rows of x (+ residual, the sum to residual_out) RMS-normed with w into int8 q and its scales."""
-    import torch
-    what, dt, f32 = "add_rmsnorm_q8", x.dtype, torch.float32
-    kind = _dtype_id(x, what)
-    _need(x.dim() == 2, what, "x has to be [rows, elements]")
-    rows, d = x.shape
-    dev, raw = _here(stream)
-    _need(w.numel() == d and w.is_contiguous() and scales.is_contiguous() and scales.numel() == rows * (d // group if group else 1), what,
-          f"w has to be {d} and scales [{rows}, groups] contiguous values")
-    ld = []
-    for name, t in (("x", x), ("residual", residual), ("residual_out", residual_out), ("q", q)):
+    torch, kinds, _, f32, _, i8, _, device, current = _torch()
+    what, dev, dt = "add_rmsnorm_q8", device(), x.dtype
+    kind = kinds.get(dt)
+    if kind is None:
+        _refuse(what, f"float32 or float16 is taken, not {dt}", X100_E_UNSUPPORTED)
+    if x.dim() != 2:
+        _refuse(what, "x has to be [rows, elements]")
+    if not (x.get_device() == dev and w.dtype is f32 and w.get_device() == dev and q.dtype is i8 and q.get_device() == dev and scales.dtype is f32
+            and scales.get_device() == dev and (residual is None or (residual.dtype is dt and residual.get_device() == dev))
+            and (residual_out is None or (residual_out.dtype is dt and residual_out.get_device() == dev))):
+        _placed(what, dev, x=(x, dt), residual=(residual, dt), residual_out=(residual_out, dt), w=(w, f32), q=(q, i8), scales=(scales, f32))
+    shape = x.shape
+    rows, d = shape
+    if not (w.numel() == d and w.is_contiguous() and scales.is_contiguous() and scales.numel() == rows * (d // group if group > 0 else 1)):
+        _refuse(what, f"w has to be {d} and scales [{rows}, groups] contiguous values")
+
+    def pitch(t, name):
         if t is None:
-            ld.append(0)
-        elif t.is_contiguous() and t.shape == x.shape:
-            ld.append(d)
-        else:
-            _need(t.shape == x.shape and (d == 1 or t.stride(1) == 1), what, f"{name} has to be [{rows}, {d}] with contiguous rows")
-            ld.append(t.stride(0) if rows > 1 else d)
-    a = NormQ8Args(kind, rows, d, group, _take(x, "x", what, dt, dev), _take(residual, "residual", what, dt, dev),
-                   _take(residual_out, "residual_out", what, dt, dev), *ld, _take(w, "w", what, f32, dev), eps,
-                   _take(q, "q", what, torch.int8, dev), _take(scales, "scales", what, f32, dev))
-    rc = lib().x100q_add_rmsnorm_q8_dev(C.byref(a), raw)
+            return 0
+        if t.shape != shape or (d > 1 and t.stride(1) != 1):
+            _refuse(what, f"{name} has to be [{rows}, {d}] with contiguous rows")
+        return d if rows <= 1 or t.is_contiguous() else t.stride(0)
+
+    a = NormQ8Args(kind, rows, d, group, x.data_ptr(), 0 if residual is None else residual.data_ptr(), 0 if residual_out is None else residual_out.data_ptr(),
+                   pitch(x, "x"), pitch(residual, "residual"), pitch(residual_out, "residual_out"), pitch(q, "q"), w.data_ptr(), eps, q.data_ptr(),
+                   scales.data_ptr())
+    rc = lib().x100q_add_rmsnorm_q8_dev(C.byref(a), current(dev) if stream is None else _stream(stream))
     if rc:
         check(rc, "x100q_add_rmsnorm_q8_dev")
 
