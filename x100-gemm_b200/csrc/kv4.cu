@@ -29,38 +29,43 @@ struct AppendArgs {
     int *status;
 };
 
-// 16 bytes of a head in fp32.
-template <typename T, int E>
-__device__ __forceinline__ void unpack(uint4 v, float (&x)[E]) {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    if constexpr (sizeof(T) == 4) {
+// 8 elements of a head, as loaded and in fp32.
+template <typename T>
+struct Eight {
+    uint4 v[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const T *p) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(w[i]);
-    } else {
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = *(reinterpret_cast<const uint4 *>(p) + i);
+    }
+    __device__ __forceinline__ void get(float (&x)[8]) const {
+        const uint32_t *w = reinterpret_cast<const uint32_t *>(v);
+        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(w + i));
-            x[2 * i] = f.x, x[2 * i + 1] = f.y;
+            for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(w[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(w + i));
+                x[2 * i] = f.x, x[2 * i + 1] = f.y;
+            }
         }
     }
-}
-template <typename T, int E>
-__device__ __forceinline__ uint4 pack(const float (&x)[E]) {
-    uint32_t w[4];
+    static __device__ __forceinline__ void store(T *p, const float (&x)[8]) {
+        if constexpr (sizeof(T) == 4) {
+            reinterpret_cast<float4 *>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+            reinterpret_cast<float4 *>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+        } else {
+            __half2 h[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(x[i]);
-        else {
-            const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
-            w[i] = *reinterpret_cast<const uint32_t *>(&h);
+            for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+            *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(h);
         }
     }
-    return make_uint4(w[0], w[1], w[2], w[3]);
-}
+};
 
-// A lane holds 16 bytes (E elements) of a head, so LH = D / E lanes have a head and a warp HW = 32 / LH
+// A lane holds 8 elements of a head (a K word's codes), so LH = D / 8 lanes have a head and a warp HW = 32 / LH
 // heads side by side.  An element's rotation partner (j + D / 2) is the same element of lane ^ LH / 2, and a block
-// of 32 is 32 / E neighbouring lanes.  A warp takes the groups of HW heads of one token that are its slice's
+// of 32 is 4 neighbouring lanes.  A warp takes the groups of HW heads of one token that are its slice's
 // (slice, slice + slices, ..), the next group's bytes on their way while one is worked on; the rotation's row is
 // loaded once.  Every product, sum and quotient up to the code is rounded by itself (no contraction), which
 // makes the codes the same on any machine that follows the formula.  Codes are taken before the factor
@@ -69,124 +74,119 @@ __device__ __forceinline__ uint4 pack(const float (&x)[E]) {
 template <typename T, int D>
 __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
     using L = Lay<D>;
-    constexpr int E = 16 / sizeof(T), LH = D / E, HW = 32 / LH, LB = 32 / E;   // LB lanes per block
+    constexpr int LH = D / 8, HW = 32 / LH;
     const int lane = threadIdx.x & 31, in = lane % LH, hl = lane / LH;          // place in the head, head of the group
     const int nkv = a.pool.nkv, gq = (a.nh + HW - 1) / HW, gk = (nkv + HW - 1) / HW, groups = gq + 2 * gk;
     const long item = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
     pdl_launch_dependents();
     pdl_wait();
     if (item >= (long)a.n_tokens * a.slices) return;
-    const int i = (int)(item / a.slices), slice = (int)(item % a.slices);
+    const int i = (int)(item / a.slices), slice = (int)item - i * a.slices;
     const int pos = a.pos[i];
     if (pos < 0) return;                                  // padding
     const int seq = a.seq ? a.seq[i] : i;
-    // bytes of group g for this lane; heads past the last one load nothing
-    auto fetch = [&](int g) {
-        const T *p;
-        int h;
-        if (g < gq) h = g * HW + hl, p = h < a.nh ? static_cast<const T *>(a.q) + i * a.qs : nullptr;
-        else if (g < gq + gk) h = (g - gq) * HW + hl, p = h < nkv ? static_cast<const T *>(a.k) + i * a.ks : nullptr;
-        else h = (g - gq - gk) * HW + hl, p = h < nkv ? static_cast<const T *>(a.v) + i * a.vs : nullptr;
-        return p ? *reinterpret_cast<const uint4 *>(p + (long)h * D + in * E) : make_uint4(0, 0, 0, 0);
+    // this lane's elements of group g; past the last head, the last one's
+    const T *const qb = static_cast<const T *>(a.q) + i * a.qs + in * 8, *const kb = static_cast<const T *>(a.k) + i * a.ks + in * 8,
+                  *const vb = static_cast<const T *>(a.v) + i * a.vs + in * 8;
+    auto at_group = [&](int g) {
+        const bool is_q = g < gq, is_k = g < gq + gk;
+        const int h = min((g - (is_q ? 0 : is_k ? gq : gq + gk)) * HW + hl, (is_q ? a.nh : nkv) - 1);
+        return (is_q ? qb : is_k ? kb : vb) + h * D;
     };
     int g = slice;
     if (g >= groups) return;
-    uint4 next = fetch(g);
+    Eight<T> next;
+    next.load(at_group(g));
     // the rotation's row and the token's page: a bad position or page is left out and reported
     const bool turn = a.rope != nullptr, far = turn && pos >= a.rope_len;
-    float2 cs[E];
-    if (turn && !far) {
-        const float4 *row = reinterpret_cast<const float4 *>(a.rope + (long)pos * (D / 2) + (in * E & (D / 2 - 1)));
+    float cs[8], sn[8];                                   // the sine with the sign that the lane's half takes it with
 #pragma unroll
-        for (int e = 0; e < E / 2; ++e) {
+    for (int e = 0; e < 8; ++e) cs[e] = 1.f, sn[e] = 0.f;
+    if (turn && !far) {
+        const float4 *row = reinterpret_cast<const float4 *>(a.rope + (long)pos * (D / 2) + (in * 8 & (D / 2 - 1)));
+        const float sign = in < LH / 2 ? -1.f : 1.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
             const float4 r = __ldg(row + e);
-            cs[2 * e] = make_float2(r.x, r.y), cs[2 * e + 1] = make_float2(r.z, r.w);
+            cs[2 * e] = r.x, sn[2 * e] = sign * r.y, cs[2 * e + 1] = r.z, sn[2 * e + 1] = sign * r.w;
         }
     }
     uint8_t *tile = nullptr;                              // of kv head 0
     if (g + (groups - 1 - g) / a.slices * a.slices >= gq) tile = tile_of(a.pool, a.tab, seq, pos, 0);   // the slice has k or v
-    bool bad = false;
+    bool bad = far;
+    if (far) g = groups;
     for (; g < groups; g += a.slices) {
-        float x[E], t[E];
-        unpack<T, E>(next, x);
-        if (g + a.slices < groups) next = fetch(g + a.slices);
+        float t[8];
+        next.get(t);
+        if (g + a.slices < groups) next.load(at_group(g + a.slices));
         const bool is_q = g < gq, is_k = !is_q && g < gq + gk;
-        const int h = (is_q ? g : is_k ? g - gq : g - gq - gk) * HW + hl;
-        const bool rotate = turn && (is_q || is_k);
-        if (far || (!is_q && !tile)) {
-            bad = true;
-            continue;
-        }
         float s = 1.f;
         const float *w = is_q ? a.qn : is_k ? a.kn : nullptr;
         if (w) {
             float ss = 0.f;
 #pragma unroll
-            for (int e = 0; e < E; ++e) ss += x[e] * x[e];
+            for (int e = 0; e < 8; ++e) ss = fmaf(t[e], t[e], ss);
 #pragma unroll
             for (int o = LH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            s = 1.f / sqrtf(ss / (float)D + a.eps);
+            s = 1.f / sqrtf(ss * (1.f / D) + a.eps);
 #pragma unroll
-            for (int e = 0; e < E; ++e) x[e] = __fmul_rn(x[e], __ldg(w + in * E + e));
+            for (int e = 0; e < 8; ++e) t[e] = __fmul_rn(t[e], __ldg(w + in * 8 + e));
         }
-        if (rotate) {
+        if (turn && (is_q || is_k)) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const float o = __shfl_xor_sync(0xffffffffu, x[e], LH / 2);
-                t[e] = in < LH / 2 ? __fsub_rn(__fmul_rn(x[e], cs[e].x), __fmul_rn(o, cs[e].y))
-                                   : __fadd_rn(__fmul_rn(x[e], cs[e].x), __fmul_rn(o, cs[e].y));
+            for (int e = 0; e < 8; ++e) {                 // x c - o s or x c + o s, each step rounded
+                const float o = __shfl_xor_sync(0xffffffffu, t[e], LH / 2);
+                t[e] = __fadd_rn(__fmul_rn(t[e], cs[e]), __fmul_rn(o, sn[e]));
             }
-        } else {
-#pragma unroll
-            for (int e = 0; e < E; ++e) t[e] = x[e];
         }
         if (is_q) {
-            if (w) {
+            const int h = g * HW + hl;
 #pragma unroll
-                for (int e = 0; e < E; ++e) t[e] *= s;
-            }
-            if (h < a.nh) *reinterpret_cast<uint4 *>(static_cast<T *>(a.qo) + i * a.qos + (long)h * D + in * E) = pack<T, E>(t);
+            for (int e = 0; e < 8; ++e) t[e] *= s;
+            if (h < a.nh) Eight<T>::store(static_cast<T *>(a.qo) + i * a.qos + (long)h * D + in * 8, t);
+            continue;
+        }
+        if (!tile) {
+            bad = true;
             continue;
         }
         float top = t[0], low = t[0], z = 0.f;            // z: 0, or NaN where a value is not finite
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
+        for (int e = 0; e < 8; ++e) {
             top = fmaxf(top, t[e]);
             low = fminf(low, t[e]);
             z = fmaf(t[e], 0.f, z);
         }
 #pragma unroll
-        for (int o = 1; o < LB; o <<= 1) {
+        for (int o = 1; o < 4; o <<= 1) {
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
             low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
         }
         const float m = top >= -low ? top : low;
         float inv = fabsf(m) < kTinyBlock ? 0.f : __fdiv_rn(-8.f, m);
         float d = __fmul_rn(__fmul_rn(m, -0.125f), s);
-        const uint32_t fine = __ballot_sync(0xffffffffu, z == 0.f && fabsf(d) < INFINITY);
-        const uint32_t mine = ((1u << LB) - 1u) << (lane & ~(LB - 1));
-        if (h >= nkv) continue;
+        const uint32_t fine = __ballot_sync(0xffffffffu, z == 0.f && fabsf(d) < INFINITY), mine = 15u << (lane & 28);
         if ((fine & mine) != mine) {                      // a NaN or an infinity in the block
             inv = 0.f, d = 0.f;
             bad = true;
 #pragma unroll
-            for (int e = 0; e < E; ++e) t[e] = 0.f;
+            for (int e = 0; e < 8; ++e) t[e] = 0.f;
         }
-        // x * inv + 8.5 lies in (0, 17): added to 2^23 rounding down, its floor is the low bits (8 where inv is 0)
-        uint32_t codes = 0;
+        // x * inv + 8.5 lies in (0, 17): added to 2^23 rounding down, its floor is the low bits (8 where inv is 0).
+        // The codes are summed up with the exponent's bits still on, whose sum is known.
+        uint32_t codes = 0u - 0x4b000000u;                // of the 8 shifted exponents only the first reaches the word
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const uint32_t c = __float_as_uint(__fadd_rd(__fadd_rn(__fmul_rn(t[e], inv), 8.5f), 8388608.f)) - 0x4b000000u;
-            codes |= min(c, 15u) << (4 * e);
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t c = __float_as_uint(__fadd_rd(__fadd_rn(__fmul_rn(t[e], inv), 8.5f), 8388608.f));
+            codes += min(c, 0x4b00000fu) << (4 * e);
+            if (e == 1) codes -= 0xb0000000u;             // 0x4b000000 << 4; the further ones leave the word
         }
         const __half dh = __float2half_rn(__bfloat162float(__float2bfloat16_rn(fminf(fmaxf(d, -kMostScale), kMostScale))));
+        const int h = (g - (is_k ? gq : gq + gk)) * HW + hl, sp = pos & 15, b = in / 4;
+        if (h >= nkv) continue;
         uint8_t *th = tile + h * a.pool.page_bytes;
-        const int sp = pos & 15, b = in * E / 32;
-        uint8_t *at = is_k ? th + L::k_word(sp, b, in * E % 32 / 8) + in * E % 8 / 2
-                           : th + L::v_piece(sp, in * E / (D / 8)) + in * E % (D / 8) / 2;
-        if constexpr (E == 4) *reinterpret_cast<uint16_t *>(at) = (uint16_t)codes;
-        else *reinterpret_cast<uint32_t *>(at) = codes;
-        if (lane % LB == 0) *reinterpret_cast<__half *>(th + (is_k ? L::k_scale(sp, b) : L::v_scale(sp, b))) = dh;
+        *reinterpret_cast<uint32_t *>(is_k ? th + L::k_word(sp, b, in & 3) : th + L::v_piece(sp, in * 8 / (D / 8)) + in * 8 % (D / 8) / 2) = codes;
+        if ((lane & 3) == 0) *reinterpret_cast<__half *>(th + (is_k ? L::k_scale(sp, b) : L::v_scale(sp, b))) = dh;
     }
     if (bad) atomicCAS(a.status, 0, X100_E_ARG);
 }
@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(256) read_kernel(const ReadArgs a) {
         float x[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = d * ((int)(codes >> (4 * e) & 15) - 8);
-        *reinterpret_cast<uint4 *>((is_k ? a.k : a.v) + ((long)i * nkv + h) * D + in * 8) = pack<__half, 8>(x);
+        Eight<__half>::store((is_k ? a.k : a.v) + ((long)i * nkv + h) * D + in * 8, x);
     }
 }
 
@@ -295,7 +295,7 @@ int x100q_kv4_append_dev(const x100q_kv4 *kv, const x100q_kv4_append_args *a, vo
     p.rope = reinterpret_cast<const float2 *>(a->rope), p.rope_len = a->rope_len;
     p.n_tokens = a->n_tokens, p.nh = a->q ? a->n_heads : 0;
     p.pos = a->pos, p.seq = a->seq, p.status = c->d_status;
-    const int hw = 512 / (kv->head_dim * es), kvg = (p.pool.nkv + hw - 1) / hw;   // heads per warp, groups of k or v
+    const int hw = 256 / kv->head_dim, kvg = (p.pool.nkv + hw - 1) / hw;   // heads per warp, groups of k or v
     p.slices = slices_for(c, p.n_tokens, (p.nh + hw - 1) / hw + 2 * kvg);
     const long ctas = ((long)p.n_tokens * p.slices + 7) / 8;
     cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -21,7 +21,7 @@ constexpr int kWarps = 8;
 // A run's share of the list, found by one whole warp: its units, and the
 // sequence holding the first with the units before it.
 struct Share {
-    uint32_t u0, u1, before;
+    uint32_t u0, u1, before, per;        // per: units of every run but the last
     int b;
 };
 __device__ __forceinline__ Share my_share(const AttnArgs &a, int R) {
@@ -38,7 +38,7 @@ __device__ __forceinline__ Share my_share(const AttnArgs &a, int R) {
         if (lane >= o) incl += up;
     }
     const uint32_t U = __reduce_add_sync(0xffffffffu, n), per = (U + gridDim.x - 1) / gridDim.x;
-    Share s = {0, 0, 0, 0};
+    Share s = {0, 0, 0, per, 0};
     if (per * blockIdx.x >= U) return s;     // the longest run is as long as with more, shorter ones; fewer items are cut
     s.u0 = per * blockIdx.x, s.u1 = min(U, s.u0 + per);
     uint32_t base = 0;
@@ -523,7 +523,10 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
                     if (k == 0 && g == 0)
 #pragma unroll
                         for (int i = 0; i < 2; ++i) a.ml[(long)slot * R + nr * 8 + 2 * t + i] = make_float2(M[i], Ls[i]);
-                    if (nr == 0 && threadIdx.x == 0) a.meta[slot] = make_int4((int)(before + item * sq.cu), b, kvh, rt | (c0 ? kInside : 0));
+                    if (nr == 0 && threadIdx.x == 0) {
+                        const uint32_t ua = before + item * sq.cu;
+                        a.meta[slot] = make_int4((int)ua, b, kvh | (int)((ua + sq.cu - 1) / s_share.per) << 16, rt | (c0 ? kInside : 0));
+                    }
                 }
             }
             if (nr == NR - 1) fence_proxy_async_smem();   // the next copies into the ring come after these accesses
@@ -535,90 +538,89 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
 }
 
 // Joins at the first cut inside an item the partials of all runs that share the
-// item, in a fixed order.  What each run left is in its meta entries, so that the many cuts
-// with nothing to do leave after one round of loads.  PW warps share the runs of
+// item, in a fixed order.  What each run left, and the last run of its item, is in its meta
+// entries, so that the many cuts with nothing to do leave after one round of loads.  PW warps share the runs of
 // one 16-dim fragment, 8 / PW fragments per CTA: with few items each is cut into
 // many parts and the loads of one warp would follow each other; with many items the CTAs would.
 template <typename T, int D, int NR, int PW>
-__global__ void __launch_bounds__(kWarps * 32) merge_kernel(const AttnArgs a, int grid) {
+__global__ void __launch_bounds__(kWarps * 32) merge_kernel(const AttnArgs a) {
     constexpr int R = 8 * NR, MT = D / 16, KC = kWarps / PW, NY = (MT + KC - 1) / KC;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int nr = blockIdx.y / NY, k = blockIdx.y % NY * KC + warp / PW, w = warp % PW;
-    __shared__ float2 s_ml[kMaxCtas][8];
-    __shared__ float4 s_o[kWarps][32];
-    __shared__ float s_l[kWarps][8];
+    __shared__ float4 s_o[kWarps][32], s_ml[kWarps][4];
     pdl_launch_dependents();
     pdl_wait();
     const int c = blockIdx.x + 1;                            // the cut before run c
-    const int4 here = __ldcg(a.meta + 2 * c);
-    const int4 p0 = __ldcg(a.meta + 2 * c - 2), p1 = __ldcg(a.meta + 2 * c - 1);
+    const int4 here = __ldcg(a.meta + 2 * c), p0 = __ldcg(a.meta + 2 * c - 2), p1 = __ldcg(a.meta + 2 * c - 1);
     if (here.x == -1 || !(here.w & kInside)) return;         // run c starts with an item of its own
     int slot0 = 2 * c - 1;                                   // the item's first part, where it lies in run c - 1
     if (p1.x != here.x) {
         if (p0.x != here.x || (p0.w & kInside)) return;      // an earlier cut joins this item
         slot0 = 2 * c - 2;
     }
-    int last = c;                                            // the last run with a part of the item
-    for (int i = c + 1; i < grid; i += 32) {
-        const int4 x = i + lane < grid ? __ldcg(a.meta + 2 * (i + lane)) : make_int4(-1, 0, 0, 0);
-        const uint32_t out = __ballot_sync(0xffffffffu, x.x != here.x || !(x.w & kInside));
-        last += out ? __ffs(out) - 1 : 32;
-        if (out) break;
-    }
-    const int b = here.y, kvh = here.z, rt = here.w & (kInside - 1), np = last - c + 2;
-    for (int e = threadIdx.x; e < np * 8; e += kWarps * 32) {
-        const int slot = e < 8 ? slot0 : 2 * (c - 1 + e / 8);
-        s_ml[e / 8][e % 8] = __ldcg(a.ml + (long)slot * R + nr * 8 + e % 8);
-    }
+    const int b = here.y, kvh = here.z & 0xffff, rt = here.w & (kInside - 1), np = (here.z >> 16) - c + 2;
     const int q0 = a.q_start ? a.q_start[b] : b;
     const int rows = min(R, (a.q_start ? a.q_start[b + 1] - q0 : 1) * a.G - rt * R);
-    __syncthreads();
-    if (nr * 8 >= rows) return;
+    // each warp its parts, four loads under way at a time, with a running max of its own
     float M[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    for (int p = g; p < np; p += 8)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) M[i] = fmaxf(M[i], s_ml[p][2 * t + i].x);
-#pragma unroll
-    for (int sh = 4; sh < 32; sh <<= 1)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) M[i] = fmaxf(M[i], __shfl_xor_sync(0xffffffffu, M[i], sh));
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     if (k < MT) {
-#pragma unroll 4
-        for (int p = w; p < np; p += PW) {
-            const int slot = p == 0 ? slot0 : 2 * (c - 1 + p);
-            const float4 y = __ldcg(reinterpret_cast<const float4 *>(a.part) + ((long)slot * NR + nr) * MT * 32 + k * 32 + lane);
-            float f[2];
+        for (int p = w; p < np; p += 4 * PW) {
+            float4 y[4];
+            float4 ml[4];                                    // (m, l) of rows 2 t, 2 t + 1
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const float2 ml = s_ml[p][2 * t + i];
-                f[i] = M[i] == -INFINITY ? 0.f : ex2(ml.x - M[i]);
-                l[i] = fmaf(ml.y, f[i], l[i]);
+            for (int j = 0; j < 4; ++j) {
+                const int pj = p + j * PW;
+                const int slot = pj == 0 ? slot0 : 2 * (c - 1 + pj);
+                const bool on = pj < np;
+                y[j] = on ? __ldcg(reinterpret_cast<const float4 *>(a.part) + ((long)slot * NR + nr) * MT * 32 + k * 32 + lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+                ml[j] = on ? __ldcg(reinterpret_cast<const float4 *>(a.ml + (long)slot * R + nr * 8 + 2 * t)) : make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
             }
-            x.x = fmaf(y.x, f[0], x.x), x.y = fmaf(y.y, f[1], x.y);
-            x.z = fmaf(y.z, f[0], x.z), x.w = fmaf(y.w, f[1], x.w);
+            const float mn[2] = {fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), M[0]),
+                                 fmaxf(fmaxf(fmaxf(ml[0].z, ml[1].z), fmaxf(ml[2].z, ml[3].z)), M[1])};
+            const float b0 = mn[0] == -INFINITY ? 0.f : mn[0], b1 = mn[1] == -INFINITY ? 0.f : mn[1];
+            const float f0 = ex2(M[0] - b0), f1 = ex2(M[1] - b1);
+            M[0] = mn[0], M[1] = mn[1];
+            o.x *= f0, o.y *= f1, o.z *= f0, o.w *= f1, l[0] *= f0, l[1] *= f1;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float h0 = ex2(ml[j].x - b0), h1 = ex2(ml[j].z - b1);
+                l[0] = fmaf(ml[j].y, h0, l[0]), l[1] = fmaf(ml[j].w, h1, l[1]);
+                o.x = fmaf(y[j].x, h0, o.x), o.y = fmaf(y[j].y, h1, o.y), o.z = fmaf(y[j].z, h0, o.z), o.w = fmaf(y[j].w, h1, o.w);
+            }
         }
     }
     if constexpr (PW > 1) {
-        s_o[warp][lane] = x;
-        if (g == 0) s_l[warp][2 * t] = l[0], s_l[warp][2 * t + 1] = l[1];
+        s_o[warp][lane] = o;
+        if (g == 0) s_ml[warp][t] = make_float4(M[0], l[0], M[1], l[1]);
         __syncthreads();
         if (w) return;
+        float4 ml[PW];
+        float b0 = -INFINITY, b1 = -INFINITY;
 #pragma unroll
-        for (int i = 1; i < PW; ++i) {
+        for (int i = 0; i < PW; ++i) {
+            ml[i] = s_ml[warp + i][t];
+            b0 = fmaxf(b0, ml[i].x), b1 = fmaxf(b1, ml[i].z);
+        }
+        b0 = b0 == -INFINITY ? 0.f : b0, b1 = b1 == -INFINITY ? 0.f : b1;
+        o = make_float4(0.f, 0.f, 0.f, 0.f);
+        l[0] = l[1] = 0.f;
+#pragma unroll
+        for (int i = 0; i < PW; ++i) {
             const float4 y = s_o[warp + i][lane];
-            x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
-            l[0] += s_l[warp + i][2 * t], l[1] += s_l[warp + i][2 * t + 1];
+            const float h0 = ex2(ml[i].x - b0), h1 = ex2(ml[i].z - b1);
+            l[0] = fmaf(ml[i].y, h0, l[0]), l[1] = fmaf(ml[i].w, h1, l[1]);
+            o.x = fmaf(y.x, h0, o.x), o.y = fmaf(y.y, h1, o.y), o.z = fmaf(y.z, h0, o.z), o.w = fmaf(y.w, h1, o.w);
         }
     }
-    if (k >= MT) return;
+    if (k >= MT || nr * 8 >= rows) return;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int rr = nr * 8 + 2 * t + i;
         if (rr >= rows) continue;
         const int r = rt * R + rr, tok = div_g(a, r);
         const float inv = l[i] > 0.f ? 1.f / l[i] : 0.f;
-        const float y0 = (i ? x.y : x.x) * inv, y1 = (i ? x.w : x.z) * inv;
+        const float y0 = (i ? o.y : o.x) * inv, y1 = (i ? o.w : o.z) * inv;
         T *p = static_cast<T *>(a.out) + (long)(q0 + tok) * a.os + (long)(kvh * a.G + r - tok * a.G) * D + g * (D / 8) + 2 * k;
         if constexpr (sizeof(T) == 4) *reinterpret_cast<float2 *>(p) = make_float2(y0, y1);
         else *reinterpret_cast<__half2 *>(p) = __floats2half2_rn(y0, y1);
@@ -643,8 +645,8 @@ static int launch(DevCtx *c, AttnArgs &a, cudaStream_t s) {
     a.meta = reinterpret_cast<int4 *>(a.ml + kMaxCtas * 2 * R);
     int st = launch_pdl(attn_kernel<T, D, NR>, dim3(grid), dim3(kWarps * 32), Cfg<D, NR>::SMEM, s, a);
     if (st || grid == 1 || cover <= 1l << a.unit_shift) return st;   // items of one unit are never cut
-    if (items * 8 >= grid) return launch_pdl(merge_kernel<T, D, NR, 1>, dim3(grid - 1, NR), dim3(kWarps * 32), 0, s, a, grid);
-    return launch_pdl(merge_kernel<T, D, NR, 8>, dim3(grid - 1, NR * (D / 16)), dim3(kWarps * 32), 0, s, a, grid);
+    if (items * 8 >= grid) return launch_pdl(merge_kernel<T, D, NR, 1>, dim3(grid - 1, NR), dim3(kWarps * 32), 0, s, a);
+    return launch_pdl(merge_kernel<T, D, NR, 8>, dim3(grid - 1, NR * (D / 16)), dim3(kWarps * 32), 0, s, a);
 }
 
 template <typename T, int D>

@@ -28,7 +28,7 @@ struct AttnArgs {
     // work: of the first (slot 0) and last (slot 1) item that a run has a part of only
     float *part;                         // [kMaxCtas][2][8 NR * D] o in fragment order
     float2 *ml;                          // [kMaxCtas][2][8 NR] running max (log2 units) and sum
-    int4 *meta;                          // [kMaxCtas][2] the item: first unit, sequence, kv head, row tile | kInside; or -1
+    int4 *meta;                          // [kMaxCtas][2] the item: first unit, sequence, kv head (kv4_attn.cu: | its last run << 16), row tile | kInside; or -1
     int *status;
 };
 
