@@ -17,6 +17,7 @@ namespace x100 {
 namespace kv4 {
 
 constexpr int kWarps = 8;
+constexpr int kLead = 3;                // units (of 128 positions) that starting an item costs: 2 and 5 measured alike, 0 5 % slower
 
 // A run's share of the list, found by one whole warp: its units, and the
 // sequence holding the first with the units before it.
@@ -153,8 +154,12 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
             before += sq.units;
             sq = load_seq(a, ++b, R, false);
         }
-        const uint32_t off = u - before, item = off / (uint32_t)sq.cu;
-        const int c0 = (int)(off - item * sq.cu), c1 = (int)min((uint32_t)sq.cu, c0 + (u1 - u));
+        // `lead` units stand for starting an item (queries, an empty ring, joining the warps): a run that ends among them
+        // has none of the item's positions
+        const uint32_t iu = sq.cu + a.lead, off = u - before, item = off / iu, k0u = off - item * iu, k1u = min(iu, k0u + (u1 - u));
+        const int c0 = max(0, (int)k0u - a.lead), c1 = max(0, (int)k1u - a.lead);
+        u += k1u - k0u;
+        if (c1 == c0) continue;
         const int kvh = sq.nrt == 1 ? (int)item : (int)(item / (uint32_t)sq.nrt), rt = row_tile((int)(item - (uint32_t)kvh * sq.nrt), sq.nrt);
         const int rows = min(R, sq.nq * a.G - rt * R);                   // live rows of the tile
         const int first = sq.len - sq.nq;                               // position of token 0
@@ -524,15 +529,14 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
 #pragma unroll
                         for (int i = 0; i < 2; ++i) a.ml[(long)slot * R + nr * 8 + 2 * t + i] = make_float2(M[i], Ls[i]);
                     if (nr == 0 && threadIdx.x == 0) {
-                        const uint32_t ua = before + item * sq.cu;
-                        a.meta[slot] = make_int4((int)ua, b, kvh | (int)((ua + sq.cu - 1) / s_share.per) << 16, rt | (c0 ? kInside : 0));
+                        const uint32_t ua = before + item * iu;
+                        a.meta[slot] = make_int4((int)ua, b, kvh | (int)((ua + iu - 1) / s_share.per) << 16, rt | (c0 ? kInside : 0));
                     }
                 }
             }
             if (nr == NR - 1) fence_proxy_async_smem();   // the next copies into the ring come after these accesses
             __syncthreads();
         }
-        u += c1 - c0;
         ++nseg;
     }
 }
@@ -638,8 +642,9 @@ static int launch(DevCtx *c, AttnArgs &a, cudaStream_t s) {
     const long nrt = ((long)a.max_q * a.G + R - 1) / R, cover = std::min(0x7fffffffl, (long)a.tab.stride << a.pool.page_shift);
     const long items = (long)a.tab.n_seqs * a.pool.nkv * nrt;
     a.unit_shift = 7;
-    while (items * ((cover >> a.unit_shift) + 1) > 0x7fffffffl) ++a.unit_shift;   // items <= 2^24: ends by 25
-    const long most = std::min<long>(items, kMaxCtas) * ((cover >> a.unit_shift) + 1);
+    a.lead = kLead;
+    while (items * ((cover >> a.unit_shift) + 1 + a.lead) > 0x7fffffffl) ++a.unit_shift;   // items <= 2^24: ends by 25
+    const long most = std::min<long>(items, kMaxCtas) * ((cover >> a.unit_shift) + 1 + a.lead);
     const int grid = (int)std::min<long>(std::min(kMaxCtas, c->sm_count * (NR == 1 ? 2 : 1)), most);
     a.ml = reinterpret_cast<float2 *>(a.part + (size_t)kMaxCtas * 2 * R * D);
     a.meta = reinterpret_cast<int4 *>(a.ml + kMaxCtas * 2 * R);

@@ -24,6 +24,7 @@ struct AttnArgs {
     int n_tokens, max_q, nh, G;
     uint32_t g_mul;                      // ceil(2^32 / G): n / G = umulhi(n, g_mul) for n < 2^32 / G
     int unit_shift;                      // positions per unit, a power of two (128 unless the list would pass 2^31 units)
+    int lead;                            // units that an item counts for besides its positions' (see kv4_attn.cu)
     float sl;                            // scale * log2(e)
     // work: of the first (slot 0) and last (slot 1) item that a run has a part of only
     float *part;                         // [kMaxCtas][2][8 NR * D] o in fragment order
@@ -39,11 +40,11 @@ constexpr int kInside = 1 << 30;         // the run starts inside the item
 __device__ __forceinline__ int div_g(const AttnArgs &a, int n) { return a.G == 1 ? n : (int)__umulhi((uint32_t)n, a.g_mul); }
 
 // ---- the work list -------------------------------------------------------------
-// Sequence b: first row of q, tokens, positions; `cu` units of every (kv head, row
+// Sequence b: first row of q, tokens, positions; `cu` units of positions in every (kv head, row
 // tile) item, at least one so that rows without positions are written.
 struct Seq {
     int q0, nq, len, nrt, cu;
-    uint32_t units;                      // of all its items
+    uint32_t units;                      // of all its items, each cu + lead
 };
 __device__ __forceinline__ Seq load_seq(const AttnArgs &a, int b, int R, bool report) {
     Seq s;
@@ -59,7 +60,7 @@ __device__ __forceinline__ Seq load_seq(const AttnArgs &a, int b, int R, bool re
     }
     s.nrt = (int)((unsigned)(s.nq * a.G + R - 1) / (unsigned)R);
     s.cu = max(1, (s.len >> a.unit_shift) + ((s.len & ((1 << a.unit_shift) - 1)) != 0));
-    s.units = (uint32_t)a.pool.nkv * s.nrt * s.cu;
+    s.units = (uint32_t)a.pool.nkv * s.nrt * (s.cu + a.lead);
     return s;
 }
 // ---- values ---------------------------------------------------------------------

@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(Roles<T>::THREADS, 1) prefill_kernel(const Att
     if (wg < 2) {
         // ================================ softmax ================================
         // registers: the launch's 65536 (512 threads of 128) or 61440 (640 of 96) shared out anew
-        regs_more<HL ? 160 : 176>();
+        regs_more<HL ? 168 : 192>();
         const int X = wg, row = threadIdx.x & 127;
         const uint32_t toff = (uint32_t)((warp & 3) * 32) << 16, sx = tS + 128 * X + toff, ox = tO + 128 * X + toff;
         uint32_t step = 0, joins = 0;            // steps of this X, meetings of the two groups so far
@@ -422,38 +422,40 @@ __global__ void __launch_bounds__(Roles<T>::THREADS, 1) prefill_kernel(const Att
             const float inv = whole ? (l > 0.f ? 1.f / l : 0.f) : 1.f;
             const float f0 = HL ? (X ? fo : f) : 1.f, f1 = HL ? (X ? f : fo) : 0.f;
             T *op = static_cast<T *>(a.out) + (long)(w.q0 + tok) * a.os + (long)(w.kvh * a.G + r - tok * a.G) * D;
+            // every round trip to tensor memory takes some hundred cycles: 64 columns at a time, 16 where two sums' are held
+            constexpr int CW = HL ? 16 : 64;
 #pragma unroll
-            for (int j = 0; j < (HL ? D / 32 : D / 16); ++j) {
-                const int i = HL ? X * (D / 32) + j : j;
-                uint32_t v[16], v1[HL ? 16 : 1];
-                tmem_ld16((HL ? tO + toff : ox) + 16 * i, v);
+            for (int j = 0; j < (HL ? D / 2 : D) / CW; ++j) {
+                const int col = (HL ? X * (D / 2) : 0) + j * CW;
+                float o[CW], o1[HL ? CW : 1];
+#pragma unroll
+                for (int k = 0; k < CW; k += 16) tmem_ld16((HL ? tO + toff : ox) + col + k, *reinterpret_cast<uint32_t(*)[16]>(o + k));
                 if constexpr (HL) {
-                    if (two) tmem_ld16(tO + 128 + toff + 16 * i, v1);
+                    if (two) tmem_ld16(tO + 128 + toff + col, *reinterpret_cast<uint32_t(*)[16]>(o1));
                 }
                 tmem_wait_ld();
-                float o[16];
 #pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                    o[k] = __uint_as_float(v[k]) * f0;
+                for (int k = 0; k < CW; ++k) {
+                    o[k] *= f0;
                     if constexpr (HL) {
-                        if (two) o[k] = fmaf(__uint_as_float(v1[k]), f1, o[k]);
+                        if (two) o[k] = fmaf(o1[k], f1, o[k]);
                     }
                 }
                 if (!whole) {
-                    float4 *pp = reinterpret_cast<float4 *>(a.part) + (long)slot * kPfRows * (D / 4) + prow;
+                    float4 *pp = reinterpret_cast<float4 *>(a.part) + ((long)slot * (D / 4) + col / 4) * kPfRows + prow;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) pp[(4 * i + k) * kPfRows] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+                    for (int k = 0; k < CW / 4; ++k) pp[k * kPfRows] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
                 } else if (live) {
                     // columns 0 .. 7 of a group of 8 are its dims 0, 4, 1, 5, 2, 6, 3, 7
 #pragma unroll
-                    for (int h = 0; h < 16; h += 8) {
+                    for (int h = 0; h < CW; h += 8) {
                         const float y[8] = {o[h] * inv, o[h + 2] * inv, o[h + 4] * inv, o[h + 6] * inv,
                                             o[h + 1] * inv, o[h + 3] * inv, o[h + 5] * inv, o[h + 7] * inv};
                         if constexpr (HL) {
-                            *reinterpret_cast<float4 *>(op + 16 * i + h) = make_float4(y[0], y[1], y[2], y[3]);
-                            *reinterpret_cast<float4 *>(op + 16 * i + h + 4) = make_float4(y[4], y[5], y[6], y[7]);
+                            *reinterpret_cast<float4 *>(op + col + h) = make_float4(y[0], y[1], y[2], y[3]);
+                            *reinterpret_cast<float4 *>(op + col + h + 4) = make_float4(y[4], y[5], y[6], y[7]);
                         } else {
-                            *reinterpret_cast<uint4 *>(op + 16 * i + h) =
+                            *reinterpret_cast<uint4 *>(op + col + h) =
                                 make_uint4(u32(__floats2half2_rn(y[0], y[1])), u32(__floats2half2_rn(y[2], y[3])),
                                            u32(__floats2half2_rn(y[4], y[5])), u32(__floats2half2_rn(y[6], y[7])));
                         }
@@ -470,7 +472,7 @@ __global__ void __launch_bounds__(Roles<T>::THREADS, 1) prefill_kernel(const Att
         }
     } else if (warp < W::kMma) {
         // ================================ codes -> fp16 tiles ================================
-        regs_less<HL ? 56 : 96>();
+        regs_less<HL ? 48 : 72>();
         const Exponents expo;
         const int th = threadIdx.x - 256;
         uint32_t tile = 0, raw = 0;                // key tiles, raw stages so far
@@ -556,7 +558,7 @@ __global__ void __launch_bounds__(Roles<T>::THREADS, 1) prefill_kernel(const Att
             }
         }
     } else {
-        regs_less<HL ? 48 : 64>();
+        regs_less<HL ? 48 : 56>();
         if (warp == W::kMma) {
             // ================================ products ================================
             const uint32_t lead = lane == 0 ? 1u : 0u;
@@ -773,7 +775,7 @@ static int launch_pf(DevCtx *c, AttnArgs &a, cudaStream_t s) {
     const int grid = (int)std::min<long>(std::min(kPfCtas, c->sm_count), most);
     a.ml = reinterpret_cast<float2 *>(a.part + (size_t)kPfCtas * 2 * kPfRows * D);
     a.meta = reinterpret_cast<int4 *>(a.ml + kPfCtas * 2 * kPfRows);
-    a.unit_shift = 7;
+    a.unit_shift = 7, a.lead = 0;
     int st = launch_pdl(prefill_kernel<T, D>, dim3(grid), dim3(Roles<T>::THREADS), Pf<D>::SMEM, s, a);
     if (st || grid == 1) return st;
     return launch_pdl(prefill_merge_kernel<T, D>, dim3(grid - 1, D / 16), dim3(kPfRows), 0, s, a, grid);
