@@ -338,6 +338,19 @@ typedef struct {
  * set_output.  head_dim must be 128, n_heads / n_kv_heads <= 8, d and
  * n_heads * head_dim multiples of 256, ctx <= 131072.                       */
 x100q_model *x100q_model_create(const x100q_model_cfg *cfg);
+/* The same with k and v in the caller's 4-bit pages (x100q_kv4) instead of fp16
+ * caches.  kv->pages is n_layers pools of x100q_kv4_bytes(kv) one behind
+ * another, layer 0's first; kv->n_kv_heads and head_dim are the model's.
+ * page_table [max_batch][table_stride] (device) serves every layer; its row b is
+ * slot b.  Pages and table are the caller's, stay where they are while the model
+ * lives, and may be read and written between steps: a slot takes another
+ * sequence, or gets another page, by changing its row.
+ * A step takes pos < 0 as a padding token: nothing is stored for it, and its
+ * logits mean nothing.  A position >= ctx, or one that the table does not cover,
+ * makes the next synchronising call report X100_E_ARG.  x100q_model_kv_copy
+ * is refused (X100_E_UNSUPPORTED): x100q_kv4_read_dev reads a layer's pool.  */
+x100q_model *x100q_model_create_kv4(const x100q_model_cfg *cfg, const x100q_kv4 *kv,
+                                    const int *page_table, int table_stride);
 void         x100q_model_destroy(x100q_model *m);
 
 /* Weights of one layer (host or device pointers, uploaded once):
@@ -541,6 +554,9 @@ int x100q_gguf_model_cfg(const x100q_gguf *g, x100q_model_cfg *cfg);
  * output.weight ties the lm_head to the token embeddings (Q8_0 of them,
  * qwen_moe_q3k.c:1747-1750).  NULL + x100_last_error() on failure.         */
 x100q_model *x100q_model_load_gguf(const x100q_gguf *g, const x100q_model_cfg *cfg);
+/* The same into a model with a paged 4-bit cache (x100q_model_create_kv4).  */
+x100q_model *x100q_model_load_gguf_kv4(const x100q_gguf *g, const x100q_model_cfg *cfg, const x100q_kv4 *kv,
+                                       const int *page_table, int table_stride);
 
 /* Device decoders used by the loader, asynchronous on `stream`:
  * n elements of GGUF `type` data (device pointer, n a whole number of

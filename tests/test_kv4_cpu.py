@@ -102,3 +102,21 @@ def test_reference_scales_make_fp16_values():
     d = ref.scale16(np.concatenate([np.float32(2.0) ** np.arange(-30, 14), np.random.default_rng(0).normal(size=4000) * 10.0 ** np.arange(-4, 4).repeat(500)]))
     v = d.astype(np.float64)[:, None] * np.arange(-8, 8)
     assert np.array_equal(v.astype(np.float16).astype(np.float64), v)
+
+
+MODEL = dict(n_layers=1, d=512, n_heads=16, n_kv_heads=2, head_dim=128, vocab=64, n_exp=8, n_act=2, moe_ffn=256, attn_qtype=x100b.Q8_0,
+             expert_qtype=x100b.Q8_0, lm_qtype=x100b.Q8_0, ctx=64, max_batch=2, expert_lo=0, expert_hi=8, rope_base=1e6, eps=1e-6)
+
+
+@pytest.mark.parametrize("pool", [dict(n_kv_heads=4), dict(head_dim=64), dict(pages=0), dict(pages=P + 8), dict(page_size=8), dict(n_pages=0)])
+def test_model_refuses_another_pool(pool):
+    L, cfg = x100b.lib(), x100b.ModelCfg(**MODEL)
+    assert L.x100q_model_create_kv4(C.byref(cfg), C.byref(kv(**pool)), P, 2) is None
+    assert x100b.last_error() == x100b.X100_E_ARG
+
+
+def test_model_refuses_no_pool_or_table():
+    L, cfg = x100b.lib(), x100b.ModelCfg(**MODEL)
+    for args in ((None, P, 2), (C.byref(kv()), None, 2), (C.byref(kv()), P, 0)):
+        assert L.x100q_model_create_kv4(C.byref(cfg), *args) is None and x100b.last_error() == x100b.X100_E_ARG
+    assert L.x100q_model_load_gguf_kv4(None, C.byref(cfg), C.byref(kv()), P, 2) is None and x100b.last_error() == x100b.X100_E_ARG

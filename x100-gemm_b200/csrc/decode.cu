@@ -23,6 +23,9 @@
 // KV cache: fp16, [layer][slot][kv_head][ctx][head_dim] for K and for V, so
 // the positions a CTA attends over are one contiguous byte range per head
 // (the reference's head-major layout, qwen_moe_q3k.c:1868-1880, in fp16).
+// A model made with x100q_model_create_kv4 keeps k and v in the caller's pages
+// of 4-bit codes instead; its step 2 is kv4.cu's append and kv4_attn.cu's or
+// kv4_prefill.cu's attention (kv4_step).
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -32,6 +35,7 @@
 #include <vector>
 
 #include "../../include/x100q.h"
+#include "kv4_attn.cuh"
 #include "moe.h"
 #include "qgemm.h"
 #include "qgemv.h"
@@ -614,6 +618,13 @@ struct x100q_model {
     void *moe_scratch = nullptr;
     MoeScratch S;
     int nsplit_max = 0;
+    // paged 4-bit cache (x100q_model_create_kv4); then no kc, vc or part
+    bool paged = false;
+    x100q_kv4 kv4 = {};                    // of layer 0; the layers' pools lie one behind another
+    size_t kv4_layer = 0;                  // bytes per layer
+    const int *kv4_table = nullptr;        // [max_batch][kv4_stride]
+    int kv4_stride = 0;
+    void *kv4_work = nullptr;
     // many-token prefill (chunks of up to pf_tmax tokens on the tensor-core
     // GEMMs), allocated on first use
     void *pf_base = nullptr;
@@ -623,6 +634,8 @@ struct x100q_model {
     int pf_kp = 0;
     MoeBigScratch pf_moe;
 };
+
+constexpr int kPrefillChunkMax = 4096;   // X100_PREFILL_CHUNK's largest
 
 static bool cfg_ok(const x100q_model_cfg *c) {
     if (!c) return false;
@@ -641,9 +654,14 @@ static int qkv_rows(const x100q_model_cfg &c) { return (c.n_heads + 2 * c.n_kv_h
 
 extern "C" {
 
-x100q_model *x100q_model_create(const x100q_model_cfg *cfg) {
+static x100q_model *create_model(const x100q_model_cfg *cfg, const x100q_kv4 *kv4, const int *page_table, int table_stride) {
     set_error(X100_OK);
     if (!cfg_ok(cfg)) {
+        set_error(X100_E_ARG);
+        return nullptr;
+    }
+    if (kv4 && (!kv4::shape_ok(kv4) || !kv4->pages || !kv4::aligned16(kv4->pages) || kv4->n_kv_heads != cfg->n_kv_heads ||
+                kv4->head_dim != cfg->head_dim || !page_table || table_stride < 1)) {
         set_error(X100_E_ARG);
         return nullptr;
     }
@@ -656,17 +674,23 @@ x100q_model *x100q_model_create(const x100q_model_cfg *cfg) {
     m->layers.resize(cfg->n_layers);
     const x100q_model_cfg &g = *cfg;
     m->layer_kv = (size_t)g.max_batch * g.n_kv_heads * g.ctx * g.head_dim;
-    const size_t kvb = (size_t)g.n_layers * m->layer_kv * 2;
+    const size_t kvb = kv4 ? 0 : (size_t)g.n_layers * m->layer_kv * 2;
+    size_t workb = 0;
+    if (kv4) {
+        m->paged = true, m->kv4 = *kv4, m->kv4_table = page_table, m->kv4_stride = table_stride;
+        m->kv4_layer = x100q_kv4_bytes(kv4);
+        workb = x100q_kv4_attn_work(kv4, kPrefillChunkMax, g.n_heads, g.max_batch);   // the larger of steps and prompts
+    }
     m->nsplit_max = (g.ctx + kChunk - 1) / kChunk;
     const size_t qkvb = (size_t)g.max_batch * qkv_rows(g) * 4, attb = (size_t)g.max_batch * g.n_heads * kHD * 4,
                  hnb = (size_t)g.max_batch * g.d * 4,
-                 partb = (size_t)g.max_batch * g.n_heads * m->nsplit_max * kPartStride * 4,
+                 partb = kv4 ? 0 : (size_t)g.max_batch * g.n_heads * m->nsplit_max * kPartStride * 4,
                  ropeb = (size_t)g.ctx * (kHD / 2) * sizeof(float2),
                  prepb = qgemv_prep_bytes(16, std::max(g.d, g.n_heads * kHD));
     auto up = [](size_t x) { return (x + 255) & ~size_t(255); };
-    const size_t sb = up(qkvb) + up(attb) + up(hnb) + up(partb) + up(ropeb) + up(prepb);
+    const size_t sb = up(qkvb) + up(attb) + up(hnb) + up(partb) + up(ropeb) + up(prepb) + up(workb);
     const size_t msb = moe_scratch_bytes(g.d, g.n_exp, g.n_act, g.moe_ffn);
-    bool ok = cudaMalloc(&m->kc, kvb) == cudaSuccess && cudaMalloc(&m->vc, kvb) == cudaSuccess &&
+    bool ok = (kv4 || (cudaMalloc(&m->kc, kvb) == cudaSuccess && cudaMalloc(&m->vc, kvb) == cudaSuccess)) &&
               cudaMalloc(&m->scratch, sb) == cudaSuccess && cudaMalloc(&m->moe_scratch, msb) == cudaSuccess;
     if (!ok) {
         cudaGetLastError();
@@ -674,11 +698,13 @@ x100q_model *x100q_model_create(const x100q_model_cfg *cfg) {
         x100q_model_destroy(m);
         return nullptr;
     }
-    cudaMemset(m->kc, 0, kvb);
-    cudaMemset(m->vc, 0, kvb);
+    if (!kv4) {
+        cudaMemset(m->kc, 0, kvb);
+        cudaMemset(m->vc, 0, kvb);
+    }
     const uint64_t rows = (uint64_t)g.n_layers * g.max_batch * g.n_kv_heads * g.ctx;
-    if (!make_tmap_2d(&m->tmK, m->kc, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, kHD, rows, kHD * 2, 64, kChunk) ||
-        !make_tmap_2d(&m->tmV, m->vc, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, kHD, rows, kHD * 2, 64, kChunk)) {
+    if (!kv4 && (!make_tmap_2d(&m->tmK, m->kc, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, kHD, rows, kHD * 2, 64, kChunk) ||
+                 !make_tmap_2d(&m->tmV, m->vc, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, kHD, rows, kHD * 2, 64, kChunk))) {
         set_error(X100_E_UNSUPPORTED);
         x100q_model_destroy(m);
         return nullptr;
@@ -697,6 +723,8 @@ x100q_model *x100q_model_create(const x100q_model_cfg *cfg) {
     m->rope = reinterpret_cast<float2 *>(p);
     p += up(ropeb);
     m->prep = p;
+    p += up(prepb);
+    m->kv4_work = kv4 ? p : nullptr;
     rope_table_kernel<<<256, 256>>>(m->rope, g.ctx, g.rope_base);
     m->S = moe_scratch_carve(m->moe_scratch, g.d, g.n_exp, g.n_act, g.moe_ffn);
     if (check_cuda(cudaDeviceSynchronize(), X100_E_ALLOC)) {
@@ -704,6 +732,17 @@ x100q_model *x100q_model_create(const x100q_model_cfg *cfg) {
         return nullptr;
     }
     return m;
+}
+
+x100q_model *x100q_model_create(const x100q_model_cfg *cfg) { return create_model(cfg, nullptr, nullptr, 0); }
+
+x100q_model *x100q_model_create_kv4(const x100q_model_cfg *cfg, const x100q_kv4 *kv, const int *page_table,
+                                    int table_stride) {
+    if (!kv) {
+        set_error(X100_E_ARG);
+        return nullptr;
+    }
+    return create_model(cfg, kv, page_table, table_stride);
 }
 
 void x100q_model_destroy(x100q_model *m) {
@@ -838,6 +877,10 @@ int x100q_model_kv_copy(x100q_model *m, int layer, int slot, int pos0, int npos,
         set_error(X100_E_ARG);
         return X100_E_ARG;
     }
+    if (m->paged) {   // the pages are the caller's: x100q_kv4_read_dev, x100q_kv4_append_dev
+        set_error(X100_E_UNSUPPORTED);
+        return X100_E_UNSUPPORTED;
+    }
     DeviceGuard dg(m->device);
     const size_t row = (size_t)g->head_dim * 2, span = (size_t)npos * row;
     for (int h = 0; h < g->n_kv_heads; ++h) {
@@ -879,6 +922,90 @@ int x100q_model_embed_dev(x100q_model *m, const int *tokens, float *h, int batch
 
 }  // extern "C"
 
+// Step 2 over the paged cache: n tokens of qkv rows at pos, of the slots in
+// slot (null: token b in slot b), normed, rotated and appended (q in place),
+// then attention into att.  q_start null: token b is the last position of a
+// sequence of its own; else {0, n}: all are one sequence, of slot[0].  Either
+// way the tokens' positions are all in the cache before one attends.
+static int kv4_step(x100q_model *m, DevCtx *c, int layer, float *qkv, float *att, const int *pos, const int *slot,
+                    const int *q_start, int n, cudaStream_t s) {
+    const x100q_model_cfg &g = m->cfg;
+    x100q_kv4 kv = m->kv4;
+    kv.pages = static_cast<uint8_t *>(kv.pages) + (size_t)layer * m->kv4_layer;
+    const float *norms = m->layers[layer].norms;
+    x100q_kv4_append_args w = {};
+    w.dtype = X100Q_F32, w.n_tokens = n, w.n_heads = g.n_heads;
+    w.q = qkv, w.q_out = qkv, w.k = qkv + (size_t)g.n_heads * g.head_dim;
+    w.v = qkv + (size_t)(g.n_heads + g.n_kv_heads) * g.head_dim;
+    w.q_stride = w.k_stride = w.v_stride = w.q_out_stride = qkv_rows(g);
+    w.q_norm = norms + 2 * g.d, w.k_norm = norms + 2 * g.d + g.head_dim, w.eps = g.eps;
+    w.rope = reinterpret_cast<const float *>(m->rope), w.rope_len = g.ctx;
+    w.pos = pos, w.seq = slot, w.page_table = m->kv4_table, w.table_stride = m->kv4_stride, w.n_seqs = g.max_batch;
+    int st = x100q_kv4_append_dev(&kv, &w, s);
+    if (st) return st;
+    kv4::AttnArgs a = {};
+    a.pool = kv4::make_pool(&kv);
+    a.tab = {m->kv4_table, m->kv4_stride, q_start ? 1 : n};
+    a.q = qkv, a.out = att, a.qs = qkv_rows(g), a.os = (long)g.n_heads * g.head_dim;
+    a.q_start = q_start, a.kv_len = q_start ? pos + n - 1 : pos, a.len_add = 1;
+    a.row_of = slot, a.n_rows = g.max_batch;
+    a.n_tokens = n, a.max_q = q_start ? n : 1;
+    kv4::attn_shape(a, g.n_heads, 1.0f / sqrtf((float)g.head_dim));
+    a.part = static_cast<float *>(m->kv4_work);
+    a.status = c->d_status;
+    return kv4::launch_attention(c, a, X100Q_F32, g.head_dim, s);
+}
+
+// Step 2 over the fp16 cache; o3, the options of the Wo call, says whether the merge prepared its activations.
+static int fp16_step(x100q_model *m, DevCtx *c, int layer, const int *pos, const int *slot, int batch, bool kv_early,
+                     GemvOpts &o3, cudaStream_t s) {
+    const x100q_model_cfg &g = m->cfg;
+    ModelLayer &L = m->layers[layer];
+    AttnArgs a;
+    a.qkv = m->qkv;
+    a.qkv_n = qkv_rows(g);
+    a.q_norm = L.norms + 2 * g.d;
+    a.k_norm = L.norms + 2 * g.d + g.head_dim;
+    a.pos = pos;
+    a.nh = g.n_heads;
+    a.nkv = g.n_kv_heads;
+    a.ctx = g.ctx;
+    a.chunk = kChunk;
+    a.cps = attn_cps(batch, g.n_kv_heads, g.ctx, c->device, c->sm_count);
+    a.nsplit = (g.ctx + kChunk * a.cps - 1) / (kChunk * a.cps);
+    a.eps = g.eps;
+    a.rope_base = g.rope_base;
+    a.rope = m->rope;
+    a.scale = 1.0f / sqrtf((float)g.head_dim);
+    a.kc = m->kc + (size_t)layer * m->layer_kv;
+    a.vc = m->vc + (size_t)layer * m->layer_kv;
+    a.row_base = (long)layer * g.max_batch * g.n_kv_heads * g.ctx;
+    a.part = m->part;
+    a.kv_early = (kv_early && !slot) ? 1 : 0;
+    a.slot = slot;
+    a.nslots = g.max_batch;
+    a.prewritten = slot ? 1 : 0;
+    a.att = m->att;
+    a.status = c->d_status;
+    int st;
+    if (slot) {
+        st = launch_pdl(kv_write_kernel, dim3(g.n_kv_heads, batch), dim3(32), 0, s, a);
+        if (st) return st;
+    }
+    st = launch_pdl(attn_decode_kernel, dim3(a.nsplit, g.n_kv_heads, batch), dim3(kAttnThreads), attn_smem(a.cps), s,
+                    m->tmK, m->tmV, a);
+    if (st) return st;
+    if (a.nsplit > 1) {
+        const int grp = qgemv_prep_group(L.o, batch, o3);
+        st = launch_pdl(grp ? attn_merge_kernel<true> : attn_merge_kernel<false>, dim3(g.n_heads, batch), dim3(128),
+                        merge_smem(a.nsplit), s, (const float *)m->part, g.n_heads, a.nsplit, m->att,
+                        grp ? m->prep : nullptr, grp, slices_per_row(g.n_heads * kHD) * 8);
+        if (st) return st;
+        o3.prepared = grp > 0;
+    }
+    return X100_OK;
+}
+
 // One layer, steps 1-4 of the file comment.  kv_early: the step began behind
 // a full barrier (see attn_decode_kernel); barrier: launch the first kernel
 // behind one.  slot: per-token cache slots (null: token b uses slot b); with
@@ -912,50 +1039,15 @@ static int layer_launch(x100q_model *m, DevCtx *c, int layer, float *h, const in
     int st = launch_qgemv_ex(c, L.qkv, h, m->qkv, batch, o1, s);
     if (st) return st;
     // 2. attention (+ merge of the splits)
-    AttnArgs a;
-    a.qkv = m->qkv;
-    a.qkv_n = qkv_rows(g);
-    a.q_norm = L.norms + 2 * g.d;
-    a.k_norm = L.norms + 2 * g.d + g.head_dim;
-    a.pos = pos;
-    a.nh = g.n_heads;
-    a.nkv = g.n_kv_heads;
-    a.ctx = g.ctx;
-    a.chunk = kChunk;
-    a.cps = attn_cps(batch, g.n_kv_heads, g.ctx, c->device, c->sm_count);
-    a.nsplit = (g.ctx + kChunk * a.cps - 1) / (kChunk * a.cps);
-    a.eps = g.eps;
-    a.rope_base = g.rope_base;
-    a.rope = m->rope;
-    a.scale = 1.0f / sqrtf((float)g.head_dim);
-    a.kc = m->kc + (size_t)layer * m->layer_kv;
-    a.vc = m->vc + (size_t)layer * m->layer_kv;
-    a.row_base = (long)layer * g.max_batch * g.n_kv_heads * g.ctx;
-    a.part = m->part;
-    a.kv_early = (kv_early && !slot) ? 1 : 0;
-    a.slot = slot;
-    a.nslots = g.max_batch;
-    a.prewritten = slot ? 1 : 0;
-    a.att = m->att;
-    a.status = c->d_status;
-    timer_mark(m->timer, X100Q_T_ATTN, s);
-    if (slot) {
-        st = launch_pdl(kv_write_kernel, dim3(g.n_kv_heads, batch), dim3(32), 0, s, a);
-        if (st) return st;
-    }
-    st = launch_pdl(attn_decode_kernel, dim3(a.nsplit, g.n_kv_heads, batch), dim3(kAttnThreads), attn_smem(a.cps), s,
-                    m->tmK, m->tmV, a);
-    if (st) return st;
     GemvOpts o3;   // the Wo call: its activations prepared by the merge when it prepares them once
     o3.accum = true;
     o3.prep = m->prep;
-    if (a.nsplit > 1) {
-        const int grp = qgemv_prep_group(L.o, batch, o3);
-        st = launch_pdl(grp ? attn_merge_kernel<true> : attn_merge_kernel<false>, dim3(g.n_heads, batch), dim3(128),
-                        merge_smem(a.nsplit), s, (const float *)m->part, g.n_heads, a.nsplit, m->att,
-                        grp ? m->prep : nullptr, grp, slices_per_row(g.n_heads * kHD) * 8);
+    timer_mark(m->timer, X100Q_T_ATTN, s);
+    if (m->paged) {
+        st = kv4_step(m, c, layer, m->qkv, m->att, pos, slot, nullptr, batch, s);
         if (st) return st;
-        o3.prepared = grp > 0;
+    } else if ((st = fp16_step(m, c, layer, pos, slot, batch, kv_early, o3, s))) {
+        return st;
     }
     // 3. h += Wo . att
     timer_mark(m->timer, X100Q_T_O, s);
@@ -1120,7 +1212,7 @@ static int forward_impl(x100q_model *m, const int *tokens, float *h, const int *
 // ~chunk * top-k / n_exp tokens each) at the cost of scratch memory (about
 // 0.28 MB per token of chunk at the config-5 shape).  X100_PREFILL_CHUNK
 // overrides the default (32 .. 4096), read when a model first prefills.
-constexpr int kPrefillChunk = 1024;
+constexpr int kPrefillChunk = 1024;   // at most kPrefillChunkMax
 
 static bool prefill_alloc(x100q_model *m) {
     if (m->pf_base) return true;
@@ -1128,7 +1220,7 @@ static bool prefill_alloc(x100q_model *m) {
     int T = kPrefillChunk;
     if (const char *e = getenv("X100_PREFILL_CHUNK")) {
         const int v = atoi(e);
-        if (v >= 32 && v <= 4096) T = v;
+        if (v >= 32 && v <= kPrefillChunkMax) T = v;
     }
     const int kpd = slices_per_row(g.d) * 256, kpq = slices_per_row(g.n_heads * g.head_dim) * 256;
     m->pf_kp = kpd > kpq ? kpd : kpq;
@@ -1172,18 +1264,82 @@ static int prefill_linear(x100q_model *m, DevCtx *c, const QMat &W, const float 
     return launch_qgemm(c, L, s);
 }
 
+// position of token i of a chunk whose first token sits at pos0 (the
+// positions of a prefill chunk are consecutive)
+static inline int hpos_last(int pos0, int i) { return pos0 + i; }
+
+// Step 2 of a prefill chunk over the fp16 cache: every token's k, v into the
+// cache, then attention per token.
+static int fp16_prefill_step(x100q_model *m, DevCtx *c, int l, const int *pos, const int *slot, int hpos0, int T,
+                             cudaStream_t s) {
+    const x100q_model_cfg &g = m->cfg;
+    ModelLayer &L = m->layers[l];
+    const int qd = g.n_heads * g.head_dim, qn = qkv_rows(g);
+    AttnArgs a;
+    a.qkv = m->pf_qkv;
+    a.qkv_n = qn;
+    a.q_norm = L.norms + 2 * g.d;
+    a.k_norm = L.norms + 2 * g.d + g.head_dim;
+    a.pos = pos;
+    a.nh = g.n_heads;
+    a.nkv = g.n_kv_heads;
+    a.ctx = g.ctx;
+    a.chunk = kChunk;
+    a.cps = 1;
+    a.nsplit = (g.ctx + kChunk - 1) / kChunk;
+    a.eps = g.eps;
+    a.rope_base = g.rope_base;
+    a.rope = m->rope;
+    a.scale = 1.0f / sqrtf((float)g.head_dim);
+    a.kc = m->kc + (size_t)l * m->layer_kv;
+    a.vc = m->vc + (size_t)l * m->layer_kv;
+    a.row_base = (long)l * g.max_batch * g.n_kv_heads * g.ctx;
+    a.part = m->part;
+    a.kv_early = 0;
+    a.slot = slot;
+    a.nslots = g.max_batch;
+    a.prewritten = 1;
+    a.att = m->pf_att;
+    a.status = c->d_status;
+    int st = launch_pdl(kv_write_kernel, dim3(g.n_kv_heads, T), dim3(32), 0, s, a);
+    // groups of tokens whose (token, split) partials fit the decode step's
+    // buffer (max_batch x nsplit_max of them); the group's splits cover
+    // its largest position only (the chunk's positions are consecutive:
+    // hpos[g0 + gb - 1] is the group's largest), so early chunks need few
+    const int cap = g.max_batch * m->nsplit_max;
+    for (int g0 = 0; st == X100_OK && g0 < T;) {
+        int gb = T - g0;
+        int nsp = (hpos_last(hpos0, g0 + gb - 1) + kChunk) / kChunk;
+        while (gb > 1 && gb * nsp > cap) {
+            gb = cap / nsp < gb ? cap / nsp : gb - 1;
+            if (gb < 1) gb = 1;
+            nsp = (hpos_last(hpos0, g0 + gb - 1) + kChunk) / kChunk;
+        }
+        AttnArgs ag = a;
+        ag.qkv = m->pf_qkv + (size_t)g0 * qn;
+        ag.pos = pos + g0;
+        ag.slot = slot + g0;
+        ag.att = m->pf_att + (size_t)g0 * qd;
+        ag.nsplit = nsp;
+        st = launch_pdl(attn_decode_kernel, dim3(ag.nsplit, g.n_kv_heads, gb), dim3(kAttnThreads), attn_smem(), s,
+                        m->tmK, m->tmV, ag);
+        if (!st && ag.nsplit > 1)
+            st = launch_pdl(attn_merge_kernel<false>, dim3(g.n_heads, gb), dim3(128), merge_smem(ag.nsplit), s,
+                            (const float *)m->part, g.n_heads, ag.nsplit, ag.att, (uint8_t *)nullptr, 0, 0);
+        g0 += gb;
+    }
+    return st;
+}
+
 // forward() over T consecutive tokens of one sequence (the reference's
 // prefill, qwen_moe_hp.c:1748-1858): per layer the q/k/v, Wo and expert
 // linears run as tensor-core GEMMs over all T tokens (each weight row
 // streamed once per 128 tokens), every token's k and v go to the cache
 // before any token attends, and the attention runs per token over its
-// positions 0 .. pos (causal) in groups of max_batch tokens.
-// position of token i of a chunk whose first token sits at pos0 (the
-// positions of a prefill chunk are consecutive)
-static inline int hpos_last(int pos0, int i) { return pos0 + i; }
-
+// positions 0 .. pos (causal) in groups of max_batch tokens; over a paged
+// cache in one call (q_start: {0, T} on the device).
 static int prefill_chunk_tc(x100q_model *m, DevCtx *c, const int *tok, float *h, const int *pos, const int *slot,
-                            int hpos0, float *logits, int T, cudaStream_t s) {
+                            int hpos0, const int *q_start, float *logits, int T, cudaStream_t s) {
     const x100q_model_cfg &g = m->cfg;
     static bool attr[64];
     if (!attr[c->device]) {
@@ -1201,60 +1357,9 @@ static int prefill_chunk_tc(x100q_model *m, DevCtx *c, const int *tok, float *h,
         // 1. qkv = Wqkv . rmsnorm(h, attn_norm)
         st = prefill_linear(m, c, L.qkv, h, g.d, T, L.norms, m->pf_qkv, qn, false, s);
         if (st) break;
-        // 2. every token's k, v into the cache, then attention per token
-        AttnArgs a;
-        a.qkv = m->pf_qkv;
-        a.qkv_n = qn;
-        a.q_norm = L.norms + 2 * g.d;
-        a.k_norm = L.norms + 2 * g.d + g.head_dim;
-        a.pos = pos;
-        a.nh = g.n_heads;
-        a.nkv = g.n_kv_heads;
-        a.ctx = g.ctx;
-        a.chunk = kChunk;
-        a.cps = 1;
-        a.nsplit = (g.ctx + kChunk - 1) / kChunk;
-        a.eps = g.eps;
-        a.rope_base = g.rope_base;
-        a.rope = m->rope;
-        a.scale = 1.0f / sqrtf((float)g.head_dim);
-        a.kc = m->kc + (size_t)l * m->layer_kv;
-        a.vc = m->vc + (size_t)l * m->layer_kv;
-        a.row_base = (long)l * g.max_batch * g.n_kv_heads * g.ctx;
-        a.part = m->part;
-        a.kv_early = 0;
-        a.slot = slot;
-        a.nslots = g.max_batch;
-        a.prewritten = 1;
-        a.att = m->pf_att;
-        a.status = c->d_status;
-        st = launch_pdl(kv_write_kernel, dim3(g.n_kv_heads, T), dim3(32), 0, s, a);
-        // groups of tokens whose (token, split) partials fit the decode step's
-        // buffer (max_batch x nsplit_max of them); the group's splits cover
-        // its largest position only (the chunk's positions are consecutive:
-        // hpos[g0 + gb - 1] is the group's largest), so early chunks need few
-        const int cap = g.max_batch * m->nsplit_max;
-        for (int g0 = 0; st == X100_OK && g0 < T;) {
-            int gb = T - g0;
-            int nsp = (hpos_last(hpos0, g0 + gb - 1) + kChunk) / kChunk;
-            while (gb > 1 && gb * nsp > cap) {
-                gb = cap / nsp < gb ? cap / nsp : gb - 1;
-                if (gb < 1) gb = 1;
-                nsp = (hpos_last(hpos0, g0 + gb - 1) + kChunk) / kChunk;
-            }
-            AttnArgs ag = a;
-            ag.qkv = m->pf_qkv + (size_t)g0 * qn;
-            ag.pos = pos + g0;
-            ag.slot = slot + g0;
-            ag.att = m->pf_att + (size_t)g0 * qd;
-            ag.nsplit = nsp;
-            st = launch_pdl(attn_decode_kernel, dim3(ag.nsplit, g.n_kv_heads, gb), dim3(kAttnThreads), attn_smem(), s,
-                            m->tmK, m->tmV, ag);
-            if (!st && ag.nsplit > 1)
-                st = launch_pdl(attn_merge_kernel<false>, dim3(g.n_heads, gb), dim3(128), merge_smem(ag.nsplit), s,
-                                (const float *)m->part, g.n_heads, ag.nsplit, ag.att, (uint8_t *)nullptr, 0, 0);
-            g0 += gb;
-        }
+        // 2. every token's k, v into the cache, then attention
+        st = m->paged ? kv4_step(m, c, l, m->pf_qkv, m->pf_att, pos, slot, q_start, T, s)
+                      : fp16_prefill_step(m, c, l, pos, slot, hpos0, T, s);
         if (st) break;
         // 3. h += Wo . att
         st = prefill_linear(m, c, L.o, m->pf_att, qd, T, nullptr, h, g.d, true, s);
@@ -1394,10 +1499,12 @@ static int prefill_tc(x100q_model *m, int slot, const int *tokens, int n, int po
     if (!buf) return get_error();
     int *dtok = reinterpret_cast<int *>(buf), *dpos = reinterpret_cast<int *>(buf + tb),
         *dslot = reinterpret_cast<int *>(buf + 2 * tb);
-    float *dh = reinterpret_cast<float *>(buf + ((3 * tb + 255) & ~size_t(255)));
+    int *dstart = reinterpret_cast<int *>(buf + 3 * tb);   // {0, tokens of the chunk}
+    float *dh = reinterpret_cast<float *>(buf + ((3 * tb + 8 + 255) & ~size_t(255)));
     float *dl = nullptr;
     if (logits && !(dl = static_cast<float *>(stage_buf(c, 1, lb)))) return get_error();
     std::vector<int> hp(T), hs(T, slot);
+    int hq[2] = {0, 0};
     int st = X100_OK;
     for (int c0 = 0; st == X100_OK && c0 < n; c0 += T) {
         const int cn = n - c0 < T ? n - c0 : T;
@@ -1405,7 +1512,9 @@ static int prefill_tc(x100q_model *m, int slot, const int *tokens, int n, int po
         st = check_cuda(cudaMemcpyAsync(dtok, tokens + c0, cn * 4, cudaMemcpyDefault, c->stream), X100_E_COPY);
         if (!st) st = check_cuda(cudaMemcpyAsync(dpos, hp.data(), cn * 4, cudaMemcpyHostToDevice, c->stream), X100_E_COPY);
         if (!st) st = check_cuda(cudaMemcpyAsync(dslot, hs.data(), cn * 4, cudaMemcpyHostToDevice, c->stream), X100_E_COPY);
-        if (!st) st = prefill_chunk_tc(m, c, dtok, dh, dpos, dslot, pos0 + c0, dl, cn, c->stream);
+        hq[1] = cn;
+        if (!st && m->paged) st = check_cuda(cudaMemcpyAsync(dstart, hq, sizeof hq, cudaMemcpyHostToDevice, c->stream), X100_E_COPY);
+        if (!st) st = prefill_chunk_tc(m, c, dtok, dh, dpos, dslot, pos0 + c0, dstart, dl, cn, c->stream);
         if (!st && logits)
             st = check_cuda(cudaMemcpyAsync(logits + (size_t)c0 * g.vocab, dl, (size_t)cn * g.vocab * 4, cudaMemcpyDefault,
                                             c->stream), X100_E_COPY);

@@ -653,7 +653,8 @@ int x100q_gguf_model_cfg(const x100q_gguf *g, x100q_model_cfg *cfg) {
     return X100_OK;
 }
 
-x100q_model *x100q_model_load_gguf(const x100q_gguf *g, const x100q_model_cfg *cfg) {
+static x100q_model *load_model(const x100q_gguf *g, const x100q_model_cfg *cfg, const x100q_kv4 *kv, const int *page_table,
+                               int table_stride) {
     set_error(X100_OK);
     if (!g || !cfg) return fail(X100_E_ARG), nullptr;
     x100q_model_cfg file;
@@ -664,7 +665,7 @@ x100q_model *x100q_model_load_gguf(const x100q_gguf *g, const x100q_model_cfg *c
         return fail(X100_E_ARG), nullptr;
     DevCtx *dc = ctx();
     if (!dc) return nullptr;
-    x100q_model *m = x100q_model_create(cfg);
+    x100q_model *m = kv ? x100q_model_create_kv4(cfg, kv, page_table, table_stride) : x100q_model_create(cfg);
     if (!m) return nullptr;
     Loader L{g, dc};
     const uint64_t d = c.d, qd = (uint64_t)c.n_heads * c.head_dim, kvd = (uint64_t)c.n_kv_heads * c.head_dim;
@@ -721,6 +722,16 @@ x100q_model *x100q_model_load_gguf(const x100q_gguf *g, const x100q_model_cfg *c
         return nullptr;
     }
     return m;
+}
+
+x100q_model *x100q_model_load_gguf(const x100q_gguf *g, const x100q_model_cfg *cfg) {
+    return load_model(g, cfg, nullptr, nullptr, 0);
+}
+
+x100q_model *x100q_model_load_gguf_kv4(const x100q_gguf *g, const x100q_model_cfg *cfg, const x100q_kv4 *kv,
+                                       const int *page_table, int table_stride) {
+    if (!kv) return fail(X100_E_ARG), nullptr;
+    return load_model(g, cfg, kv, page_table, table_stride);
 }
 
 int x100q_gguf_dequant_dev(int type, const void *data, long n, float *out, void *stream) {

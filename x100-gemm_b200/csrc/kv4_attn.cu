@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
         // ---- start the ring (lane 0).  128 or 256 positions between a warp's stages are whole pages, so the place in
         // the page stays; a page out of range is read as page 0 here and masked below ----
         const int ps = a.pool.page_shift, tp = ps - 4;       // log2 tiles per page
-        const int *row = a.tab.page + (long)b * a.tab.stride;
+        const int *row = a.tab.page + (long)sq.row * a.tab.stride;
         const int *nxt = row + (ts0 >> tp);                   // table entry of the stage to be issued next
         const int pstep = (tps * kWarps) >> tp;
         const bool two = ps == 4 && tps == 2;                 // a stage's tiles lie on two pages
@@ -662,6 +662,18 @@ static int launch_rows(DevCtx *c, AttnArgs &a, cudaStream_t s) {
     return launch<T, D, 4>(c, a, s);
 }
 
+int launch_attention(DevCtx *c, AttnArgs &p, int dtype, int head_dim, cudaStream_t s) {
+    if ((long)p.max_q * p.G >= kPrefillRows) return launch_prefill(c, p, dtype, head_dim, s);
+    if (dtype == X100Q_F32) return head_dim == 128 ? launch_rows<float, 128>(c, p, s) : launch_rows<float, 64>(c, p, s);
+    return head_dim == 128 ? launch_rows<__half, 128>(c, p, s) : launch_rows<__half, 64>(c, p, s);
+}
+
+void attn_shape(AttnArgs &p, int n_heads, float scale) {
+    p.nh = n_heads, p.G = n_heads / p.pool.nkv;
+    p.g_mul = (uint32_t)(((1ull << 32) + p.G - 1) / p.G);
+    p.sl = scale * 1.4426950408889634f;
+}
+
 }  // namespace kv4
 }  // namespace x100
 
@@ -698,24 +710,18 @@ int x100q_kv4_attn_dev(const x100q_kv4 *kv, const x100q_kv4_attn_args *a, void *
     if (a->n_seqs > 65536) return refuse(X100_E_TOO_LARGE);
     DevCtx *c = ctx();
     if (!c) return get_error();
-    AttnArgs p;
+    AttnArgs p = {};
     p.pool = make_pool(kv);
     p.tab = {a->page_table, a->table_stride, a->n_seqs};
     p.q = a->q, p.out = a->out, p.qs = a->q_stride, p.os = a->out_stride;
     p.q_start = a->q_start, p.kv_len = a->kv_len;
     p.n_tokens = a->n_tokens, p.max_q = a->q_start ? std::min(a->max_q, a->n_tokens) : 1;
-    p.nh = a->n_heads, p.G = a->n_heads / kv->n_kv_heads;
-    p.g_mul = (uint32_t)(((1ull << 32) + p.G - 1) / p.G);
-    p.sl = a->scale * 1.4426950408889634f;
+    attn_shape(p, a->n_heads, a->scale);
     p.part = static_cast<float *>(a->work);
     p.status = c->d_status;
     const long items = (long)a->n_seqs * kv->n_kv_heads * (((long)p.max_q * p.G + 7) / 8);
     if (items > (1l << 24) || (long)p.max_q * p.G > (1l << 20)) return refuse(X100_E_TOO_LARGE);
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if ((long)p.max_q * p.G >= kPrefillRows) return launch_prefill(c, p, a->dtype, kv->head_dim, s);
-    if (a->dtype == X100Q_F32)
-        return kv->head_dim == 128 ? launch_rows<float, 128>(c, p, s) : launch_rows<float, 64>(c, p, s);
-    return kv->head_dim == 128 ? launch_rows<__half, 128>(c, p, s) : launch_rows<__half, 64>(c, p, s);
+    return launch_attention(c, p, a->dtype, kv->head_dim, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

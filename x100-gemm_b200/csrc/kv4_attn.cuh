@@ -21,6 +21,10 @@ struct AttnArgs {
     void *out;
     long qs, os;
     const int *q_start, *kv_len;
+    // the model's calls: sequence b reads row row_of[b] < n_rows of the page table (null: row b) and has
+    // kv_len[b] + len_add positions
+    const int *row_of = nullptr;
+    int n_rows = 0, len_add = 0;
     int n_tokens, max_q, nh, G;
     uint32_t g_mul;                      // ceil(2^32 / G): n / G = umulhi(n, g_mul) for n < 2^32 / G
     int unit_shift;                      // positions per unit, a power of two (128 unless the list would pass 2^31 units)
@@ -43,14 +47,16 @@ __device__ __forceinline__ int div_g(const AttnArgs &a, int n) { return a.G == 1
 // Sequence b: first row of q, tokens, positions; `cu` units of positions in every (kv head, row
 // tile) item, at least one so that rows without positions are written.
 struct Seq {
-    int q0, nq, len, nrt, cu;
+    int q0, nq, len, nrt, cu, row;       // row: of the page table
     uint32_t units;                      // of all its items, each cu + lead
 };
 __device__ __forceinline__ Seq load_seq(const AttnArgs &a, int b, int R, bool report) {
     Seq s;
     s.q0 = a.q_start ? a.q_start[b] : b;
     s.nq = a.q_start ? a.q_start[b + 1] - s.q0 : 1;
-    s.len = a.kv_len[b];
+    s.len = (int)((unsigned)a.kv_len[b] + a.len_add);
+    s.row = a.row_of ? a.row_of[b] : b;
+    if (a.row_of && (unsigned)s.row >= (unsigned)a.n_rows) s.row = 0, s.len = -1;
     const int cover = a.tab.stride > (0x7fffffff >> a.pool.page_shift) ? 0x7fffffff : a.tab.stride << a.pool.page_shift;
     const bool bad_q = s.q0 < 0 || s.nq < 0 || s.nq > a.max_q || s.q0 > a.n_tokens - s.nq;
     if (bad_q) s.nq = 0;
@@ -111,6 +117,10 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t 
 constexpr long kPrefillRows = 256;
 size_t prefill_work(int head_dim);
 int launch_prefill(DevCtx *c, AttnArgs &a, int dtype, int head_dim, cudaStream_t s);
+
+// n_heads, G and the scale; then the call, its arguments checked (kv4_attn.cu).
+void attn_shape(AttnArgs &p, int n_heads, float scale);
+int launch_attention(DevCtx *c, AttnArgs &p, int dtype, int head_dim, cudaStream_t s);
 
 }  // namespace kv4
 }  // namespace x100

@@ -104,6 +104,13 @@ __device__ __forceinline__ uint32_t head_units(const AttnArgs &a, const Seq &s) 
     for (int rt = threadIdx.x & 31; rt < s.nrt; rt += 32) n += units_of<RT>(a, s, rt);
     return __reduce_add_sync(0xffffffffu, n);
 }
+// What units_of needs of sequence `j` of the 32 that the lanes have loaded.
+__device__ __forceinline__ Seq seq_of_lane(const Seq &mine, int j) {
+    Seq s;
+    s.nq = __shfl_sync(0xffffffffu, mine.nq, j), s.len = __shfl_sync(0xffffffffu, mine.len, j);
+    s.nrt = __shfl_sync(0xffffffffu, mine.nrt, j);
+    return s;
+}
 // Where a run starts: unit u0 is unit `c` of (sequence b, kv head, row tile rt),
 // whose first unit is `item`.
 struct Start {
@@ -115,22 +122,30 @@ __device__ __forceinline__ Start my_start(const AttnArgs &a) {
     const int lane = threadIdx.x & 31;
     Start r = {0, 0, 0, 0, 0, 0};
     uint32_t U = 0;
-    for (int b = 0; b < a.tab.n_seqs; ++b) {
-        const Seq s = load_seq(a, b, RT, blockIdx.x == 0 && lane == 0);
-        if (s.nrt) U += a.pool.nkv * head_units<RT>(a, s);
+    for (int b0 = 0; b0 < a.tab.n_seqs; b0 += 32) {
+        Seq mine;
+        mine.nrt = 0;
+        if (b0 + lane < a.tab.n_seqs) mine = load_seq(a, b0 + lane, RT, blockIdx.x == 0);
+        for (uint32_t has = __ballot_sync(0xffffffffu, mine.nrt > 0); has; has &= has - 1)
+            U += a.pool.nkv * head_units<RT>(a, seq_of_lane(mine, __ffs(has) - 1));
     }
     const uint32_t per = (U + gridDim.x - 1) / gridDim.x;
     if (per * blockIdx.x >= U) return r;
     r.u0 = per * blockIdx.x, r.u1 = min(U, r.u0 + per);
-    uint32_t base = 0;
-    for (;; ++r.b) {                       // ends: u0 < U
-        const Seq s = load_seq(a, r.b, RT, false);
-        if (!s.nrt) continue;
-        const uint32_t hu = head_units<RT>(a, s);
-        if (r.u0 - base >= hu * a.pool.nkv) {
+    uint32_t base = 0, hu = 0;
+    for (int b0 = 0;; b0 += 32) {          // ends: u0 < U
+        Seq mine;
+        mine.nrt = 0;
+        if (b0 + lane < a.tab.n_seqs) mine = load_seq(a, b0 + lane, RT, false);
+        uint32_t has = __ballot_sync(0xffffffffu, mine.nrt > 0);
+        for (; has; has &= has - 1) {
+            hu = head_units<RT>(a, seq_of_lane(mine, __ffs(has) - 1));
+            if (r.u0 - base < hu * a.pool.nkv) break;
             base += hu * a.pool.nkv;
-            continue;
         }
+        if (!has) continue;
+        r.b = b0 + __ffs(has) - 1;
+        const Seq s = seq_of_lane(mine, __ffs(has) - 1);
         r.kvh = (int)((r.u0 - base) / hu);
         base += r.kvh * hu;
         for (int r0 = 0;; r0 += 32) {
@@ -155,7 +170,7 @@ __device__ __forceinline__ Start my_start(const AttnArgs &a) {
 // A segment: key tiles c0 .. c1 - 1 of an item (all cu of them, or a part).
 struct Seg {
     int n;                                 // c1 - c0; 0: the run is over
-    int c0, cu, b, kvh, rt, q0, nq, len;
+    int c0, cu, b, kvh, rt, q0, nq, len, row;
     uint32_t item;                         // the item's first unit
 };
 constexpr int kSegs = 4;                   // ring of segments
@@ -293,7 +308,7 @@ __global__ void __launch_bounds__(Roles<T>::THREADS, 1) prefill_kernel(const Att
             const Seg &w = bars.seg[nseg % kSegs];
             const int n = w.n;
             if (n == 0) break;
-            const int *trow = a.tab.page + (long)w.b * a.tab.stride;
+            const int *trow = a.tab.page + (long)w.row * a.tab.stride;
             const int c0 = w.c0, len = w.len;
             int lim;                             // positions the row sees
             {
@@ -631,7 +646,7 @@ __global__ void __launch_bounds__(Roles<T>::THREADS, 1) prefill_kernel(const Att
                 if (!ok) break;
                 const Seg &w = bars.seg[nseg % kSegs];
                 const int n = w.n, c0 = w.c0, len = w.len;
-                const int *trow = a.tab.page + (long)w.b * a.tab.stride;
+                const int *trow = a.tab.page + (long)w.row * a.tab.stride;
                 const uint8_t *base = a.pool.pages + (long)w.kvh * a.pool.page_bytes;
                 release(nseg);
                 if (n == 0) break;
@@ -674,7 +689,7 @@ __global__ void __launch_bounds__(Roles<T>::THREADS, 1) prefill_kernel(const Att
                     const int cu = units_of<RT>(a, sq, rt) - kLead, k0 = (int)(u - item), k1 = (int)min((uint32_t)(cu + kLead), k0 + (at.u1 - u));
                     g.c0 = max(0, k0 - kLead);
                     g.n = max(0, k1 - kLead) - g.c0;
-                    g.cu = cu, g.b = b, g.kvh = kvh, g.rt = rt, g.q0 = sq.q0, g.nq = sq.nq, g.len = sq.len, g.item = item;
+                    g.cu = cu, g.b = b, g.kvh = kvh, g.rt = rt, g.q0 = sq.q0, g.nq = sq.nq, g.len = sq.len, g.row = sq.row, g.item = item;
                     item += cu + kLead;
                     u = item;
                     if (u < at.u1 && ++rt == sq.nrt) {

@@ -81,6 +81,7 @@ _SIGS = {
     "x100q_router_topk_noalloc": ([vp, vp, i32, i32, i32, i32, vp, vp, vp], i32),
     # decode step
     "x100q_model_create": ([vp], vp),
+    "x100q_model_create_kv4": ([vp, vp, vp, i32], vp),
     "x100q_model_destroy": ([vp], None),
     "x100q_model_set_layer": ([vp, i32] + [vp] * 12, i32),
     "x100q_model_set_output": ([vp, vp, vp, vp], i32),
@@ -115,6 +116,7 @@ _SIGS = {
     "x100q_gguf_get_str": ([vp, C.c_char_p, vp], i32),
     "x100q_gguf_model_cfg": ([vp, vp], i32),
     "x100q_model_load_gguf": ([vp, vp], vp),
+    "x100q_model_load_gguf_kv4": ([vp, vp, vp, vp, i32], vp),
     "x100q_gguf_dequant_dev": ([i32, vp, C.c_long, vp, vp], i32),
     "x100q_quantize_q8_0_dev": ([vp, C.c_long, vp, vp], i32),
     "x100q_pack_act_dev": ([i32, vp, i32, i32, vp, vp], i32),
@@ -334,14 +336,40 @@ class Moe:
 
 
 class Model:
-    """x100q_model handle: a Qwen3-MoE-shaped decode model (weights, fp16 KV
-    cache, scratch) resident on the current device."""
+    """x100q_model handle: a Qwen3-MoE-shaped decode model (weights, KV cache,
+    scratch) resident on the current device.  The cache is fp16, or, with
+    kv4 = (n_pages, page_size, table), pages of 4-bit codes: table int32
+    [max_batch, entries] on the GPU names each slot's pages, for all layers."""
 
-    def __init__(self, **cfg):
+    def __init__(self, kv4=None, **cfg):
         self.cfg = ModelCfg(**cfg)
-        self.h = lib().x100q_model_create(C.byref(self.cfg))
+        self._open("x100q_model_create", (), kv4)
+
+    def _open(self, fn, args, kv4):
+        """Call fn(*args, cfg), or with a paged cache fn_kv4(*args, cfg, pool, table, entries)."""
+        self.h, args = None, (*args, C.byref(self.cfg))
+        if kv4 is not None:
+            torch, c, fn = _torch()[0], self.cfg, fn + "_kv4"
+            n_pages, page_size, table = kv4
+            if not (table.dtype is torch.int32 and table.is_cuda and table.get_device() == torch.cuda.current_device()
+                    and table.is_contiguous() and table.dim() == 2 and table.shape[0] >= c.max_batch):
+                _refuse(fn, f"the page table has to be contiguous int32 [{c.max_batch}, entries] on the current device")
+            kv = Kv4(None, n_pages, page_size, c.n_kv_heads, c.head_dim)
+            n = lib().x100q_kv4_bytes(C.byref(kv))
+            if n == 0 or c.n_layers < 1:
+                _refuse(fn, f"no pool of {n_pages} pages of {page_size} x {c.n_kv_heads} x {c.head_dim}")
+            self._pages = torch.zeros(c.n_layers, n, dtype=torch.uint8, device="cuda")
+            torch.cuda.current_stream().synchronize()   # zeroed before a step on another stream
+            kv.pages, self.kv4_table, self._kv4 = self._pages.data_ptr(), table, kv
+            args += (C.byref(kv), table.data_ptr(), table.shape[1])
+        self.h = getattr(lib(), fn)(*args)
         if not self.h:
-            check_last("x100q_model_create")
+            check_last(fn)
+
+    def kv4_cache(self, layer: int) -> "Kv4Cache":
+        """The pool of a layer of a model made with kv4, on the model's own pages."""
+        kv = self._kv4
+        return Kv4Cache(kv.n_pages, kv.page_size, kv.n_kv_heads, kv.head_dim, pages=self._pages[layer])
 
     def set_layer(self, layer, attn_norm, wq, wk, wv, q_norm, k_norm, wo, ffn_norm, router, gate, up, down):
         check(lib().x100q_model_set_layer(self.h, layer, *(_p(a) for a in (attn_norm, wq, wk, wv, q_norm, k_norm,
@@ -475,15 +503,14 @@ class Gguf:
         check(lib().x100q_gguf_model_cfg(self.h, C.byref(c)), "x100q_gguf_model_cfg")
         return {n: getattr(c, n) for n, _ in ModelCfg._fields_}
 
-    def load_model(self, **overrides) -> "Model":
+    def load_model(self, kv4=None, **overrides) -> "Model":
         """x100q_model_load_gguf with the file's configuration, fields such as
-        ctx, max_batch or expert_lo / expert_hi replaced by `overrides`."""
+        ctx, max_batch or expert_lo / expert_hi replaced by `overrides`; kv4
+        as of Model."""
         cfg = dict(self.model_cfg(), **overrides)
         m = Model.__new__(Model)
         m.cfg = ModelCfg(**cfg)
-        m.h = lib().x100q_model_load_gguf(self.h, C.byref(m.cfg))
-        if not m.h:
-            check_last("x100q_model_load_gguf")
+        m._open("x100q_model_load_gguf", (self.h,), kv4)
         return m
 
     def close(self):
