@@ -127,3 +127,21 @@ def norm_q8(x, res, w, eps, group):
     q = np.clip(np.rint((t * inv[..., None]).astype(F32)), -127, 127).astype(np.int8).reshape(x.shape)
     rms = np.sqrt((h.astype(np.float64) ** 2).mean(1) + eps)
     return h, q, np.where(tiny, 0.0, top.astype(np.float64) / 127 / rms[:, None])
+
+
+def prompt_bound(q, k, v, scale, n, half):
+    """The same for calls of 256 rows and more, whose products are tcgen05's (128 positions a tile, 8 steps of 16).
+
+    Scores as in attention_bound. fp16 q: p is rounded to fp16 in the numerator alone, half a step of p, 2^-11, or 2^-25 where it
+    is subnormal (the sum below it is at least 1, of the position that set the maximum); its sums take n / 16 steps of 2^-23.
+    fp32 q: p in halves as there; hi and lo go 2 steps for 16 positions, every other tile to a sum of its own, and a sum
+    ends after 32 tiles, so n / 16 and at most 512 steps, then at most n / 8192 + 1 joins of 2^-22."""
+    D = q.shape[-1]
+    A = scale * max(float(np.abs(q).reshape(-1, D).max(0) @ np.abs(k).reshape(-1, D).max(0)), 1e-30) if k.size else 0.0
+    top = float(np.abs(v).max()) if v.size else 0.0
+    rel = 2 * (A * (2.0 ** -22 + (D / 8 + D / 32 + 1) * 2.0 ** -23) + 2.0 ** -21) + 330 * 2.0 ** -24
+    if half:
+        rel += 2 * 2.0 ** -11 + n * 2.0 ** -25 + (n / 16 + 8) * 2.0 ** -23
+    else:
+        rel += min(n / 16 + 16, 528) * 2.0 ** -23 + (n / 8192 + 1) * 2.0 ** -22
+    return top * rel + 1e-12

@@ -120,3 +120,18 @@ def test_model_refuses_no_pool_or_table():
     for args in ((None, P, 2), (C.byref(kv()), None, 2), (C.byref(kv()), P, 0)):
         assert L.x100q_model_create_kv4(C.byref(cfg), *args) is None and x100b.last_error() == x100b.X100_E_ARG
     assert L.x100q_model_load_gguf_kv4(None, C.byref(cfg), C.byref(kv()), P, 2) is None and x100b.last_error() == x100b.X100_E_ARG
+
+
+def test_scratch_follows_the_rows_a_sequence_can_have():
+    """256 rows (tokens times query heads per kv head) need the prompt kernel's scratch, fewer the other's; neither depends on lengths."""
+    L, p = x100b.lib(), C.byref(kv())
+    few, many = L.x100q_kv4_attn_work(p, 1, 2, 1), L.x100q_kv4_attn_work(p, 4096, 32, 1)
+    assert 0 < few < many
+    assert L.x100q_kv4_attn_work(p, 255, 2, 3) == few and L.x100q_kv4_attn_work(p, 256, 2, 3) == many
+    assert L.x100q_kv4_attn_work(p, 31, 16, 1) == few and L.x100q_kv4_attn_work(p, 32, 16, 1) == many
+
+
+@pytest.mark.parametrize("big", [dict(n_seqs=4096, max_q=1 << 19), dict(n_seqs=64, max_q=1 << 19, table_stride=1 << 20), dict(n_seqs=1, max_q=1 << 20), dict(n_seqs=65537)])
+def test_calls_past_the_work_list_are_refused(big):
+    a = x100b.Kv4AttnArgs(**dict(ATTN, n_tokens=1 << 20, work_bytes=1 << 40, **big))
+    assert x100b.lib().x100q_kv4_attn_dev(C.byref(kv()), C.byref(a), None) == x100b.X100_E_TOO_LARGE

@@ -708,8 +708,6 @@ int x100q_kv4_attn_dev(const x100q_kv4 *kv, const x100q_kv4_attn_args *a, void *
         return refuse(X100_E_ARG);
     if (a->work_bytes < x100q_kv4_attn_work(kv, a->n_tokens, a->n_heads, a->n_seqs)) return refuse(X100_E_TOO_LARGE);
     if (a->n_seqs > 65536) return refuse(X100_E_TOO_LARGE);
-    DevCtx *c = ctx();
-    if (!c) return get_error();
     AttnArgs p = {};
     p.pool = make_pool(kv);
     p.tab = {a->page_table, a->table_stride, a->n_seqs};
@@ -717,10 +715,12 @@ int x100q_kv4_attn_dev(const x100q_kv4 *kv, const x100q_kv4_attn_args *a, void *
     p.q_start = a->q_start, p.kv_len = a->kv_len;
     p.n_tokens = a->n_tokens, p.max_q = a->q_start ? std::min(a->max_q, a->n_tokens) : 1;
     attn_shape(p, a->n_heads, a->scale);
+    const long rows = (long)p.max_q * p.G, items = (long)a->n_seqs * kv->n_kv_heads * ((rows + 7) / 8);
+    if (items > (1l << 24) || rows > (1l << 20) || (rows >= kPrefillRows && !prefill_fits(p, a->dtype))) return refuse(X100_E_TOO_LARGE);
+    DevCtx *c = ctx();
+    if (!c) return get_error();
     p.part = static_cast<float *>(a->work);
     p.status = c->d_status;
-    const long items = (long)a->n_seqs * kv->n_kv_heads * (((long)p.max_q * p.G + 7) / 8);
-    if (items > (1l << 24) || (long)p.max_q * p.G > (1l << 20)) return refuse(X100_E_TOO_LARGE);
     return launch_attention(c, p, a->dtype, kv->head_dim, static_cast<cudaStream_t>(stream));
 }
 

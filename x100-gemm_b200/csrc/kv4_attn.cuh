@@ -116,6 +116,7 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t 
 // sequence may have this many query rows.
 constexpr long kPrefillRows = 256;
 size_t prefill_work(int head_dim);
+bool prefill_fits(const AttnArgs &a, int dtype);   // its units can be counted in 32 bits, whatever q_start and kv_len hold
 int launch_prefill(DevCtx *c, AttnArgs &a, int dtype, int head_dim, cudaStream_t s);
 
 // n_heads, G and the scale; then the call, its arguments checked (kv4_attn.cu).

@@ -167,10 +167,15 @@ __device__ __forceinline__ Start my_start(const AttnArgs &a) {
         }
     }
 }
-// A segment: key tiles c0 .. c1 - 1 of an item (all cu of them, or a part).
+// A segment: key tiles c0 .. c0 + n - 1 of an item (all cu of them, or a part).  A run's part of an item is one segment, but for
+// fp32 q at most kPiece key tiles long: a tensor-core sum loses up to an ulp of what it holds with each product (it truncates; 1.9e-8
+// relative a step measured), which over 131072 positions would be 1.5e-4.  Pieces are added up in fp32 in the slot of their part.
+constexpr int kPiece = 64;
 struct Seg {
-    int n;                                 // c1 - c0; 0: the run is over
+    int n;                                 // 0: the run is over
     int c0, cu, b, kvh, rt, q0, nq, len, row;
+    int first, slot;                       // the first key tile of the part, and its slot (of the CTA's two)
+    bool more;                             // the part has another piece
     uint32_t item;                         // the item's first unit
 };
 constexpr int kSegs = 4;                   // ring of segments
@@ -302,6 +307,7 @@ __global__ void __launch_bounds__(Roles<T>::THREADS, 1) prefill_kernel(const Att
             if (lane == 0) mbar_arrive(&bars.q_full);
         };
         uint32_t nseg = 0;
+        float m_sum = -INFINITY, l_sum = 0.f;    // of the part's earlier pieces (HL)
         ok = segment(0);
         if (ok && bars.seg[0].n) put_q(bars.seg[0]);
         for (; ok; ++nseg) {
@@ -428,12 +434,25 @@ __global__ void __launch_bounds__(Roles<T>::THREADS, 1) prefill_kernel(const Att
                 l = l * f + other.y * fo;
                 m = M;
             }
+            // with what the part's earlier pieces left in the slot, times fs
+            const bool join = HL && c0 != w.first, more = HL && w.more;
+            float fs = 0.f;
+            if constexpr (HL) {
+                if (join) {
+                    const float M = fmaxf(m, m_sum), g = M == -INFINITY ? 0.f : ex2(m - M);
+                    fs = M == -INFINITY ? 0.f : ex2(m_sum - M);
+                    l = l * g + l_sum * fs;
+                    f *= g, fo *= g;
+                    m = M;
+                }
+                m_sum = m, l_sum = l;
+            }
             if (!ok) break;
             tc_fence_after();
             const int r = w.rt * RT + (HL ? 0 : 128 * X) + row;
-            const bool live = r < w.nq * a.G, whole = n == w.cu, two = HL && n > 1;   // one key tile: step 1 has no sums
+            const bool live = r < w.nq * a.G, whole = w.first == 0 && c0 + n == w.cu, two = HL && n > 1;   // one key tile: step 1 has no sums
             const int tok = live ? div_g(a, r) : 0;
-            const int slot = (int)blockIdx.x * 2 + (nseg ? 1 : 0), prow = HL ? row : 128 * X + row;
+            const int slot = (int)blockIdx.x * 2 + w.slot, prow = HL ? row : 128 * X + row;
             const float inv = whole ? (l > 0.f ? 1.f / l : 0.f) : 1.f;
             const float f0 = HL ? (X ? fo : f) : 1.f, f1 = HL ? (X ? f : fo) : 0.f;
             T *op = static_cast<T *>(a.out) + (long)(w.q0 + tok) * a.os + (long)(w.kvh * a.G + r - tok * a.G) * D;
@@ -456,8 +475,18 @@ __global__ void __launch_bounds__(Roles<T>::THREADS, 1) prefill_kernel(const Att
                         if (two) o[k] = fmaf(o1[k], f1, o[k]);
                     }
                 }
-                if (!whole) {
-                    float4 *pp = reinterpret_cast<float4 *>(a.part) + ((long)slot * (D / 4) + col / 4) * kPfRows + prow;
+                float4 *pp = reinterpret_cast<float4 *>(a.part) + ((long)slot * (D / 4) + col / 4) * kPfRows + prow;
+                if constexpr (HL) {
+                    if (join) {
+#pragma unroll
+                        for (int k = 0; k < CW / 4; ++k) {
+                            const float4 y = pp[k * kPfRows];
+                            o[4 * k] = fmaf(y.x, fs, o[4 * k]), o[4 * k + 1] = fmaf(y.y, fs, o[4 * k + 1]);
+                            o[4 * k + 2] = fmaf(y.z, fs, o[4 * k + 2]), o[4 * k + 3] = fmaf(y.w, fs, o[4 * k + 3]);
+                        }
+                    }
+                }
+                if (!whole || more) {
 #pragma unroll
                     for (int k = 0; k < CW / 4; ++k) pp[k * kPfRows] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
                 } else if (live) {
@@ -477,9 +506,9 @@ __global__ void __launch_bounds__(Roles<T>::THREADS, 1) prefill_kernel(const Att
                     }
                 }
             }
-            if (!whole && (!HL || X == 0)) {
+            if (!whole && !more && (!HL || X == 0)) {
                 a.ml[(long)slot * kPfRows + prow] = make_float2(m, l);
-                if (X == 0 && row == 0) a.meta[slot] = make_int4((int)w.item, w.b, w.kvh, w.rt | (c0 ? kInside : 0));
+                if (X == 0 && row == 0) a.meta[slot] = make_int4((int)w.item, w.b, w.kvh, w.rt | (w.first ? kInside : 0));
             }
             tc_fence_before();                      // the next step's products overwrite the sums
             if constexpr (HL) ok = meet();          // both groups have read them
@@ -677,7 +706,7 @@ __global__ void __launch_bounds__(Roles<T>::THREADS, 1) prefill_kernel(const Att
         } else if (warp == W::kMma + 2) {
             // ================================ work list ================================
             const Start at = my_start<RT>(a);
-            uint32_t u = at.u0, item = at.item, nseg = 0;
+            uint32_t u = at.u0, item = at.item, nseg = 0, parts = 0;
             int b = at.b, kvh = at.kvh, rt = at.rt;
             Seq sq;
             if (u < at.u1) sq = load_seq(a, b, RT, false);
@@ -687,8 +716,9 @@ __global__ void __launch_bounds__(Roles<T>::THREADS, 1) prefill_kernel(const Att
                 if (more) {
                     // a run that ends within an item's kLead units has none of its key tiles, and one that starts there has all
                     const int cu = units_of<RT>(a, sq, rt) - kLead, k0 = (int)(u - item), k1 = (int)min((uint32_t)(cu + kLead), k0 + (at.u1 - u));
-                    g.c0 = max(0, k0 - kLead);
+                    g.c0 = g.first = max(0, k0 - kLead);
                     g.n = max(0, k1 - kLead) - g.c0;
+                    g.slot = parts ? 1 : 0;
                     g.cu = cu, g.b = b, g.kvh = kvh, g.rt = rt, g.q0 = sq.q0, g.nq = sq.nq, g.len = sq.len, g.row = sq.row, g.item = item;
                     item += cu + kLead;
                     u = item;
@@ -701,14 +731,21 @@ __global__ void __launch_bounds__(Roles<T>::THREADS, 1) prefill_kernel(const Att
                         }
                     }
                     if (g.n == 0) continue;
+                    ++parts;
                 }
-                ok = wait(&bars.seg_empty[nseg % kSegs], (nseg / kSegs & 1) ^ 1);
-                if (!ok) break;
-                if (lane == 0) {
-                    bars.seg[nseg % kSegs] = g;
-                    mbar_arrive(&bars.seg_full[nseg % kSegs]);
+                for (int left = g.n;; g.c0 += g.n) {
+                    if (HL) g.n = min(left, kPiece);
+                    left -= g.n;
+                    g.more = left > 0;
+                    ok = wait(&bars.seg_empty[nseg % kSegs], (nseg / kSegs & 1) ^ 1);
+                    if (!ok) break;
+                    if (lane == 0) {
+                        bars.seg[nseg % kSegs] = g;
+                        mbar_arrive(&bars.seg_full[nseg % kSegs]);
+                    }
+                    ++nseg;
+                    if (!g.more) break;
                 }
-                ++nseg;
             }
         }
     }
@@ -774,6 +811,12 @@ __global__ void __launch_bounds__(kPfRows) prefill_merge_kernel(const AttnArgs a
 
 size_t prefill_work(int head_dim) {
     return (size_t)kPfCtas * 2 * (kPfRows * (head_dim + 2) * sizeof(float) + sizeof(int4));
+}
+
+bool prefill_fits(const AttnArgs &a, int dtype) {
+    const long RT = dtype == X100Q_F32 ? 128 : 256, cover = std::min(0x7fffffffl, (long)a.tab.stride << a.pool.page_shift);
+    const long items = (long)a.tab.n_seqs * a.pool.nkv * (((long)a.max_q * a.G + RT - 1) / RT);
+    return items <= 0xfffff000l / (cover / kKeys + 1 + kLead);
 }
 
 template <typename T, int D>
