@@ -205,7 +205,8 @@ int x100q_rope_table_dev(float *rope, int n_pos, int head_dim, float base, void 
  * to 22 bits; X100Q_F16: from 256 rows (tokens times n_heads / n_kv_heads) a sequence
  * on, probabilities are rounded to fp16, and out is rounded once.  All sums are
  * fp32, the tensor cores' own (truncating) for 16 positions at a time: over 131072
- * positions they lose at most 3e-5 of a value in fp32.
+ * positions they are off by less than 1e-4 (6e-5 measured, where one block has them
+ * all; 2e-5 where the call spreads a sequence over blocks).
  * The result does not depend on the order in which blocks run.
  * work: 16-byte aligned device scratch of x100q_kv4_attn_work() bytes; its
  * contents need not be kept or cleared, but calls that overlap on the GPU
