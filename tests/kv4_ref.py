@@ -105,13 +105,15 @@ def attention_bound(q, k, v, scale, n, half):
     size at each of its 2 D / 16 steps and D / 32 fp32 updates follow: with A = scale * max sum |q k| at most
     A * (2^-22 + (D / 8 + D / 32) * 2^-23). exp2 of it (and its argument's rounding, A * 2^-23 again) moves p by that
     relatively, 2^-21 more for exp2 itself and p's split into halves. Numerator and sum both carry it (factor 2).
-    The sum over positions takes 2 steps for 16 positions of a warp, at most n / 128 * 2 + 2 of them, and 2^-23 each; joining
-    8 warps and up to 320 runs adds 2^-24 each. All relative to sum p |v| <= max |v|. fp16 output adds half a step."""
+    The sum over positions takes a step for 16 positions of a warp (two for fp32 q), at most n / 128 * 2 + 2 of them, and 2^-23
+    each; joining 8 warps and up to 320 runs adds 2^-24 each. All relative to sum p |v| <= max |v|. fp16 q: p of the numerator is
+    rounded to fp16, 2^-11, or 2^-25 where it is subnormal (the sum below is at least 1, of the position that set the maximum), and
+    the output adds half a step."""
     D = q.shape[-1]
     A = scale * max(float(np.abs(q).reshape(-1, D).max(0) @ np.abs(k).reshape(-1, D).max(0)), 1e-30) if k.size else 0.0
     top = float(np.abs(v).max()) if v.size else 0.0
     rel = 2 * (A * (2.0 ** -22 + (D / 8 + D / 32 + 1) * 2.0 ** -23) + 2.0 ** -21) + (n / 64 + 2) * 2.0 ** -23 + 330 * 2.0 ** -24
-    return top * (rel + (2.0 ** -11 if half else 0.0)) + 1e-12
+    return top * (rel + (2 * 2.0 ** -11 + n * 2.0 ** -25 if half else 0.0)) + 1e-12
 
 
 def norm_q8(x, res, w, eps, group):

@@ -102,13 +102,15 @@ struct Cfg {
 
 // S^T = K Q^T and O^T = V^T P^T: positions (then dims) are the M side of
 // m16n8k16, the 8 query rows the N side, so that a group of 8 heads wastes no
-// tensor rows.  K codes go into the product as 64 + code (fp16 q: every second
-// pair as 1024 + code), one instruction each, and the sum starts from
-// -sum (72 or 1032) q, which each row and block has once: what is left is
-// sum (code - 8) q, which the block's scale multiplies in fp32.  V codes become scale * (code - 8), an exact fp16.
+// tensor rows.  For fp16 q K codes go into the product as 64 + code or 1024 + code, one instruction each, and the
+// sum starts from -sum (72 or 1032) q, which each row and block has once: what is left is
+// sum (code - 8) q, which the block's scale multiplies in fp32.  What cancels there costs fp32 q too many bits
+// (outputs off by 5e-6 instead of 3e-7): its codes are made code - 8 first.  V codes become scale * (code - 8), an exact fp16.
 // Position k of a tile's MMA rows r: r / 2 + 4 (r % 2) of each half, so that
 // transposing the score fragment gives P^T's B fragment for the positions t,
-// t + 4, t + 8, t + 12 that a lane's V codes hold.  HL: q as hi + lo halves.
+// t + 4, t + 8, t + 12 that a lane's V codes hold.  HL (fp32 q): q and p as hi + lo halves, and each tile's
+// P V in sums of its own that fp32 additions take up: the tensor core truncates what it adds to, 1.2e-8 of it a step.
+// fp16 q: p rounded to fp16, whose error is no larger than the output's own rounding (16 x 16384 positions 36.5 -> 33.9 us).
 // Every warp walks its own positions with its own ring of bulk copies (two tiles a
 // stage), so the loop has no CTA barrier.
 template <typename T, int D, int NR>
@@ -229,23 +231,25 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
                 }
             }
             // half2 number j of a block's K words holds codes j and j + 4
-            float bias = 0.f;
+            [[maybe_unused]] float bias = 0.f;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 uint4 f;
                 split2(x[2 * j], x[2 * j + 4], f.x, f.z);
                 split2(x[2 * j + 1], x[2 * j + 5], f.y, f.w);
                 qf[(nr * (D / 16) + 2 * blk + j) * 32 + ln] = f;
-                bias = fmaf(HL ? -72.f : -1032.f, x[2 * j] + x[2 * j + 4], fmaf(-72.f, x[2 * j + 1] + x[2 * j + 5], bias));
+                bias = fmaf(-1032.f, x[2 * j] + x[2 * j + 4], fmaf(-72.f, x[2 * j + 1] + x[2 * j + 5], bias));
             }
-            bias += __shfl_xor_sync(0xffffffffu, bias, 1);    // e runs over whole warps
-            bias += __shfl_xor_sync(0xffffffffu, bias, 2);
-            if ((ln & 3) == 0) qb[(nr * NB + blk) * 8 + ln / 4] = bias;
+            if constexpr (!HL) {
+                bias += __shfl_xor_sync(0xffffffffu, bias, 1);    // e runs over whole warps
+                bias += __shfl_xor_sync(0xffffffffu, bias, 2);
+                if ((ln & 3) == 0) qb[(nr * NB + blk) * 8 + ln / 4] = bias;
+            }
         }
         const bool any_hole = __syncthreads_or(hole);
         float m[NR][2], nm[NR][2], l[NR][2], o[NR][MT][4];   // m in units of log2: score * sl; nm = -m, or 0 at the start
         int lim[NR][2];                         // positions that rows 2 t, 2 t + 1 of a group see
-        float qi[NR == 1 ? NB : 1][2];          // the lane's qb, in registers where they fit
+        float qi[NR == 1 && !HL ? NB : 1][2];   // the lane's qb, in registers where they fit
 #pragma unroll
         for (int nr = 0; nr < NR; ++nr) {
 #pragma unroll
@@ -257,7 +261,7 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
 #pragma unroll
             for (int i = 0; i < MT; ++i) o[nr][i][0] = o[nr][i][1] = o[nr][i][2] = o[nr][i][3] = 0.f;
         }
-        if constexpr (NR == 1) {
+        if constexpr (NR == 1 && !HL) {
 #pragma unroll
             for (int blk = 0; blk < NB; ++blk) qi[blk][0] = qb[blk * 8 + 2 * t], qi[blk][1] = qb[blk * 8 + 2 * t + 1];
         }
@@ -299,8 +303,8 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
                     for (int i = 0; i < 2; ++i) {
                         const uint32_t w = kw[i][blk];
                         if constexpr (HL) {
-                            f[i][0] = field(w << 4, kHigh, expo.e64), f[i][1] = field(w, kHigh, expo.e64);
-                            f[i][2] = field(w >> 4, kHigh, expo.e64), f[i][3] = field(w >> 8, kHigh, expo.e64);
+                            f[i][0] = u32(low_codes(w, expo)), f[i][1] = u32(high_codes(w, expo));
+                            f[i][2] = u32(low_codes(w >> 8, expo)), f[i][3] = u32(high_codes(w >> 8, expo));
                         } else {
                             f[i][0] = field(w, kLow, expo.e1024), f[i][1] = field(w, kHigh, expo.e64);
                             f[i][2] = field(w >> 8, kLow, expo.e1024), f[i][3] = field(w >> 8, kHigh, expo.e64);
@@ -309,8 +313,9 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
                     const float d0 = __half2float(kd[0][blk]), d1 = __half2float(kd[1][blk]);
 #pragma unroll
                     for (int nr = 0; nr < NR; ++nr) {
-                        float acc[4], i0, i1;
-                        if constexpr (NR == 1) i0 = qi[blk][0], i1 = qi[blk][1];
+                        float acc[4], i0 = 0.f, i1 = 0.f;
+                        if constexpr (HL) {
+                        } else if constexpr (NR == 1) i0 = qi[blk][0], i1 = qi[blk][1];
                         else {
                             const float2 v = *reinterpret_cast<const float2 *>(qb + (nr * NB + blk) * 8 + 2 * t);
                             i0 = v.x, i1 = v.y;
@@ -377,7 +382,8 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
 #pragma unroll
             for (int tt = 0; tt < TT; ++tt) {
                 if (EDGE && tt >= n) break;
-                uint32_t ph[NR][2], pl[NR][2];
+                uint32_t ph[NR][2];
+                [[maybe_unused]] uint32_t pl[NR][2];
 #pragma unroll
                 for (int nr = 0; nr < NR; ++nr) {
                     float p[4];
@@ -385,10 +391,16 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
                     for (int i = 0; i < 4; ++i) p[i] = ex2(fmaf(sc[tt][nr][i], a.sl, nm[nr][i & 1]));
                     l[nr][0] += p[0] + p[2];
                     l[nr][1] += p[1] + p[3];
-                    split2(p[0], p[1], ph[nr][0], pl[nr][0]);
-                    split2(p[2], p[3], ph[nr][1], pl[nr][1]);
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) ph[nr][i] = transpose8(ph[nr][i]), pl[nr][i] = transpose8(pl[nr][i]);
+                    for (int i = 0; i < 2; ++i) {
+                        if constexpr (HL) {
+                            split2(p[2 * i], p[2 * i + 1], ph[nr][i], pl[nr][i]);
+                            pl[nr][i] = transpose8(pl[nr][i]);
+                        } else {
+                            ph[nr][i] = u32(__floats2half2_rn(p[2 * i], p[2 * i + 1]));
+                        }
+                        ph[nr][i] = transpose8(ph[nr][i]);
+                    }
                 }
                 // ---- O += P V: this lane's positions t + 4 m, dims g * D / 8 .. ----
                 const uint8_t *vp = sp + tt * L::BYTES;
@@ -427,8 +439,16 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
                             const uint32_t a2 = u32(__hmul2(low_codes(ye, expo), db)), a3 = u32(__hmul2(high_codes(ye, expo), db));
 #pragma unroll
                             for (int nr = 0; nr < NR; ++nr) {
-                                mma(o[nr][4 * w + 2 * hf + e], a0, a1, a2, a3, ph[nr][0], ph[nr][1]);
-                                mma(o[nr][4 * w + 2 * hf + e], a0, a1, a2, a3, pl[nr][0], pl[nr][1]);
+                                float(&sum)[4] = o[nr][4 * w + 2 * hf + e];
+                                if constexpr (HL) {
+                                    float x4[4];
+                                    mma_init(x4, a0, a1, a2, a3, ph[nr][0], ph[nr][1], 0.f, 0.f);
+                                    mma(x4, a0, a1, a2, a3, pl[nr][0], pl[nr][1]);
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i) sum[i] += x4[i];
+                                } else {
+                                    mma(sum, a0, a1, a2, a3, ph[nr][0], ph[nr][1]);
+                                }
                             }
                         }
                     }
