@@ -202,11 +202,10 @@ int x100q_rope_table_dev(float *rope, int n_pos, int head_dim, float base, void 
  * not decrease or pass n_tokens; a sequence that breaks this is left out, and the
  * next synchronising call reports X100_E_ARG.
  * X100Q_F32: q (|q| <= 65504, as two fp16 halves) and the probabilities are used
- * to 22 bits; X100Q_F16: from 256 rows (tokens times n_heads / n_kv_heads) a sequence
- * on, probabilities are rounded to fp16, and out is rounded once.  All sums are
- * fp32, the tensor cores' own (truncating) for 16 positions at a time: over 131072
- * positions they are off by less than 1e-4 (6e-5 measured, where one block has them
- * all; 2e-5 where the call spreads a sequence over blocks).
+ * to 22 bits, and sums are fp32 additions over tiles of 16 or 128 positions.
+ * X100Q_F16: probabilities are rounded to fp16 and out is rounded once; sums are the
+ * tensor cores' own, fp32 and truncating, which over 131072 positions loses less
+ * than 1e-4 of them.
  * The result does not depend on the order in which blocks run.
  * work: 16-byte aligned device scratch of x100q_kv4_attn_work() bytes; its
  * contents need not be kept or cleared, but calls that overlap on the GPU

@@ -105,8 +105,8 @@ def attention_bound(q, k, v, scale, n, half):
     size at each of its 2 D / 16 steps and D / 32 fp32 updates follow: with A = scale * max sum |q k| at most
     A * (2^-22 + (D / 8 + D / 32) * 2^-23). exp2 of it (and its argument's rounding, A * 2^-23 again) moves p by that
     relatively, 2^-21 more for exp2 itself and p's split into halves. Numerator and sum both carry it (factor 2).
-    The sum over positions takes a step for 16 positions of a warp (two for fp32 q), at most n / 128 * 2 + 2 of them, and 2^-23
-    each; joining 8 warps and up to 320 runs adds 2^-24 each. All relative to sum p |v| <= max |v|. fp16 q: p of the numerator is
+    The sum over positions takes a step for 16 positions of a warp (two, and an fp32 addition, for fp32 q), at most n / 128 * 2 + 2
+    of them, and 2^-23 each; joining 8 warps and up to 320 runs adds 2^-24 each. All relative to sum p |v| <= max |v|. fp16 q: p of the numerator is
     rounded to fp16, 2^-11, or 2^-25 where it is subnormal (the sum below is at least 1, of the position that set the maximum), and
     the output adds half a step."""
     D = q.shape[-1]
@@ -136,8 +136,8 @@ def prompt_bound(q, k, v, scale, n, half):
 
     Scores as in attention_bound. fp16 q: p is rounded to fp16 in the numerator alone, half a step of p, 2^-11, or 2^-25 where it
     is subnormal (the sum below it is at least 1, of the position that set the maximum); its sums take n / 16 steps of 2^-23.
-    fp32 q: p in halves as there; hi and lo go 2 steps for 16 positions, every other tile to a sum of its own, and a sum
-    ends after 32 tiles, so n / 16 and at most 512 steps, then at most n / 8192 + 1 joins of 2^-22."""
+    fp32 q: p in halves as there; a tile's sum takes 16 steps, and the tiles are added in fp32, 2^-24 each and as much
+    again for the factor of a tile's max."""
     D = q.shape[-1]
     A = scale * max(float(np.abs(q).reshape(-1, D).max(0) @ np.abs(k).reshape(-1, D).max(0)), 1e-30) if k.size else 0.0
     top = float(np.abs(v).max()) if v.size else 0.0
@@ -145,5 +145,5 @@ def prompt_bound(q, k, v, scale, n, half):
     if half:
         rel += 2 * 2.0 ** -11 + n * 2.0 ** -25 + (n / 16 + 8) * 2.0 ** -23
     else:
-        rel += min(n / 16 + 16, 528) * 2.0 ** -23 + (n / 8192 + 1) * 2.0 ** -22
+        rel += 16 * 2.0 ** -23 + (n / 128 + 1) * 2.0 ** -23
     return top * rel + 1e-12

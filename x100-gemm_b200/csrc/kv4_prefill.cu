@@ -6,13 +6,16 @@
 // 128 x 128 x D tcgen05.mma with S, P (over S) and O in TMEM.  One CTA per SM:
 //   warps 0-3, 4-7   softmax of step X = 0, 1: a thread owns a row; S from TMEM, running max
 //                    (moved only when a score passes it by 2^8), P as fp16 back to TMEM
+//   fp32 q: 4 warps  add up the products of the steps, a row each (below)
 //   4 or 8 warps     raw codes in shared memory -> fp16 K and V tiles in the 128-byte-swizzled
 //                    layouts the MMA reads; scale * (code - 8) is an fp16 value, so exact
 //   a warp each      issues the MMAs; copies the raw tiles (bulk copies);
 //                    walks the work list and hands every role its segments through shared memory
 // fp16 q: the steps X are two row tiles over the same key tile (256 rows per item), so that
-// a key tile is unpacked once for both.  fp32 q: q and P are carried as hi + lo halves, two
-// products each, and the steps X are every other key tile of one row tile, joined at the end.
+// a key tile is unpacked once for both; O stays in TMEM.  fp32 q: q and P are carried as hi + lo halves, two
+// products each, the steps X are every other key tile of one row tile, and O of a step is added to fp32
+// registers: summed in TMEM it was off by 3e-6 at 2600 positions and more at each further one, and is now by 3e-7,
+// for 134 us instead of 108 (1024 tokens over 2600 positions, 32 heads).
 // Either way one step's softmax runs beside the other's products.
 //
 // The work list is the one of kv4_attn.cu with units of 128 positions, each row
@@ -29,11 +32,12 @@ constexpr int kKeys = 128;                 // positions per key tile
 constexpr int kPfCtas = 160;               // bound of the grid, which sizes the workspace
 constexpr int kPfRows = 256;               // rows per slot of the workspace
 
-// Warps that unpack: four feed two row tiles per key tile (fp16 q; more of them only take issue slots from the
-// softmax: 488 against 509 us for 2048 tokens over 16384 positions), eight feed a key tile per step (fp32 q).
+// Warps: 8 of softmax, ACC that add up the sums (fp32 q), DQ that unpack, then one each.  SEGS: those that read segments.  Four
+// unpacking warps feed two row tiles per key tile (fp16 q; eight only take issue slots from the softmax: 488 against 509 us
+// for 2048 tokens over 16384 positions), eight a key tile per step (fp32 q; 135 against 168 us with four).
 template <typename T>
 struct Roles {
-    static constexpr int DQ = sizeof(T) == 4 ? 8 : 4, kMma = 8 + DQ, THREADS = (8 + DQ + 4) * 32, SEGS = 8 + DQ + 2;   // SEGS: warps that read segments
+    static constexpr int ACC = sizeof(T) == 4 ? 4 : 0, DQ = sizeof(T) == 4 ? 8 : 4, kDq = 8 + ACC, kMma = kDq + DQ, THREADS = (kMma + 4) * 32, SEGS = kMma + 2;
 };
 
 template <int D>
@@ -78,6 +82,11 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r) {
         "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t *r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 template <int N>
@@ -167,15 +176,10 @@ __device__ __forceinline__ Start my_start(const AttnArgs &a) {
         }
     }
 }
-// A segment: key tiles c0 .. c0 + n - 1 of an item (all cu of them, or a part).  A run's part of an item is one segment, but for
-// fp32 q at most kPiece key tiles long: a tensor-core sum loses up to an ulp of what it holds with each product (it truncates; 1.9e-8
-// relative a step measured), which over 131072 positions would be 1.5e-4.  Pieces are added up in fp32 in the slot of their part.
-constexpr int kPiece = 64;
+// A segment: key tiles c0 .. c0 + n - 1 of an item (all cu of them, or a part).
 struct Seg {
     int n;                                 // 0: the run is over
     int c0, cu, b, kvh, rt, q0, nq, len, row;
-    int first, slot;                       // the first key tile of the part, and its slot (of the CTA's two)
-    bool more;                             // the part has another piece
     uint32_t item;                         // the item's first unit
 };
 constexpr int kSegs = 4;                   // ring of segments
@@ -184,12 +188,13 @@ constexpr int kSegs = 4;                   // ring of segments
 // also what frees that tile's stage (fp16 q, X = 1) and the issuing warp commits only twice a step.
 struct PfBars {
     uint64_t raw_full[kRawStages], raw_empty[kRawStages], k_full[2], k_empty[2], v_full[2], v_empty[2];
-    uint64_t s_full[2][2], p_ready[2], o_done[2][2], q_full, q_empty, joined, drain, seg_full[kSegs], seg_empty[kSegs];
+    uint64_t s_full[2][2], p_ready[2], o_done[2][2], q_full, q_empty, drain, o_free[2], fin, ml_free, seg_full[kSegs], seg_empty[kSegs];
     uint32_t raw_ok[kRawStages];           // bit i: 16-position tile i of the raw stage was copied
     uint32_t tmem;
     int abort_flag;
     Seg seg[kSegs];
-    float2 ml[2][128];
+    float2 ml[2][128];                     // fp32 q: (m, l) of the two steps' rows at a segment's end
+    float m_step[2][2][128];               // and the max that a step's products are relative to
 };
 
 // 8 codes of a word times their scale, as fp16 in the order 0, 4, 1, 5, 2, 6, 3, 7
@@ -218,6 +223,29 @@ __device__ __forceinline__ uint64_t add2(uint64_t s, float x, float y) {
     return s;
 }
 
+// C columns of a row from `col` on: times inv to `op` (a live row of a whole item), or as they are to the slot of a part
+template <typename T, int D, int C>
+__device__ __forceinline__ void put_sums(const AttnArgs &a, const float (&o)[C], float inv, int col, bool whole, bool live, T *op, int slot, int prow) {
+    if (!whole) {
+        float4 *pp = reinterpret_cast<float4 *>(a.part) + ((long)slot * (D / 4) + col / 4) * kPfRows + prow;
+#pragma unroll
+        for (int k = 0; k < C / 4; ++k) pp[k * kPfRows] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+    } else if (live) {
+        // columns 0 .. 7 of a group of 8 are its dims 0, 4, 1, 5, 2, 6, 3, 7
+#pragma unroll
+        for (int h = 0; h < C; h += 8) {
+            const float y[8] = {o[h] * inv, o[h + 2] * inv, o[h + 4] * inv, o[h + 6] * inv, o[h + 1] * inv, o[h + 3] * inv, o[h + 5] * inv, o[h + 7] * inv};
+            if constexpr (sizeof(T) == 4) {
+                *reinterpret_cast<float4 *>(op + col + h) = make_float4(y[0], y[1], y[2], y[3]);
+                *reinterpret_cast<float4 *>(op + col + h + 4) = make_float4(y[4], y[5], y[6], y[7]);
+            } else {
+                *reinterpret_cast<uint4 *>(op + col + h) = make_uint4(u32(__floats2half2_rn(y[0], y[1])), u32(__floats2half2_rn(y[2], y[3])),
+                                                                      u32(__floats2half2_rn(y[4], y[5])), u32(__floats2half2_rn(y[6], y[7])));
+            }
+        }
+    }
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(Roles<T>::THREADS, 1) prefill_kernel(const AttnArgs a) {
     using L = Lay<D>;
@@ -240,7 +268,8 @@ __global__ void __launch_bounds__(Roles<T>::THREADS, 1) prefill_kernel(const Att
             mbar_init(&bars.p_ready[i], 4);
             for (int k = 0; k < 2; ++k) mbar_init(&bars.s_full[i][k], 1), mbar_init(&bars.o_done[i][k], 1);
         }
-        mbar_init(&bars.q_full, 8), mbar_init(&bars.q_empty, 1), mbar_init(&bars.joined, 8), mbar_init(&bars.drain, 1);
+        mbar_init(&bars.q_full, 8), mbar_init(&bars.q_empty, 1), mbar_init(&bars.drain, 1);
+        mbar_init(&bars.o_free[0], 4), mbar_init(&bars.o_free[1], 4), mbar_init(&bars.fin, 8), mbar_init(&bars.ml_free, 4);
         fence_barrier_init();
     }
     if (warp == W::kMma) {
@@ -268,16 +297,11 @@ __global__ void __launch_bounds__(Roles<T>::THREADS, 1) prefill_kernel(const Att
     if (!ok && threadIdx.x == 0) atomicCAS(a.status, 0, X100_E_LAUNCH);
     if (wg < 2) {
         // ================================ softmax ================================
-        // registers: the launch's 65536 (512 threads of 128) or 61440 (640 of 96) shared out anew
-        regs_more<HL ? 168 : 192>();
+        // registers: the launch's 65536 (512 threads of 128) or 61440 (768 of 80) shared out anew; fp32 q's softmax keeps its 80
+        regs_more<HL ? 80 : 192>();
         const int X = wg, row = threadIdx.x & 127;
         const uint32_t toff = (uint32_t)((warp & 3) * 32) << 16, sx = tS + 128 * X + toff, ox = tO + 128 * X + toff;
-        uint32_t step = 0, joins = 0;            // steps of this X, meetings of the two groups so far
-        auto meet = [&]() {                      // both groups (bounded, unlike a named barrier)
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bars.joined);
-            return wait(&bars.joined, joins++ & 1);
-        };
+        uint32_t step = 0;                       // steps of this X
         // q of a segment: this row's halves into the swizzled K-major tiles (HL: both groups, half of the dims each)
         auto put_q = [&](const Seg &v) {
             const int r = v.rt * RT + (HL ? 0 : 128 * X) + row;
@@ -307,7 +331,6 @@ __global__ void __launch_bounds__(Roles<T>::THREADS, 1) prefill_kernel(const Att
             if (lane == 0) mbar_arrive(&bars.q_full);
         };
         uint32_t nseg = 0;
-        float m_sum = -INFINITY, l_sum = 0.f;    // of the part's earlier pieces (HL)
         ok = segment(0);
         if (ok && bars.seg[0].n) put_q(bars.seg[0]);
         for (; ok; ++nseg) {
@@ -329,45 +352,51 @@ __global__ void __launch_bounds__(Roles<T>::THREADS, 1) prefill_kernel(const Att
                 if (hole && lane == 0) atomicCAS(a.status, 0, X100_E_ARG);
             }
             float m = -INFINITY, nm = 0.f, l = 0.f;
-            const bool any = !HL || X < n;       // this group has steps
             const uint64_t sl2 = both(a.sl);
             for (int c = HL ? X : 0; c < n; c += HL ? 2 : 1, ++step) {
                 const int p0 = (c0 + c) * kKeys;
                 ok = wait(&bars.s_full[X][step & 1], step >> 1 & 1);
                 if (!ok) break;
                 tc_fence_after();
-                float s[128];
+                const bool mask = __any_sync(0xffffffffu, p0 + kKeys > lim) || hole;
+                uint32_t gone = 0;               // 16-position tiles without a page
+                if (hole)
+                    for (int i = 0; i < 8 && p0 + 16 * i < len; ++i)
+                        if ((unsigned)__ldg(trow + ((p0 + 16 * i) >> a.pool.page_shift)) >= (unsigned)a.pool.n_pages) gone |= 1u << i;
+                // scores 32 i .. of the row.  fp16 q keeps all of them; fp32 q, whose registers the sums need, loads them twice
+                auto load = [&](float *v, int i) { tmem_ld32(sx + 32 * i, *reinterpret_cast<uint32_t(*)[32]>(v)); };
+                auto cover = [&](float *v, int i) {
+                    const int cut = lim - p0 - 32 * i;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) tmem_ld32(sx + 32 * i, *reinterpret_cast<uint32_t(*)[32]>(s + 32 * i));
-                tmem_wait_ld();
-                if (__any_sync(0xffffffffu, p0 + kKeys > lim) || hole) {
-                    const int cut = lim - p0;
+                    for (int k = 0; k < 32; ++k)
+                        if (k >= cut) v[k] = -INFINITY;
+                    if (gone) {
 #pragma unroll
-                    for (int i = 0; i < 128; ++i)
-                        if (i >= cut) s[i] = -INFINITY;
-                    if (hole) {
-                        uint32_t gone = 0;
-                        for (int i = 0; i < 8 && p0 + 16 * i < len; ++i)
-                            if ((unsigned)__ldg(trow + ((p0 + 16 * i) >> a.pool.page_shift)) >= (unsigned)a.pool.n_pages) gone |= 1u << i;
-#pragma unroll
-                        for (int i = 0; i < 128; ++i)
-                            if (gone >> (i / 16) & 1) s[i] = -INFINITY;
+                        for (int k = 0; k < 32; ++k)
+                            if (gone >> (2 * i + k / 16) & 1) v[k] = -INFINITY;
                     }
+                };
+                float s[HL ? 32 : 128], mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int h = 0; h < 128; h += HL ? 32 : 128) {
+#pragma unroll
+                    for (int i = 0; i < (HL ? 1 : 4); ++i) load(s + 32 * i, h / 32 + i);
+                    tmem_wait_ld();
+                    if (mask)
+#pragma unroll
+                        for (int i = 0; i < (HL ? 1 : 4); ++i) cover(s + 32 * i, h / 32 + i);
+#pragma unroll
+                    for (int i = 0; i < (HL ? 32 : 128); i += 8)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) mx[k] = fmaxf(fmaxf(mx[k], s[i + k]), s[i + 4 + k]);
                 }
-                float mx[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-                for (int i = 4; i < 124; i += 8)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) mx[k] = fmaxf(fmaxf(mx[k], s[i + k]), s[i + 4 + k]);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], s[124 + k]);
                 const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.sl;
                 if (__any_sync(0xffffffffu, top > m + 8.f)) {
                     const float mn = fmaxf(m, top), f = mn == -INFINITY ? 1.f : ex2(m - mn);
                     m = mn;
                     nm = mn == -INFINITY ? 0.f : -mn;
                     l *= f;
-                    if (c >= (HL ? 2 : 1)) {     // O holds sums
+                    if (!HL && c >= 1) {         // O holds sums
                         ok = wait(&bars.o_done[X][(step - 1) & 1], (step - 1) >> 1 & 1);
                         if (!ok) break;
                         tc_fence_after();
@@ -382,22 +411,32 @@ __global__ void __launch_bounds__(Roles<T>::THREADS, 1) prefill_kernel(const Att
                         }
                     }
                 }
+                if constexpr (HL) bars.m_step[X][step & 1][row] = m;
                 const uint64_t nm2 = both(nm);
                 uint64_t sum[2] = {0ull, 0ull};   // two floats each
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    uint32_t hi[16], lo[16];
+                    float *v = s + (HL ? 0 : 32 * i);
+                    if constexpr (HL) {
+                        load(v, i);
+                        tmem_wait_ld();
+                        if (mask) cover(v, i);
+                    }
+                    uint32_t hi[16], lo[8];
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
-                        float x = s[32 * i + 2 * k], y = s[32 * i + 2 * k + 1];
+                        float x = v[2 * k], y = v[2 * k + 1];
                         fma2(x, y, sl2, nm2);
                         x = ex2(x), y = ex2(y);
                         sum[k & 1] = add2(sum[k & 1], x, y);
-                        if constexpr (HL) split2(x, y, hi[k], lo[k]);
-                        else hi[k] = u32(__floats2half2_rn(x, y));
+                        if constexpr (HL) {              // 16 positions' hi and lo over the scores they came from
+                            split2(x, y, hi[k & 7], lo[k & 7]);
+                            if (k % 8 == 7) tmem_st8(sx + 32 * i + 2 * (k - 7), hi), tmem_st8(sx + 32 * i + 2 * (k - 7) + 8, lo);
+                        } else {
+                            hi[k] = u32(__floats2half2_rn(x, y));
+                        }
                     }
-                    tmem_st16(sx + 16 * i, hi);
-                    if constexpr (HL) tmem_st16(sx + 64 + 16 * i, lo);
+                    if constexpr (!HL) tmem_st16(sx + 16 * i, hi);
                 }
                 {
                     float s0, s1, s2, s3;
@@ -418,107 +457,107 @@ __global__ void __launch_bounds__(Roles<T>::THREADS, 1) prefill_kernel(const Att
                 ok = wait(&bars.q_empty, nseg & 1);
                 if (ok) put_q(bars.seg[(nseg + 1) % kSegs]);
             }
+            if constexpr (HL) {
+                if (ok) ok = wait(&bars.ml_free, (nseg & 1) ^ 1);
+                bars.ml[X][row] = make_float2(m, l);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars.fin);
+                release(nseg);
+                continue;
+            }
             // ---- out ----
-            if (ok && any) ok = wait(&bars.o_done[X][(step - 1) & 1], (step - 1) >> 1 & 1);
-            // HL: each group puts half of the dims out, of its own sums and of the other's (the same lanes of tensor memory)
-            float f = 1.f, fo = 0.f;
-            if constexpr (HL) {
-                if (ok) {
-                    bars.ml[X][row] = make_float2(m, l);
-                    ok = meet();
-                }
-                const float2 other = bars.ml[X ^ 1][row];
-                const float M = fmaxf(m, other.x);
-                f = M == -INFINITY ? 0.f : ex2(m - M);
-                fo = M == -INFINITY ? 0.f : ex2(other.x - M);
-                l = l * f + other.y * fo;
-                m = M;
-            }
-            // with what the part's earlier pieces left in the slot, times fs
-            const bool join = HL && c0 != w.first, more = HL && w.more;
-            float fs = 0.f;
-            if constexpr (HL) {
-                if (join) {
-                    const float M = fmaxf(m, m_sum), g = M == -INFINITY ? 0.f : ex2(m - M);
-                    fs = M == -INFINITY ? 0.f : ex2(m_sum - M);
-                    l = l * g + l_sum * fs;
-                    f *= g, fo *= g;
-                    m = M;
-                }
-                m_sum = m, l_sum = l;
-            }
+            if (ok) ok = wait(&bars.o_done[X][(step - 1) & 1], (step - 1) >> 1 & 1);
             if (!ok) break;
             tc_fence_after();
-            const int r = w.rt * RT + (HL ? 0 : 128 * X) + row;
-            const bool live = r < w.nq * a.G, whole = w.first == 0 && c0 + n == w.cu, two = HL && n > 1;   // one key tile: step 1 has no sums
+            const int r = w.rt * RT + 128 * X + row;
+            const bool live = r < w.nq * a.G, whole = n == w.cu;
             const int tok = live ? div_g(a, r) : 0;
-            const int slot = (int)blockIdx.x * 2 + w.slot, prow = HL ? row : 128 * X + row;
+            const int slot = (int)blockIdx.x * 2 + (nseg ? 1 : 0);
             const float inv = whole ? (l > 0.f ? 1.f / l : 0.f) : 1.f;
-            const float f0 = HL ? (X ? fo : f) : 1.f, f1 = HL ? (X ? f : fo) : 0.f;
             T *op = static_cast<T *>(a.out) + (long)(w.q0 + tok) * a.os + (long)(w.kvh * a.G + r - tok * a.G) * D;
-            // every round trip to tensor memory takes some hundred cycles: 64 columns at a time, 16 where two sums' are held
-            constexpr int CW = HL ? 16 : 64;
 #pragma unroll
-            for (int j = 0; j < (HL ? D / 2 : D) / CW; ++j) {
-                const int col = (HL ? X * (D / 2) : 0) + j * CW;
-                float o[CW], o1[HL ? CW : 1];
+            for (int col = 0; col < D; col += 64) {  // every round trip to tensor memory takes some hundred cycles
+                float o[64];
 #pragma unroll
-                for (int k = 0; k < CW; k += 16) tmem_ld16((HL ? tO + toff : ox) + col + k, *reinterpret_cast<uint32_t(*)[16]>(o + k));
-                if constexpr (HL) {
-                    if (two) tmem_ld16(tO + 128 + toff + col, *reinterpret_cast<uint32_t(*)[16]>(o1));
-                }
+                for (int k = 0; k < 64; k += 16) tmem_ld16(ox + col + k, *reinterpret_cast<uint32_t(*)[16]>(o + k));
                 tmem_wait_ld();
-#pragma unroll
-                for (int k = 0; k < CW; ++k) {
-                    o[k] *= f0;
-                    if constexpr (HL) {
-                        if (two) o[k] = fmaf(o1[k], f1, o[k]);
-                    }
-                }
-                float4 *pp = reinterpret_cast<float4 *>(a.part) + ((long)slot * (D / 4) + col / 4) * kPfRows + prow;
-                if constexpr (HL) {
-                    if (join) {
-#pragma unroll
-                        for (int k = 0; k < CW / 4; ++k) {
-                            const float4 y = pp[k * kPfRows];
-                            o[4 * k] = fmaf(y.x, fs, o[4 * k]), o[4 * k + 1] = fmaf(y.y, fs, o[4 * k + 1]);
-                            o[4 * k + 2] = fmaf(y.z, fs, o[4 * k + 2]), o[4 * k + 3] = fmaf(y.w, fs, o[4 * k + 3]);
-                        }
-                    }
-                }
-                if (!whole || more) {
-#pragma unroll
-                    for (int k = 0; k < CW / 4; ++k) pp[k * kPfRows] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
-                } else if (live) {
-                    // columns 0 .. 7 of a group of 8 are its dims 0, 4, 1, 5, 2, 6, 3, 7
-#pragma unroll
-                    for (int h = 0; h < CW; h += 8) {
-                        const float y[8] = {o[h] * inv, o[h + 2] * inv, o[h + 4] * inv, o[h + 6] * inv,
-                                            o[h + 1] * inv, o[h + 3] * inv, o[h + 5] * inv, o[h + 7] * inv};
-                        if constexpr (HL) {
-                            *reinterpret_cast<float4 *>(op + col + h) = make_float4(y[0], y[1], y[2], y[3]);
-                            *reinterpret_cast<float4 *>(op + col + h + 4) = make_float4(y[4], y[5], y[6], y[7]);
-                        } else {
-                            *reinterpret_cast<uint4 *>(op + col + h) =
-                                make_uint4(u32(__floats2half2_rn(y[0], y[1])), u32(__floats2half2_rn(y[2], y[3])),
-                                           u32(__floats2half2_rn(y[4], y[5])), u32(__floats2half2_rn(y[6], y[7])));
-                        }
-                    }
-                }
+                put_sums<T, D, 64>(a, o, inv, col, whole, live, op, slot, 128 * X + row);
             }
-            if (!whole && !more && (!HL || X == 0)) {
-                a.ml[(long)slot * kPfRows + prow] = make_float2(m, l);
-                if (X == 0 && row == 0) a.meta[slot] = make_int4((int)w.item, w.b, w.kvh, w.rt | (w.first ? kInside : 0));
+            if (!whole) {
+                a.ml[(long)slot * kPfRows + 128 * X + row] = make_float2(m, l);
+                if (X == 0 && row == 0) a.meta[slot] = make_int4((int)w.item, w.b, w.kvh, w.rt | (c0 ? kInside : 0));
             }
             tc_fence_before();                      // the next step's products overwrite the sums
-            if constexpr (HL) ok = meet();          // both groups have read them
+            release(nseg);
+        }
+    } else if (HL && warp < W::kDq) {
+        // ================================ sums (fp32 q) ================================
+        // A tensor-core sum truncates, 1.9e-8 of what it holds at each product, 16 a step.  So each step's products start
+        // from zero, and these warps add the steps up, each by its max; a thread has a row.
+        regs_more<176>();
+        const int row = threadIdx.x & 127;
+        const uint32_t toff = (uint32_t)((warp & 3) * 32) << 16;
+        uint32_t steps = 0;                      // X = 1's in the high half
+        for (uint32_t nseg = 0; ok; ++nseg) {
+            ok = segment(nseg);
+            if (!ok) break;
+            const Seg &w = bars.seg[nseg % kSegs];
+            const int n = w.n;
+            if (n == 0) break;
+            float o[HL ? D : 64], M = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < D; ++i) o[i] = 0.f;
+            for (int c = 0; c < n; ++c) {
+                const int X = c & 1;
+                const uint32_t st = steps >> (16 * X);
+                ok = wait(&bars.o_done[X][st & 1], st >> 1 & 1);
+                if (!ok) break;
+                tc_fence_after();
+                const float mx = bars.m_step[X][st & 1][row], mn = fmaxf(M, mx);
+                if (__any_sync(0xffffffffu, mx > M)) {
+                    const float f = mn == -INFINITY ? 0.f : ex2(M - mn);
+#pragma unroll
+                    for (int i = 0; i < D; ++i) o[i] *= f;
+                    M = mn;
+                }
+                const float f = mx == -INFINITY ? 0.f : ex2(mx - M);
+#pragma unroll
+                for (int i = 0; i < D; i += 32) {
+                    float v[32];
+                    tmem_ld32(tO + 128 * X + toff + i, *reinterpret_cast<uint32_t(*)[32]>(v));
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) o[i + k] = fmaf(v[k], f, o[i + k]);
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars.o_free[X]);
+                steps = X ? steps + 0x10000u : (steps & 0xffff0000u) | (steps + 1 & 0xffffu);
+            }
+            if (ok) ok = wait(&bars.fin, nseg & 1);
+            if (!ok) break;
+            const float2 s0 = bars.ml[0][row], s1 = bars.ml[1][row];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.ml_free);
+            // M is the larger max of the last step of either; a later, lower one cannot be
+            const float l = M == -INFINITY ? 0.f : s0.y * ex2(s0.x - M) + s1.y * ex2(s1.x - M);
+            const int r = w.rt * RT + row;
+            const bool live = r < w.nq * a.G, whole = n == w.cu;
+            const int tok = live ? div_g(a, r) : 0, slot = (int)blockIdx.x * 2 + (nseg ? 1 : 0);
+            const float inv = whole ? (l > 0.f ? 1.f / l : 0.f) : 1.f;
+            T *op = static_cast<T *>(a.out) + (long)(w.q0 + tok) * a.os + (long)(w.kvh * a.G + r - tok * a.G) * D;
+            put_sums<T, D, HL ? D : 64>(a, o, inv, 0, whole, live, op, slot, row);
+            if (!whole) {
+                a.ml[(long)slot * kPfRows + row] = make_float2(M, l);
+                if (row == 0) a.meta[slot] = make_int4((int)w.item, w.b, w.kvh, w.rt | (w.c0 ? kInside : 0));
+            }
             release(nseg);
         }
     } else if (warp < W::kMma) {
         // ================================ codes -> fp16 tiles ================================
         regs_less<HL ? 48 : 72>();
         const Exponents expo;
-        const int th = threadIdx.x - 256;
+        const int th = threadIdx.x - W::kDq * 32;
         uint32_t tile = 0, raw = 0;                // key tiles, raw stages so far
         for (uint32_t nseg = 0; ok; ++nseg) {
             ok = segment(nseg);
@@ -571,7 +610,7 @@ __global__ void __launch_bounds__(Roles<T>::THREADS, 1) prefill_kernel(const Att
 #pragma unroll
                 for (int u = 0; u < 8 / kDqWarps; ++u) {
                     // a warp has a 16-position tile; a lane the D / 8 dims from g * D / 8 of positions t + 4 m
-                    const int tl = u * kDqWarps + warp - 8, g = lane >> 2, t = lane & 3;
+                    const int tl = u * kDqWarps + warp - W::kDq, g = lane >> 2, t = lane & 3;
                     const uint32_t rs = (raw + (tl >> 2)) % kRawStages;
                     const uint8_t *tp = sm + P::RAW0 + rs * P::RAW + (tl & 3) * L::BYTES;
                     const int left = bars.raw_ok[rs] >> (tl & 3) & 1 ? len - c * kKeys : 0;   // positions of the sequence from the key tile on
@@ -647,15 +686,16 @@ __global__ void __launch_bounds__(Roles<T>::THREADS, 1) prefill_kernel(const Att
                     const uint32_t tl = tile + (HL ? s : s >> 1), st = tl & 1, done = pdone >> (16 * X);
                     ok = wait(&bars.p_ready[X], done & 1);
                     if (ok && (HL || X == 0)) ok = wait(&bars.v_full[st], tl >> 1 & 1);
+                    if (HL && ok) ok = wait(&bars.o_free[X], (done & 1) ^ 1);
                     if (!ok) break;
                     tc_fence_after();
                     const uint64_t vd = descV + st * (P::KT >> 4);
-                    const uint32_t more = s >= 2 ? 1u : 0u;      // O of X holds sums of the segment
+                    const uint32_t more = !HL && s >= 2 ? 1u : 0u;      // O of X holds sums of the segment
 #pragma unroll
                     for (int p = 0; p < (HL ? 2 : 1); ++p)
 #pragma unroll
                         for (int k = 0; k < VS; ++k)
-                            umma_ts(tO + 128 * X, tS + 128 * X + 64 * p + 8 * k, vd + k * (2048 >> 4), idO, (p | k) ? 1u : more, lead);
+                            umma_ts(tO + 128 * X, tS + 128 * X + (HL ? 16 * k + 8 * p : 8 * k), vd + k * (2048 >> 4), idO, (p | k) ? 1u : more, lead);
                     umma_commit_lead(&bars.o_done[X][done & 1], lead);
                     pdone += 1u << (16 * X);
                     if (HL) umma_commit_lead(&bars.v_empty[st], lead);
@@ -706,7 +746,7 @@ __global__ void __launch_bounds__(Roles<T>::THREADS, 1) prefill_kernel(const Att
         } else if (warp == W::kMma + 2) {
             // ================================ work list ================================
             const Start at = my_start<RT>(a);
-            uint32_t u = at.u0, item = at.item, nseg = 0, parts = 0;
+            uint32_t u = at.u0, item = at.item, nseg = 0;
             int b = at.b, kvh = at.kvh, rt = at.rt;
             Seq sq;
             if (u < at.u1) sq = load_seq(a, b, RT, false);
@@ -716,9 +756,8 @@ __global__ void __launch_bounds__(Roles<T>::THREADS, 1) prefill_kernel(const Att
                 if (more) {
                     // a run that ends within an item's kLead units has none of its key tiles, and one that starts there has all
                     const int cu = units_of<RT>(a, sq, rt) - kLead, k0 = (int)(u - item), k1 = (int)min((uint32_t)(cu + kLead), k0 + (at.u1 - u));
-                    g.c0 = g.first = max(0, k0 - kLead);
+                    g.c0 = max(0, k0 - kLead);
                     g.n = max(0, k1 - kLead) - g.c0;
-                    g.slot = parts ? 1 : 0;
                     g.cu = cu, g.b = b, g.kvh = kvh, g.rt = rt, g.q0 = sq.q0, g.nq = sq.nq, g.len = sq.len, g.row = sq.row, g.item = item;
                     item += cu + kLead;
                     u = item;
@@ -731,21 +770,14 @@ __global__ void __launch_bounds__(Roles<T>::THREADS, 1) prefill_kernel(const Att
                         }
                     }
                     if (g.n == 0) continue;
-                    ++parts;
                 }
-                for (int left = g.n;; g.c0 += g.n) {
-                    if (HL) g.n = min(left, kPiece);
-                    left -= g.n;
-                    g.more = left > 0;
-                    ok = wait(&bars.seg_empty[nseg % kSegs], (nseg / kSegs & 1) ^ 1);
-                    if (!ok) break;
-                    if (lane == 0) {
-                        bars.seg[nseg % kSegs] = g;
-                        mbar_arrive(&bars.seg_full[nseg % kSegs]);
-                    }
-                    ++nseg;
-                    if (!g.more) break;
+                ok = wait(&bars.seg_empty[nseg % kSegs], (nseg / kSegs & 1) ^ 1);
+                if (!ok) break;
+                if (lane == 0) {
+                    bars.seg[nseg % kSegs] = g;
+                    mbar_arrive(&bars.seg_full[nseg % kSegs]);
                 }
+                ++nseg;
             }
         }
     }
