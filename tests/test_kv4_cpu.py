@@ -135,3 +135,11 @@ def test_scratch_follows_the_rows_a_sequence_can_have():
 def test_calls_past_the_work_list_are_refused(big):
     a = x100b.Kv4AttnArgs(**dict(ATTN, n_tokens=1 << 20, work_bytes=1 << 40, **big))
     assert x100b.lib().x100q_kv4_attn_dev(C.byref(kv()), C.byref(a), None) == x100b.X100_E_TOO_LARGE
+
+
+@pytest.mark.parametrize("pack,args", [(x100b._APPEND, x100b.Kv4AppendArgs), (x100b._ATTN, x100b.Kv4AttnArgs), (x100b._NORM, x100b.NormQ8Args)])
+def test_packed_arguments_are_the_structs(pack, args):
+    values = [1 + 3 * i for i in range(len(args._fields_))]
+    raw = pack(*values)
+    assert len(raw) == C.sizeof(args)
+    assert [getattr(args.from_buffer_copy(raw), name) for name, _ in args._fields_] == values
