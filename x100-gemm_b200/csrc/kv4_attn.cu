@@ -7,6 +7,9 @@
 // sequence both fill the card, whatever the lengths (which only the device
 // knows).  Row tiles that a run cuts leave partial (o, m, l) sums in `work`;
 // merge_kernel joins them in run order, so results do not depend on timing.
+// Long contexts are bound by instructions, not bytes: 233 for 16 positions of 8 fp16 rows, most of them unpacking, issued at half
+// of the peak rate over the whole kernel (DRAM 0.35, tensor pipe 0.17): 16 tokens over 16384 positions each, 85 MB, in 34 us; one
+// fp32 token over 131071, 76 MB, in 32 us.  Short ones by a chain of round trips: one token over 4096 positions 10.6 us, merge included.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
