@@ -123,6 +123,8 @@ def test_steps_of_several_slots(world):
     with pytest.raises(x100b.X100Error) as e:
         m.kv_read(0, 0, 0, 1)
     assert e.value.code == x100b.X100_E_UNSUPPORTED
+    with pytest.raises(x100b.X100Error):
+        m.kv4_cache(c["n_layers"])
 
 
 @pytest.mark.parametrize("first,n", [(1, 4), (30, 3), (5, 20), (17, 40), (40, 333)])

@@ -173,3 +173,40 @@ def test_bad_starts_of_prompts_are_reported():
         out = torch.full_like(q, 9.0)
         cache.attend(q, out, table, ints(lens), q_start=ints(starts), max_q=max_q)
         assert status() == x100b.X100_E_ARG and torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+def test_single_tokens_of_large_groups(kind):
+    """300 query heads of one kv head are a prompt's rows, without q_start."""
+    rng = np.random.default_rng(31)
+    lens, D, G = [5, 400, 0, 129], 64, 300
+    pool = ref.random_pool(rng, 30, 32, 1, D)
+    table = page_table(rng, lens, 32, 30)
+    q = rng.normal(size=(4, G, D)).astype(np.float32 if kind == "f32" else np.float16)
+    got = cache_of(pool).attend(dev(q), None, ints(table), ints(lens)).cpu().numpy()
+    assert status() == 0
+    for b, n in enumerate(lens):
+        k, v = pool.values(table[b], n, False), pool.values(table[b], n, True)
+        want = ref.attention(q[b:b + 1], k, v, n - 1, D ** -0.5)
+        bound = ref.prompt_bound(q[b:b + 1], k, v, D ** -0.5, n, kind == "f16") + (2.0 ** -11 * np.abs(want).max() if kind == "f16" else 0)
+        assert np.abs(got[b:b + 1].astype(np.float64) - want).max() <= bound
+
+
+def test_another_stream():
+    """A call on a stream that is not the current one takes its outputs and scratch from the caller."""
+    rng = np.random.default_rng(32)
+    pool = ref.random_pool(rng, 10, 64, 2, 128)
+    cache, table, n = cache_of(pool), ints(page_table(rng, [600], 64, 10)), ints([600])
+    q, side = torch.randn(1, 8, 128, device="cuda"), torch.cuda.Stream()
+    want, pos, seq = cache.attend(q, None, table, n), ints([599]), ints([0])
+    kv = torch.randn(1, 2, 128, device="cuda")
+    for call in (lambda: cache.attend(q, None, table, n, stream=side), lambda: cache.attend(q, torch.empty_like(q), table, n, stream=side),
+                 lambda: cache.read(pos, table, seq=seq, stream=side), lambda: cache.append(kv, kv, pos, table, seq=seq, q=q, stream=side)):
+        with pytest.raises(x100b.X100Error) as e:
+            call()
+        assert e.value.code == x100b.X100_E_ARG
+    out, work = torch.empty_like(q), cache.attend_work(1, 8, 1)
+    side.wait_stream(torch.cuda.current_stream())
+    cache.attend(q, out, table, n, work=work, stream=side)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(out, want) and status() == 0

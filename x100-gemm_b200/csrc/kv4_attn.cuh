@@ -46,6 +46,7 @@ __device__ __forceinline__ int div_g(const AttnArgs &a, int n) { return a.G == 1
 // ---- the work list -------------------------------------------------------------
 // Sequence b: first row of q, tokens, positions; `cu` units of positions in every (kv head, row
 // tile) item, at least one so that rows without positions are written.
+constexpr int kMostPositions = 0x7fffff00;      // a tile past it still is an int
 struct Seq {
     int q0, nq, len, nrt, cu, row;       // row: of the page table
     uint32_t units;                      // of all its items, each cu + lead
@@ -57,7 +58,7 @@ __device__ __forceinline__ Seq load_seq(const AttnArgs &a, int b, int R, bool re
     s.len = (int)((unsigned)a.kv_len[b] + a.len_add);
     s.row = a.row_of ? a.row_of[b] : b;
     if (a.row_of && (unsigned)s.row >= (unsigned)a.n_rows) s.row = 0, s.len = -1;
-    const int cover = a.tab.stride > (0x7fffffff >> a.pool.page_shift) ? 0x7fffffff : a.tab.stride << a.pool.page_shift;
+    const int cover = min(a.tab.stride, kMostPositions >> a.pool.page_shift) << a.pool.page_shift;
     const bool bad_q = s.q0 < 0 || s.nq < 0 || s.nq > a.max_q || s.q0 > a.n_tokens - s.nq;
     if (bad_q) s.nq = 0;
     if (bad_q || s.len < 0 || s.len > cover) {

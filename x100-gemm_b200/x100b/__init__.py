@@ -348,7 +348,7 @@ class Model:
 
     def _open(self, fn, args, kv4):
         """Call fn(*args, cfg), or with a paged cache fn_kv4(*args, cfg, pool, table, entries)."""
-        self.h, args = None, (*args, C.byref(self.cfg))
+        self.h, self._kv4, args = None, None, (*args, C.byref(self.cfg))
         if kv4 is not None:
             torch, c, fn = _torch()[0], self.cfg, fn + "_kv4"
             n_pages, page_size, table = kv4
@@ -370,6 +370,8 @@ class Model:
     def kv4_cache(self, layer: int) -> "Kv4Cache":
         """The pool of a layer of a model made with kv4, on the model's own pages."""
         kv = self._kv4
+        if kv is None or not 0 <= layer < self.cfg.n_layers:
+            _refuse("Model.kv4_cache", "a layer of a model made with kv4 has one")
         return Kv4Cache(kv.n_pages, kv.page_size, kv.n_kv_heads, kv.head_dim, pages=self._pages[layer])
 
     def set_layer(self, layer, attn_norm, wq, wk, wv, q_norm, k_norm, wo, ffn_norm, router, gate, up, down):
@@ -549,6 +551,10 @@ _APPEND, _ATTN, _NORM = (struct.Struct(f).pack for f in ("@3i4P4q2PfPi3P2i", "@2
 _TORCH = None   # (torch, {dtype: Q_F32 / Q_F16}, float16, float32, int32, int8, uint8, current device, its current stream)
 
 
+# a tensor made here belongs to the current stream, and the allocator may hand its memory on while another one writes it
+_OWN_STREAM = "outputs and scratch have to be given together with a stream"
+
+
 def _torch():
     global _TORCH
     if _TORCH is None:
@@ -613,6 +619,8 @@ class Kv4Cache:
         if kind is None:
             _refuse(what, f"float32 or float16 is taken, not {dt}", X100_E_UNSUPPORTED)
         if q is not None and q_out is None:
+            if stream is not None:
+                _refuse(what, _OWN_STREAM)
             q_out = torch.empty(q.shape, dtype=dt, device=q.device)
         if not (k.get_device() == dev and v.get_device() == dev and v.dtype is dt and pos.dtype is i32_ and pos.get_device() == dev and pos.is_contiguous()
                 and table.dtype is i32_ and table.get_device() == dev and table.is_contiguous()
@@ -654,6 +662,8 @@ class Kv4Cache:
         if dev != self.device:
             self._elsewhere(what, dev)
         if k_out is None and v_out is None:
+            if stream is not None:
+                _refuse(what, _OWN_STREAM)
             k_out, v_out = (torch.zeros(n, self.n_kv_heads, self.head_dim, dtype=f16, device=pos.device) for _ in range(2))
         if not (pos.dtype is i32_ and pos.get_device() == dev and pos.is_contiguous() and table.dtype is i32_ and table.get_device() == dev and table.is_contiguous()
                 and (seq is None or (seq.dtype is i32_ and seq.get_device() == dev and seq.is_contiguous()))
@@ -687,6 +697,8 @@ class Kv4Cache:
         if q.dim() != 3 or q.shape[2] != D:
             _refuse(what, f"q has to be [tokens, heads, {D}]")
         rows, heads, _ = q.shape
+        if stream is not None and (out is None or work is None):
+            _refuse(what, _OWN_STREAM)
         if out is None:
             out = torch.empty(q.shape, dtype=dt, device=q.device)
         if work is None:
