@@ -249,6 +249,32 @@ def test_decode_lengths(kind, D, page, kv, heads):
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16"])
+@pytest.mark.parametrize("D,heads,kv,lens,q_lens", [(128, 8, 2, [300, 5, 0, 2100, 17, 640], [1, 2, 1, 3, 0, 1]), (64, 6, 2, [1500, 33], [1, 1]), (128, 7, 1, [4000], [1]),
+                                                    (128, 12, 1, [900, 1, 700], [1, 1, 2]), (64, 30, 1, [200, 0, 1300], [1, 1, 4])])
+def test_narrow_and_wide_tables(kind, D, heads, kv, lens, q_lens):
+    """The same sequences over a table that just holds them (clusters) and one that could hold far longer ones (runs and a merge)."""
+    rng = np.random.default_rng(heads + len(lens))
+    page = 32
+    n_pages = sum(-(-n // page) for n in lens) + 1
+    pool = ref.random_pool(rng, n_pages, page, kv, D)
+    table = page_table(rng, lens, page, n_pages)
+    wide = np.full((len(lens), 6000), -1, np.int32)
+    wide[:, :table.shape[1]] = table
+    for t in (table, wide):
+        check_attention(pool, t, lens, q_lens, heads, kind, extra=1)
+
+
+def test_sequences_around_a_cluster():
+    """Every count of items around those that fill the card with clusters of 16, 8 and 4 CTAs."""
+    rng = np.random.default_rng(40)
+    pool = ref.random_pool(rng, 24, 64, 1, 128)
+    for B in (1, 6, 7, 8, 9, 13, 15, 16, 17, 30, 31, 32, 33, 36, 60, 64, 70, 74, 80):
+        lens = [int(n) for n in rng.integers(0, 1500, B)]
+        table = rng.integers(0, 24, (B, 24)).astype(np.int32)
+        check_attention(pool, table, lens, [1] * B, 8, "f16", seed=B)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
 @pytest.mark.parametrize("D,heads,kv", [(128, 8, 2), (64, 6, 2), (128, 7, 1)])
 def test_several_tokens_each(kind, D, heads, kv):
     """Ragged token counts, none among them; a sequence shorter than its tokens has rows that see nothing."""

@@ -6,10 +6,11 @@
 // the grid takes the i-th run of equally many units, so ragged lengths and a single long
 // sequence both fill the card, whatever the lengths (which only the device
 // knows).  Row tiles that a run cuts leave partial (o, m, l) sums in `work`;
-// merge_kernel joins them in run order, so results do not depend on timing.
+// merge_kernel joins them in run order, so results do not depend on timing.  Few items of
+// few positions take clusters instead, which join without it.
 // Long contexts are bound by instructions, not bytes: 233 for 16 positions of 8 fp16 rows, most of them unpacking, issued at half
 // of the peak rate over the whole kernel (DRAM 0.35, tensor pipe 0.17): 16 tokens over 16384 positions each, 85 MB, in 34 us; one
-// fp32 token over 131071, 76 MB, in 32 us.  Short ones by a chain of round trips: one token over 4096 positions 10.6 us, merge included.
+// fp32 token over 131071, 76 MB, in 32 us.  Short ones by a chain of round trips: one token over 4096 positions 8.9 us.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -21,6 +22,12 @@ namespace kv4 {
 
 constexpr int kWarps = 8;
 constexpr int kLead = 3;                // units (of 128 positions) that starting an item costs: 2 and 5 measured alike, 0 5 % slower
+
+// Few items over a table that cannot hold long sequences go to clusters: of the most CTAs of which all items' fit the card at
+// once, if that makes at most cluster_units units a CTA.  One fp32 token over 1024, 4096, 8192 positions 9.5, 10.6,
+// 12.5 us by runs and 7.7, 8.1, 11.3 by clusters of 16, over 12288 (6 units each) 13.4 and 14.3; 16 fp16 tokens over 4096 each (8 units)
+// 17.0 and 14.2; 3 fp32 tokens over 4096 (24 rows, 2 units) 18.0 and 18.4.
+constexpr int cluster_units(int row_groups, bool fp32) { return row_groups > 1 ? 1 : fp32 ? 4 : 8; }
 
 // A run's share of the list, found by one whole warp: its units, and the
 // sequence holding the first with the units before it.
@@ -83,6 +90,17 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
+__device__ __forceinline__ int cluster_ctas() {
+    uint32_t n;
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
+    return (int)n;
+}
+// 16 bytes of another CTA's shared memory
+__device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
 // D = A B + C with C apart (registers or zeros)
 __device__ __forceinline__ void mma_init(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1, float c0, float c1) {
@@ -116,7 +134,9 @@ struct Cfg {
 // fp16 q: p rounded to fp16, whose error is no larger than the output's own rounding (16 x 16384 positions 36.5 -> 33.9 us).
 // Every warp walks its own positions with its own ring of bulk copies (two tiles a
 // stage), so the loop has no CTA barrier.
-template <typename T, int D, int NR>
+// CLUSTER: an item is a cluster's, its positions shared out among the CTAs and their sums joined through shared memory,
+// with no second kernel.
+template <typename T, int D, int NR, bool CLUSTER>
 __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(const AttnArgs a) {
     using L = Lay<D>;
     using C = Cfg<D, NR>;
@@ -138,34 +158,57 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
     fence_barrier_init();
     pdl_launch_dependents();
     pdl_wait();
-    if (warp == 0) {
-        const Share s = my_share(a, R);
-        if (lane == 0) s_share = s;
+    uint32_t u = 0, u1 = 1, before = 0;
+    int b, rank = 0, cl = 1, kvh = 0, rt = 0;
+    Seq sq;
+    if constexpr (CLUSTER) {
+        rank = cluster_ctarank(), cl = cluster_ctas();
+        const int id = blockIdx.x / cl, h = id / a.nrt_max;
+        rt = id - h * a.nrt_max, b = h / a.pool.nkv, kvh = h - b * a.pool.nkv;
+        sq = load_seq(a, b, R, rank + rt + kvh == 0);
+        if (rt >= sq.nrt) return;                  // the whole cluster
+        __syncthreads();
+    } else {
+        if (warp == 0) {
+            const Share s = my_share(a, R);
+            if (lane == 0) s_share = s;
+        }
+        if (threadIdx.x >= 32 && threadIdx.x < 34) a.meta[blockIdx.x * 2 + threadIdx.x - 32] = make_int4(-1, 0, 0, 0);
+        __syncthreads();
+        u1 = s_share.u1;
+        u = s_share.u0, before = s_share.before;
+        b = s_share.b;
+        if (u >= u1) return;
+        sq = load_seq(a, b, R, false);
     }
-    if (threadIdx.x >= 32 && threadIdx.x < 34) a.meta[blockIdx.x * 2 + threadIdx.x - 32] = make_int4(-1, 0, 0, 0);
-    __syncthreads();
-    const uint32_t u1 = s_share.u1;
-    uint32_t u = s_share.u0, before = s_share.before;
-    int b = s_share.b;
-    if (u >= u1) return;
     const Exponents expo;
-    Seq sq = load_seq(a, b, R, false);
     int nseg = 0;                              // segments done
     uint32_t st = 0, phase = 0;                // this warp's ring: next stage to read, and its parity
     uint64_t *bar = bars + warp * C::ST;
     uint8_t *wring = ring + warp * C::ST * 2 * L::BYTES;
     while (u < u1) {
-        while (u - before >= sq.units) {
-            before += sq.units;
-            sq = load_seq(a, ++b, R, false);
+        uint32_t iu = 0, item = 0;
+        int c0, c1;
+        if constexpr (CLUSTER) {
+            const int per = (sq.cu + cl - 1) / cl;
+            c0 = min(rank * per, sq.cu), c1 = min(c0 + per, sq.cu);
+            u = u1;
+        } else {
+            while (u - before >= sq.units) {
+                before += sq.units;
+                sq = load_seq(a, ++b, R, false);
+            }
+            // `lead` units stand for starting an item (queries, an empty ring, joining the warps): a run that ends among them
+            // has none of the item's positions
+            iu = sq.cu + a.lead;
+            const uint32_t off = u - before;
+            item = off / iu;
+            const uint32_t k0u = off - item * iu, k1u = min(iu, k0u + (u1 - u));
+            c0 = max(0, (int)k0u - a.lead), c1 = max(0, (int)k1u - a.lead);
+            u += k1u - k0u;
+            if (c1 == c0) continue;
+            kvh = sq.nrt == 1 ? (int)item : (int)(item / (uint32_t)sq.nrt), rt = row_tile((int)(item - (uint32_t)kvh * sq.nrt), sq.nrt);
         }
-        // `lead` units stand for starting an item (queries, an empty ring, joining the warps): a run that ends among them
-        // has none of the item's positions
-        const uint32_t iu = sq.cu + a.lead, off = u - before, item = off / iu, k0u = off - item * iu, k1u = min(iu, k0u + (u1 - u));
-        const int c0 = max(0, (int)k0u - a.lead), c1 = max(0, (int)k1u - a.lead);
-        u += k1u - k0u;
-        if (c1 == c0) continue;
-        const int kvh = sq.nrt == 1 ? (int)item : (int)(item / (uint32_t)sq.nrt), rt = row_tile((int)(item - (uint32_t)kvh * sq.nrt), sq.nrt);
         const int rows = min(R, sq.nq * a.G - rt * R);                   // live rows of the tile
         const int first = sq.len - sq.nq;                               // position of token 0
         const int nk = max(0, min(sq.len, first + div_g(a, rt * R + rows - 1) + 1));   // positions the last row sees
@@ -494,7 +537,8 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
                 }
             }
         __syncthreads();
-        if (abort_flag) return;                    // uniform: set before the barrier by a warp that gave up
+        if (!CLUSTER && abort_flag) return;        // uniform: set before the barrier by a warp that gave up
+        float4 *const xo = reinterpret_cast<float4 *>(smem + C::RED), *const xm = xo + NR * MT * 32;   // sums and (m, l) for the cluster
         const bool whole = c0 == 0 && c1 == sq.cu;
         const int slot = (int)blockIdx.x * 2 + (nseg ? 1 : 0);
 #pragma unroll
@@ -530,7 +574,10 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
                         if (M[i] != -INFINITY) Ls[i] += sl[e] * ex2(sm[e] - M[i]);
                     }
                 }
-                if (whole) {
+                if constexpr (CLUSTER) {
+                    xo[nr * MT * 32 + threadIdx.x] = x;
+                    if (k == 0 && g == 0) xm[(nr * 8 + 2 * t) / 2] = make_float4(M[0], Ls[0], M[1], Ls[1]);
+                } else if (whole) {
                     const int dim = g * (D / 8) + 2 * k;
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
@@ -561,6 +608,42 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
             __syncthreads();
         }
         ++nseg;
+        if constexpr (CLUSTER) {
+            // ---- join the CTAs: `cl` neighbouring lanes have a place of the fragments, each the sums of one CTA ----
+            cluster_sync_all();
+            constexpr int E = NR * MT * 32;
+            const int p = lane & (cl - 1), per = E / cl;
+            for (int j = threadIdx.x; j < E; j += kWarps * 32) {
+                const int e = rank * per + j / cl, nr = e / (MT * 32), k = e / 32 % MT, gg = e % 32 >> 2, tt = e & 3;
+                const float4 y = ld_cluster(mapa_shared(xo + e, p)), ml = ld_cluster(mapa_shared(xm + nr * 4 + tt, p));
+                const float v[2][3] = {{ml.y, y.x, y.z}, {ml.w, y.y, y.w}}, mx[2] = {ml.x, ml.z};   // l and two dims of rows 2 t, 2 t + 1
+                float out[2][3];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    float M = mx[i];
+                    for (int o = 1; o < cl; o <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+                    const float f = M == -INFINITY ? 0.f : ex2(mx[i] - M);
+#pragma unroll
+                    for (int n = 0; n < 3; ++n) {
+                        float z = v[i][n] * f;
+                        for (int o = 1; o < cl; o <<= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+                        out[i][n] = z;
+                    }
+                }
+                if (p < 2) {
+                    const int rr = nr * 8 + 2 * tt + p;
+                    if (rr < rows) {
+                        const float l_ = p ? out[1][0] : out[0][0], inv = l_ > 0.f ? 1.f / l_ : 0.f;
+                        const float y0 = (p ? out[1][1] : out[0][1]) * inv, y1 = (p ? out[1][2] : out[0][2]) * inv;
+                        const int r = rt * R + rr, tok = div_g(a, r);
+                        T *q = static_cast<T *>(a.out) + (long)(sq.q0 + tok) * a.os + (long)(kvh * a.G + r - tok * a.G) * D + gg * (D / 8) + 2 * k;
+                        if constexpr (HL) *reinterpret_cast<float2 *>(q) = make_float2(y0, y1);
+                        else *reinterpret_cast<__half2 *>(q) = __floats2half2_rn(y0, y1);
+                    }
+                }
+            }
+            cluster_sync_all();                    // the others have read this CTA's
+        }
     }
 }
 
@@ -654,24 +737,54 @@ __global__ void __launch_bounds__(kWarps * 32) merge_kernel(const AttnArgs a) {
     }
 }
 
+static int launch_cluster(void (*kernel)(const AttnArgs), int grid, int cl, int smem, cudaStream_t s, const AttnArgs &a) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid), cfg.blockDim = dim3(kWarps * 32), cfg.dynamicSmemBytes = smem, cfg.stream = s;
+    cudaLaunchAttribute at[2] = {};
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization, at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension, at[1].val.clusterDim = {(unsigned)cl, 1, 1};
+    cfg.attrs = at, cfg.numAttrs = 2;
+    return check_cuda(cudaLaunchKernelEx(&cfg, kernel, a), X100_E_LAUNCH);
+}
+
 template <typename T, int D, int NR>
 static int launch(DevCtx *c, AttnArgs &a, cudaStream_t s) {
     constexpr int R = 8 * NR;
     static bool attr[64];
+    static int fit[64][3];                 // clusters of 16, 8, 4 CTAs on the card at once
     if (!attr[c->device]) {
-        set_qkernel_attrs(attn_kernel<T, D, NR>, Cfg<D, NR>::SMEM);
+        set_qkernel_attrs(attn_kernel<T, D, NR, false>, Cfg<D, NR>::SMEM);
+        set_qkernel_attrs(attn_kernel<T, D, NR, true>, Cfg<D, NR>::SMEM);
+        cudaFuncSetAttribute(attn_kernel<T, D, NR, true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        for (int i = 0; i < 3; ++i) {
+            cudaLaunchAttribute at = {};
+            at.id = cudaLaunchAttributeClusterDimension, at.val.clusterDim = {16u >> i, 1, 1};
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(16 >> i), cfg.blockDim = dim3(kWarps * 32), cfg.dynamicSmemBytes = Cfg<D, NR>::SMEM, cfg.attrs = &at, cfg.numAttrs = 1;
+            if (cudaOccupancyMaxActiveClusters(&fit[c->device][i], attn_kernel<T, D, NR, true>, &cfg) != cudaSuccess) {
+                cudaGetLastError();
+                fit[c->device][i] = 0;
+            }
+        }
         attr[c->device] = true;
     }
     const long nrt = ((long)a.max_q * a.G + R - 1) / R, cover = std::min(0x7fffffffl, (long)a.tab.stride << a.pool.page_shift);
     const long items = (long)a.tab.n_seqs * a.pool.nkv * nrt;
     a.unit_shift = 7;
+    int cl = 16;
+    for (const int *f = fit[c->device]; cl > 2 && (items > *f || (cl > 4 && cover <= 64 * cl)); ++f) cl >>= 1;
+    if (cl > 2 && cover > 128 && cover <= 128l * cluster_units(NR, sizeof(T) == 4) * cl) {   // one unit needs no joining either way
+        a.lead = 0;
+        a.nrt_max = (int)nrt;
+        return launch_cluster(attn_kernel<T, D, NR, true>, (int)items * cl, cl, Cfg<D, NR>::SMEM, s, a);
+    }
     a.lead = kLead;
     while (items * ((cover >> a.unit_shift) + 1 + a.lead) > 0x7fffffffl) ++a.unit_shift;   // items <= 2^24: ends by 25
     const long most = std::min<long>(items, kMaxCtas) * ((cover >> a.unit_shift) + 1 + a.lead);
     const int grid = (int)std::min<long>(std::min(kMaxCtas, c->sm_count * (NR == 1 ? 2 : 1)), most);
     a.ml = reinterpret_cast<float2 *>(a.part + (size_t)kMaxCtas * 2 * R * D);
     a.meta = reinterpret_cast<int4 *>(a.ml + kMaxCtas * 2 * R);
-    int st = launch_pdl(attn_kernel<T, D, NR>, dim3(grid), dim3(kWarps * 32), Cfg<D, NR>::SMEM, s, a);
+    int st = launch_pdl(attn_kernel<T, D, NR, false>, dim3(grid), dim3(kWarps * 32), Cfg<D, NR>::SMEM, s, a);
     if (st || grid == 1 || cover <= 1l << a.unit_shift) return st;   // items of one unit are never cut
     if (items * 8 >= grid) return launch_pdl(merge_kernel<T, D, NR, 1>, dim3(grid - 1, NR), dim3(kWarps * 32), 0, s, a);
     return launch_pdl(merge_kernel<T, D, NR, 8>, dim3(grid - 1, NR * (D / 16)), dim3(kWarps * 32), 0, s, a);

@@ -25,6 +25,7 @@ struct AttnArgs {
     // kv_len[b] + len_add positions
     const int *row_of = nullptr;
     int n_rows = 0, len_add = 0;
+    int nrt_max;                         // row tiles of a sequence of max_q tokens (clusters)
     int n_tokens, max_q, nh, G;
     uint32_t g_mul;                      // ceil(2^32 / G): n / G = umulhi(n, g_mul) for n < 2^32 / G
     int unit_shift;                      // positions per unit, a power of two (128 unless the list would pass 2^31 units)
