@@ -71,20 +71,21 @@ struct Eight {
 // makes the codes the same on any machine that follows the formula.  Codes are taken before the factor
 // 1 / rms, which a block's scale carries: rounding of the sum of squares cannot move a value over a code's
 // border.
-// Bound by HBM when there are many tokens, by the launch when there are few.  1024 tokens of 32 + 2 x 4 heads of 128, fp32:
-// 39 MB in 11 us (3.5 TB/s; q is moved, too); 8 x 2047 of 14 + 2 x 2 heads of 64, fp16: 112 MB with the read-back in
-// 48 us.  A warp per head with 4 elements a lane took 195 us there, a loop per kind of head 4 us more than one over all.
+// Bound by instructions when there are many tokens (issue slots 0.75 busy for fp16, DRAM 0.27), by the launch when there are
+// few.  1024 tokens of 32 + 2 x 4 heads of 128, fp32: 38 MB in 10.6 us; 8 x 2047 of 14 + 2 x 2 heads of 64, fp16: 76 MB in
+// 33 us.  A warp per head with 4 elements a lane took 195 us there (with the read-back), a loop per kind of head 4 us more than
+// one over all, two groups on their way or k's and v's heads as one list the same.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(256, sizeof(T) == 4 ? 3 : 4) append_kernel(const AppendArgs a) {
     using L = Lay<D>;
     constexpr int LH = D / 8, HW = 32 / LH;
     const int lane = threadIdx.x & 31, in = lane % LH, hl = lane / LH;          // place in the head, head of the group
     const int nkv = a.pool.nkv, gq = (a.nh + HW - 1) / HW, gk = (nkv + HW - 1) / HW, groups = gq + 2 * gk;
-    const long item = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const uint32_t item = blockIdx.x * 8 + (threadIdx.x >> 5);   // slices are several only for few tokens
     pdl_launch_dependents();
     pdl_wait();
-    if (item >= (long)a.n_tokens * a.slices) return;
-    const int i = (int)(item / a.slices), slice = (int)item - i * a.slices;
+    if (item >= (uint32_t)a.n_tokens * a.slices) return;
+    const int i = a.slices == 1 ? item : item / a.slices, slice = (int)item - i * a.slices;
     const int pos = a.pos[i];
     if (pos < 0) return;                                  // padding
     const int seq = a.seq ? a.seq[i] : i;
@@ -116,6 +117,11 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
     }
     uint8_t *tile = nullptr;                              // of kv head 0
     if (g + (groups - 1 - g) / a.slices * a.slices >= gq) tile = tile_of(a.pool, a.tab, seq, pos, 0);   // the slice has k or v
+    float wq[sizeof(T) == 4 ? 8 : 1];                      // q has most of the groups; fp16's registers are better spent on warps
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) wq[e] = a.qn && g < gq ? __ldg(a.qn + in * 8 + e) : 1.f;
+    }
     bool bad = far;
     if (far) g = groups;
     for (; g < groups; g += a.slices) {
@@ -131,9 +137,9 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
             for (int e = 0; e < 8; ++e) ss = fmaf(t[e], t[e], ss);
 #pragma unroll
             for (int o = LH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            s = 1.f / sqrtf(ss * (1.f / D) + a.eps);
+            s = __frsqrt_rn(ss * (1.f / D) + a.eps);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) t[e] = __fmul_rn(t[e], __ldg(w + in * 8 + e));
+            for (int e = 0; e < 8; ++e) t[e] = __fmul_rn(t[e], sizeof(T) == 4 && is_q ? wq[sizeof(T) == 4 ? e : 0] : __ldg(w + in * 8 + e));
         }
         if (turn && (is_q || is_k)) {
 #pragma unroll
@@ -203,19 +209,20 @@ struct ReadArgs {
     int *status;
 };
 
-// The inverse (5 us for the 1024 tokens, 14 us for the 8 x 2047): a lane has 8 dims of a head (a word of codes, 16 bytes out), d * (code - 8) in fp16 (exact); warps and
-// slices as in append_kernel.
+// The inverse: a lane has 8 dims of a head (a word of codes, 16 bytes out), d * (code - 8) in fp16 (exact); warps and
+// slices as in append_kernel, over k's and v's heads as one list.  Bound by the chain position -> page -> codes, so
+// 32 registers: 3.0 us for the 1024 tokens and 10.5 us for the 8 x 2047 (5 and 15 with lists apart and 48 registers).
 template <int D>
-__global__ void __launch_bounds__(256) read_kernel(const ReadArgs a) {
+__global__ void __launch_bounds__(256, 8) read_kernel(const ReadArgs a) {
     using L = Lay<D>;
     constexpr int LH = D / 8, HW = 32 / LH;
     const int lane = threadIdx.x & 31, in = lane % LH, hl = lane / LH, nkv = a.pool.nkv;
-    const int gk = (nkv + HW - 1) / HW, groups = gk * ((a.k ? 1 : 0) + (a.v ? 1 : 0));
-    const long item = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int nk = a.k ? nkv : 0, heads = nk + (a.v ? nkv : 0), groups = (heads + HW - 1) / HW;
+    const uint32_t item = blockIdx.x * 8 + (threadIdx.x >> 5);
     pdl_launch_dependents();
     pdl_wait();
-    if (item >= (long)a.n_tokens * a.slices) return;
-    const int i = (int)(item / a.slices), slice = (int)(item % a.slices);
+    if (item >= (uint32_t)a.n_tokens * a.slices) return;
+    const int i = a.slices == 1 ? item : item / a.slices, slice = (int)item - i * a.slices;
     const int pos = a.pos[i];
     if (pos < 0) return;
     const uint8_t *tile = tile_of(a.pool, a.tab, a.seq ? a.seq[i] : i, pos, 0);
@@ -226,17 +233,15 @@ __global__ void __launch_bounds__(256) read_kernel(const ReadArgs a) {
     const int sp = pos & 15, b = in / 4;
 #pragma unroll 2
     for (int g = slice; g < groups; g += a.slices) {
-        const bool is_k = a.k && g < gk;
-        const int h = (a.k && !is_k ? g - gk : g) * HW + hl;
-        if (h >= nkv) continue;
+        const int at = g * HW + hl, h = at < nk ? at : at - nk;
+        if (at >= heads) break;
         const uint8_t *th = tile + h * a.pool.page_bytes;
-        const uint8_t *at = is_k ? th + L::k_word(sp, b, in & 3) : th + L::v_piece(sp, in * 8 / (D / 8)) + in * 8 % (D / 8) / 2;
-        const uint32_t codes = *reinterpret_cast<const uint32_t *>(at);
-        const float d = __half2float(*reinterpret_cast<const __half *>(th + (is_k ? L::k_scale(sp, b) : L::v_scale(sp, b))));
+        const uint32_t codes = *reinterpret_cast<const uint32_t *>(at < nk ? th + L::k_word(sp, b, in & 3) : th + L::v_piece(sp, in * 8 / (D / 8)) + in * 8 % (D / 8) / 2);
+        const float d = __half2float(*reinterpret_cast<const __half *>(th + (at < nk ? L::k_scale(sp, b) : L::v_scale(sp, b))));
         float x[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = d * ((int)(codes >> (4 * e) & 15) - 8);
-        Eight<__half>::store((is_k ? a.k : a.v) + ((long)i * nkv + h) * D + in * 8, x);
+        Eight<__half>::store((at < nk ? a.k : a.v) + ((long)i * nkv + h) * D + in * 8, x);
     }
 }
 
@@ -323,7 +328,7 @@ int x100q_kv4_read_dev(const x100q_kv4 *kv, const int *pos, const int *seq, int 
         return refuse(X100_E_ARG);
     DevCtx *c = ctx();
     if (!c) return get_error();
-    const int hw = 256 / kv->head_dim, groups = (kv->n_kv_heads + hw - 1) / hw * ((k_out ? 1 : 0) + (v_out ? 1 : 0));
+    const int hw = 256 / kv->head_dim, groups = (kv->n_kv_heads * ((k_out ? 1 : 0) + (v_out ? 1 : 0)) + hw - 1) / hw;
     ReadArgs p = {make_pool(kv), {page_table, table_stride, n_seqs}, pos, seq, n_tokens, slices_for(c, n_tokens, groups), static_cast<__half *>(k_out),
                   static_cast<__half *>(v_out), c->d_status};
     const long ctas = ((long)n_tokens * p.slices + 7) / 8;
