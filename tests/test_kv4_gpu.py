@@ -452,3 +452,14 @@ def test_prompt_then_decode_steps(kind):
     kk, vv = (pool.values(table[0], total, i) for i in (False, True))
     want = ref.attention(qr, kk, vv, 0, D ** -0.5)
     assert np.abs(got.astype(np.float64) - want).max() <= ref.attention_bound(qr, kk, vv, D ** -0.5, total, kind == "f16")
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+@pytest.mark.parametrize("D,G", [(128, 5), (64, 7)])
+def test_row_tiles(kind, D, G):
+    """Every number of tokens from one to where the prompt kernel begins: one to four groups of eight rows in one tile and in several."""
+    rng = np.random.default_rng(G)
+    pool = ref.random_pool(rng, 14, 32, 1, D)
+    for T in [*range(1, 18), 25, 33, 255 // G]:
+        lens = [T, 300 + T, T // 2]
+        check_attention(pool, rng.integers(0, 14, (3, 20)).astype(np.int32), lens, [T, T, T], G, kind, seed=T)
