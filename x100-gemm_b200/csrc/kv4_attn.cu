@@ -26,7 +26,7 @@ constexpr int kLead = 3;                // units (of 128 positions) that startin
 // Few items over a table that cannot hold long sequences go to clusters: of the most CTAs of which all items' fit the card at
 // once, if that makes at most cluster_units units a CTA.  One fp32 token over 1024, 4096, 8192 positions 9.5, 10.6,
 // 12.5 us by runs and 7.7, 8.1, 11.3 by clusters of 16, over 12288 (6 units each) 13.4 and 14.3; 16 fp16 tokens over 4096 each (8 units)
-// 17.0 and 14.2; 3 fp32 tokens over 4096 (24 rows, 2 units) 18.0 and 18.4.
+// 17.0 and 14.2; with several row groups 2 units a CTA took as long either way.
 constexpr int cluster_units(int row_groups, bool fp32) { return row_groups > 1 ? 1 : fp32 ? 4 : 8; }
 
 // A run's share of the list, found by one whole warp: its units, and the
