@@ -210,3 +210,20 @@ def test_another_stream():
     cache.attend(q, out, table, n, work=work, stream=side)
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(out, want) and status() == 0
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+@pytest.mark.parametrize("q_lens,width", [([1, 1, 1], None), ([1, 1, 1], 5000), ([40, 1, 500], None)])
+def test_in_place(kind, q_lens, width):
+    """out is q: clusters, runs with cut items, prompts."""
+    rng = np.random.default_rng(len(q_lens))
+    lens = [3000, 50, 900]
+    pool = ref.random_pool(rng, 70, 64, 1, 128)
+    table = page_table(rng, lens, 64, 70)
+    if width:
+        table = np.concatenate([table, np.full((3, width), -1, np.int32)], 1)
+    cache, table, n = cache_of(pool), ints(table), ints(lens)
+    starts = ints(np.concatenate([[0], np.cumsum(q_lens)]))
+    q = torch.randn(sum(q_lens), 8, 128, device="cuda").to(DT[kind])
+    want = cache.attend(q, None, table, n, q_start=starts, max_q=max(q_lens))
+    assert torch.equal(cache.attend(q, q, table, n, q_start=starts, max_q=max(q_lens)), want) and status() == 0
