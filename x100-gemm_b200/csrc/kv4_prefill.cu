@@ -358,13 +358,16 @@ __global__ void __launch_bounds__(Roles<T>::THREADS, 1) prefill_kernel(const Att
                 ok = wait(&bars.s_full[X][step & 1], step >> 1 & 1);
                 if (!ok) break;
                 tc_fence_after();
-                const bool mask = __any_sync(0xffffffffu, p0 + kKeys > lim) || hole;
-                uint32_t gone = 0;               // 16-position tiles without a page
-                if (hole)
-                    for (int i = 0; i < 8 && p0 + 16 * i < len; ++i)
-                        if ((unsigned)__ldg(trow + ((p0 + 16 * i) >> a.pool.page_shift)) >= (unsigned)a.pool.n_pages) gone |= 1u << i;
-                // scores 32 i .. of the row.  fp16 q keeps all of them; fp32 q, whose registers the sums need, loads them twice
+                // fp16 q keeps all scores of the row; fp32 q, whose registers the sums need, loads them twice, 32 at a time
+                float s[HL ? 32 : 128], mx[4];
                 auto load = [&](float *v, int i) { tmem_ld32(sx + 32 * i, *reinterpret_cast<uint32_t(*)[32]>(v)); };
+                bool mask = false;               // fp32 q: this tile has masked positions
+                uint32_t gone = 0;               // 16-position tiles without a page
+                auto find_gone = [&]() {
+                    if (hole)
+                        for (int i = 0; i < 8 && p0 + 16 * i < len; ++i)
+                            if ((unsigned)__ldg(trow + ((p0 + 16 * i) >> a.pool.page_shift)) >= (unsigned)a.pool.n_pages) gone |= 1u << i;
+                };
                 auto cover = [&](float *v, int i) {
                     const int cut = lim - p0 - 32 * i;
 #pragma unroll
@@ -376,19 +379,43 @@ __global__ void __launch_bounds__(Roles<T>::THREADS, 1) prefill_kernel(const Att
                             if (gone >> (2 * i + k / 16) & 1) v[k] = -INFINITY;
                     }
                 };
-                float s[HL ? 32 : 128], mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                if constexpr (HL) {
+                    mask = __any_sync(0xffffffffu, p0 + kKeys > lim) || hole;
+                    find_gone();
+                    mx[0] = mx[1] = mx[2] = mx[3] = -INFINITY;
 #pragma unroll
-                for (int h = 0; h < 128; h += HL ? 32 : 128) {
+                    for (int h = 0; h < 4; ++h) {
+                        load(s, h);
+                        tmem_wait_ld();
+                        if (mask) cover(s, h);
 #pragma unroll
-                    for (int i = 0; i < (HL ? 1 : 4); ++i) load(s + 32 * i, h / 32 + i);
+                        for (int i = 0; i < 32; i += 8)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) mx[k] = fmaxf(fmaxf(mx[k], s[i + k]), s[i + 4 + k]);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) load(s + 32 * i, i);
                     tmem_wait_ld();
-                    if (mask)
+                    if (__any_sync(0xffffffffu, p0 + kKeys > lim) || hole) {
+                        const int cut = lim - p0;
 #pragma unroll
-                        for (int i = 0; i < (HL ? 1 : 4); ++i) cover(s + 32 * i, h / 32 + i);
+                        for (int i = 0; i < 128; ++i)
+                            if (i >= cut) s[i] = -INFINITY;
+                        find_gone();
+                        if (gone)
 #pragma unroll
-                    for (int i = 0; i < (HL ? 32 : 128); i += 8)
+                            for (int i = 0; i < 128; ++i)
+                                if (gone >> (i / 16) & 1) s[i] = -INFINITY;
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) mx[k] = s[k];
+#pragma unroll
+                    for (int i = 4; i < 124; i += 8)
 #pragma unroll
                         for (int k = 0; k < 4; ++k) mx[k] = fmaxf(fmaxf(mx[k], s[i + k]), s[i + 4 + k]);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], s[124 + k]);
                 }
                 const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.sl;
                 if (__any_sync(0xffffffffu, top > m + 8.f)) {
