@@ -359,23 +359,29 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
                     const float d0 = __half2float(kd[0][blk]), d1 = __half2float(kd[1][blk]);
 #pragma unroll
                     for (int nr = 0; nr < NR; ++nr) {
-                        float acc[4], i0 = 0.f, i1 = 0.f;
+                        float acc[4];
+                        [[maybe_unused]] float i0 = 0.f, i1 = 0.f;
                         if constexpr (HL) {
                         } else if constexpr (NR == 1) i0 = qi[blk][0], i1 = qi[blk][1];
                         else {
                             const float2 v = *reinterpret_cast<const float2 *>(qb + (nr * NB + blk) * 8 + 2 * t);
                             i0 = v.x, i1 = v.y;
                         }
+                        const uint4 *qp = qf + (nr * (D / 16) + 2 * blk) * 32 + lane;
+                        uint4 q[2];
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            const uint4 *qp = qf + (nr * (D / 16) + 2 * blk + h) * 32 + lane;
-                            uint4 q;
-                            if constexpr (HL) q = *qp;
-                            else *reinterpret_cast<uint2 *>(&q) = *reinterpret_cast<const uint2 *>(qp);
-                            if (h == 0) mma_init(acc, f[0][0], f[1][0], f[0][1], f[1][1], q.x, q.y, i0, i1);
-                            else mma(acc, f[0][2], f[1][2], f[0][3], f[1][3], q.x, q.y);
-                            if (HL) mma(acc, f[0][2 * h], f[1][2 * h], f[0][2 * h + 1], f[1][2 * h + 1], q.z, q.w);
+                            if constexpr (HL) q[h] = qp[h * 32];
+                            else *reinterpret_cast<uint2 *>(q + h) = *reinterpret_cast<const uint2 *>(qp + h * 32);
                         }
+                        if constexpr (HL) {             // lo first: what is added to is small then, and with it what is cut off
+                            mma_init(acc, f[0][0], f[1][0], f[0][1], f[1][1], q[0].z, q[0].w, 0.f, 0.f);
+                            mma(acc, f[0][2], f[1][2], f[0][3], f[1][3], q[1].z, q[1].w);
+                            mma(acc, f[0][0], f[1][0], f[0][1], f[1][1], q[0].x, q[0].y);
+                        } else {
+                            mma_init(acc, f[0][0], f[1][0], f[0][1], f[1][1], q[0].x, q[0].y, i0, i1);
+                        }
+                        mma(acc, f[0][2], f[1][2], f[0][3], f[1][3], q[1].x, q[1].y);
                         float(&x)[4] = sc[tt][nr];
                         if (blk == 0) x[0] = acc[0] * d0, x[1] = acc[1] * d0, x[2] = acc[2] * d1, x[3] = acc[3] * d1;
                         else {
@@ -488,8 +494,8 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
                                 float(&sum)[4] = o[nr][4 * w + 2 * hf + e];
                                 if constexpr (HL) {
                                     float x4[4];
-                                    mma_init(x4, a0, a1, a2, a3, ph[nr][0], ph[nr][1], 0.f, 0.f);
-                                    mma(x4, a0, a1, a2, a3, pl[nr][0], pl[nr][1]);
+                                    mma_init(x4, a0, a1, a2, a3, pl[nr][0], pl[nr][1], 0.f, 0.f);
+                                    mma(x4, a0, a1, a2, a3, ph[nr][0], ph[nr][1]);
 #pragma unroll
                                     for (int i = 0; i < 4; ++i) sum[i] += x4[i];
                                 } else {

@@ -14,7 +14,7 @@
 // fp16 q: the steps X are two row tiles over the same key tile (256 rows per item), so that
 // a key tile is unpacked once for both; O stays in TMEM.  fp32 q: q and P are carried as hi + lo halves, two
 // products each, the steps X are every other key tile of one row tile, and O of a step is added to fp32
-// registers: summed in TMEM it was off by 3e-6 at 2600 positions and more at each further one, and is now by 3e-7,
+// registers: summed in TMEM it was off by 3e-6 at 2600 positions and more at each further one, and is now by 5e-7,
 // for 134 us instead of 108 (1024 tokens over 2600 positions, 32 heads).
 // Either way one step's softmax runs beside the other's products.
 //
@@ -695,11 +695,11 @@ __global__ void __launch_bounds__(Roles<T>::THREADS, 1) prefill_kernel(const Att
                     tc_fence_after();
                     const uint64_t qd = descQ + (HL ? 0 : X * (P::QT >> 4)), kd = descK + st * (P::KT >> 4);
 #pragma unroll
-                    for (int p = 0; p < (HL ? 2 : 1); ++p)
+                    for (int p = HL ? 1 : 0; p >= 0; --p)    // lo first: what is added to is small then, and with it what is cut off
 #pragma unroll
                         for (int k = 0; k < KS; ++k) {
                             const uint32_t off = ((k >> 2) * P::SUB + (k & 3) * 32) >> 4;
-                            umma_ss(tS + 128 * X, qd + p * (P::QT >> 4) + off, kd + off, idS, (p | k) ? 1u : 0u, lead);
+                            umma_ss(tS + 128 * X, qd + p * (P::QT >> 4) + off, kd + off, idS, (p < (HL ? 1 : 0) || k) ? 1u : 0u, lead);
                         }
                     umma_commit_lead(&bars.s_full[X][sdone >> (16 * X) & 1], lead);
                     sdone += 1u << (16 * X);
@@ -719,10 +719,10 @@ __global__ void __launch_bounds__(Roles<T>::THREADS, 1) prefill_kernel(const Att
                     const uint64_t vd = descV + st * (P::KT >> 4);
                     const uint32_t more = !HL && s >= 2 ? 1u : 0u;      // O of X holds sums of the segment
 #pragma unroll
-                    for (int p = 0; p < (HL ? 2 : 1); ++p)
+                    for (int p = HL ? 1 : 0; p >= 0; --p)
 #pragma unroll
                         for (int k = 0; k < VS; ++k)
-                            umma_ts(tO + 128 * X, tS + 128 * X + (HL ? 16 * k + 8 * p : 8 * k), vd + k * (2048 >> 4), idO, (p | k) ? 1u : more, lead);
+                            umma_ts(tO + 128 * X, tS + 128 * X + (HL ? 16 * k + 8 * p : 8 * k), vd + k * (2048 >> 4), idO, (p < (HL ? 1 : 0) || k) ? 1u : more, lead);
                     umma_commit_lead(&bars.o_done[X][done & 1], lead);
                     pdone += 1u << (16 * X);
                     if (HL) umma_commit_lead(&bars.v_empty[st], lead);
