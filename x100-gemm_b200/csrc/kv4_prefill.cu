@@ -676,7 +676,7 @@ __global__ void __launch_bounds__(Roles<T>::THREADS, 1) prefill_kernel(const Att
             // matrix descriptors; tiles and slices of them differ in the address field (16-byte steps) alone
             const uint64_t descQ = smem_desc_sw128(smem_u32(sm), 16, 1024), descK = smem_desc_sw128(smem_u32(sm + P::K0), 16, 1024);
             const uint64_t descV = smem_desc_sw128(smem_u32(sm + P::V0), P::SUB, 1024);
-            uint32_t tile = 0, sdone = 0, pdone = 0;   // key tiles; scores and sums issued so far, X = 1's in the high half
+            uint32_t tile = 0, sdone = 0, pdone = 0;   // key tiles; bit X: scores and sums issued of step X so far, odd or even
             for (uint32_t nseg = 0; ok; ++nseg) {
                 ok = segment(nseg);
                 if (!ok) break;
@@ -701,8 +701,8 @@ __global__ void __launch_bounds__(Roles<T>::THREADS, 1) prefill_kernel(const Att
                             const uint32_t off = ((k >> 2) * P::SUB + (k & 3) * 32) >> 4;
                             umma_ss(tS + 128 * X, qd + p * (P::QT >> 4) + off, kd + off, idS, (p < (HL ? 1 : 0) || k) ? 1u : 0u, lead);
                         }
-                    umma_commit_lead(&bars.s_full[X][sdone >> (16 * X) & 1], lead);
-                    sdone += 1u << (16 * X);
+                    umma_commit_lead(&bars.s_full[X][sdone >> X & 1], lead);
+                    sdone ^= 1u << X;
                     if (HL) umma_commit_lead(&bars.k_empty[st], lead);
                     if (s == S - 1) umma_commit_lead(&bars.q_empty, lead);
                     return true;
@@ -710,10 +710,10 @@ __global__ void __launch_bounds__(Roles<T>::THREADS, 1) prefill_kernel(const Att
                 for (int s = 0; s < 2 && s < S && ok; ++s) ok = scores(s);
                 for (int s = 0; s < S && ok; ++s) {
                     const int X = s & 1;
-                    const uint32_t tl = tile + (HL ? s : s >> 1), st = tl & 1, done = pdone >> (16 * X);
-                    ok = wait(&bars.p_ready[X], done & 1);
+                    const uint32_t tl = tile + (HL ? s : s >> 1), st = tl & 1, odd = pdone >> X & 1;
+                    ok = wait(&bars.p_ready[X], odd);
                     if (ok && (HL || X == 0)) ok = wait(&bars.v_full[st], tl >> 1 & 1);
-                    if (HL && ok) ok = wait(&bars.o_free[X], (done & 1) ^ 1);
+                    if (HL && ok) ok = wait(&bars.o_free[X], odd ^ 1);
                     if (!ok) break;
                     tc_fence_after();
                     const uint64_t vd = descV + st * (P::KT >> 4);
@@ -723,8 +723,8 @@ __global__ void __launch_bounds__(Roles<T>::THREADS, 1) prefill_kernel(const Att
 #pragma unroll
                         for (int k = 0; k < VS; ++k)
                             umma_ts(tO + 128 * X, tS + 128 * X + (HL ? 16 * k + 8 * p : 8 * k), vd + k * (2048 >> 4), idO, (p < (HL ? 1 : 0) || k) ? 1u : more, lead);
-                    umma_commit_lead(&bars.o_done[X][done & 1], lead);
-                    pdone += 1u << (16 * X);
+                    umma_commit_lead(&bars.o_done[X][odd], lead);
+                    pdone ^= 1u << X;
                     if (HL) umma_commit_lead(&bars.v_empty[st], lead);
                     if (s + 2 < S) ok = scores(s + 2);
                 }
