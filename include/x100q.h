@@ -198,7 +198,8 @@ int x100q_rope_table_dev(float *rope, int n_pos, int head_dim, float base, void 
  * (NULL: one token each, row b); they are its last positions, and each attends to
  * all positions up to its own.  A row that sees no position (kv_len[b]
  * shorter than the sequence's tokens) is zero.  Rows past q_start[n_seqs] stay as
- * they were; out may be q itself.  max_q bounds the tokens of any one sequence, and q_start must
+ * they were; out may be q itself.  What q_start, kv_len and the page table hold has to
+ * stay until the call has run.  max_q bounds the tokens of any one sequence, and q_start must
  * not decrease or pass n_tokens; a sequence that breaks this is left out, and the
  * next synchronising call reports X100_E_ARG.
  * X100Q_F32: q (|q| <= 65504, as two fp16 halves) and the probabilities are used

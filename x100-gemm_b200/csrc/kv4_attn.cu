@@ -53,7 +53,7 @@ __device__ __forceinline__ Share my_share(const AttnArgs &a, int R) {
     if (per * blockIdx.x >= U) return s;     // the longest run is as long as with more, shorter ones; fewer items are cut
     s.u0 = per * blockIdx.x, s.u1 = min(U, s.u0 + per);
     uint32_t base = 0;
-    for (int b0 = 0;; b0 += 32) {        // ends: u0 < U
+    for (int b0 = 0; b0 < a.tab.n_seqs; b0 += 32) {
         if (a.tab.n_seqs > 32) {         // else the one chunk's sums are still here
             mine = b0 + lane < a.tab.n_seqs ? load_seq(a, b0 + lane, R, false).units : 0;
             incl = mine;
@@ -72,6 +72,8 @@ __device__ __forceinline__ Share my_share(const AttnArgs &a, int R) {
         }
         base += __shfl_sync(0xffffffffu, incl, 31);
     }
+    s.u0 = s.u1 = 0;                     // u0 < U: only if the lengths changed since they were added up
+    return s;
 }
 // Row tile of an item index: from both ends in turn, so that a run of neighbouring
 // items of a causal prompt holds early (short) and late (long) ones alike.
@@ -166,7 +168,6 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
         const int id = blockIdx.x / cl, h = id / a.nrt_max;
         rt = id - h * a.nrt_max, b = h / a.pool.nkv, kvh = h - b * a.pool.nkv;
         sq = load_seq(a, b, R, rank + rt + kvh == 0);
-        if (rt >= sq.nrt) return;                  // the whole cluster
         __syncthreads();
     } else {
         if (warp == 0) {
@@ -190,13 +191,14 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
         uint32_t iu = 0, item = 0;
         int c0, c1;
         if constexpr (CLUSTER) {
-            const int per = (sq.cu + cl - 1) / cl;
+            const int per = rt < sq.nrt ? (sq.cu + cl - 1) / cl : 0;   // a tile that the sequence does not have: no positions, no rows
             c0 = min(rank * per, sq.cu), c1 = min(c0 + per, sq.cu);
             u = u1;
         } else {
             while (u - before >= sq.units) {
                 before += sq.units;
-                sq = load_seq(a, ++b, R, false);
+                if (++b >= a.tab.n_seqs) return;
+                sq = load_seq(a, b, R, false);
             }
             // `lead` units stand for starting an item (queries, an empty ring, joining the warps): a run that ends among them
             // has none of the item's positions
@@ -674,9 +676,10 @@ __global__ void __launch_bounds__(kWarps * 32) merge_kernel(const AttnArgs a) {
         if (p0.x != here.x || (p0.w & kInside)) return;      // an earlier cut joins this item
         slot0 = 2 * c - 2;
     }
-    const int b = here.y, kvh = here.z & 0xffff, rt = here.w & (kInside - 1), np = (here.z >> 16) - c + 2;
-    const int q0 = a.q_start ? a.q_start[b] : b;
-    const int rows = min(R, (a.q_start ? a.q_start[b + 1] - q0 : 1) * a.G - rt * R);
+    const int b = here.y, kvh = here.z & 0xffff, rt = here.w & (kInside - 1), np = min(here.z >> 16, (int)gridDim.x) - c + 2;
+    int q0, nq;
+    load_rows(a, b, q0, nq);
+    const int rows = min(R, nq * a.G - rt * R);
     // each warp its parts, four loads under way at a time, with a running max of its own
     float M[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);

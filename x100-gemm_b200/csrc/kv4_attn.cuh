@@ -52,16 +52,23 @@ struct Seq {
     int q0, nq, len, nrt, cu, row;       // row: of the page table
     uint32_t units;                      // of all its items, each cu + lead
 };
+// Rows q0 .. q0 + nq - 1 of sequence b; false (and none) where they are not the call's.
+__device__ __forceinline__ bool load_rows(const AttnArgs &a, int b, int &q0, int &nq) {
+    q0 = a.q_start ? a.q_start[b] : b;
+    nq = a.q_start ? a.q_start[b + 1] - q0 : 1;
+    const bool bad = q0 < 0 || nq < 0 || nq > a.max_q || q0 > a.n_tokens - nq;
+    if (bad) nq = 0;
+    return !bad;
+}
+// The arrays are read more than once in a call.  Should they change meanwhile (a caller's mistake) results mean nothing, but
+// the walks end with the list, and what is read and written stays in the call's tensors.
 __device__ __forceinline__ Seq load_seq(const AttnArgs &a, int b, int R, bool report) {
     Seq s;
-    s.q0 = a.q_start ? a.q_start[b] : b;
-    s.nq = a.q_start ? a.q_start[b + 1] - s.q0 : 1;
+    const bool bad_q = !load_rows(a, b, s.q0, s.nq);
     s.len = (int)((unsigned)a.kv_len[b] + a.len_add);
     s.row = a.row_of ? a.row_of[b] : b;
     if (a.row_of && (unsigned)s.row >= (unsigned)a.n_rows) s.row = 0, s.len = -1;
     const int cover = min(a.tab.stride, kMostPositions >> a.pool.page_shift) << a.pool.page_shift;
-    const bool bad_q = s.q0 < 0 || s.nq < 0 || s.nq > a.max_q || s.q0 > a.n_tokens - s.nq;
-    if (bad_q) s.nq = 0;
     if (bad_q || s.len < 0 || s.len > cover) {
         if (report) atomicCAS(a.status, 0, X100_E_ARG);
         s.len = s.len < 0 ? 0 : min(s.len, cover);

@@ -142,7 +142,7 @@ __device__ __forceinline__ Start my_start(const AttnArgs &a) {
     if (per * blockIdx.x >= U) return r;
     r.u0 = per * blockIdx.x, r.u1 = min(U, r.u0 + per);
     uint32_t base = 0, hu = 0;
-    for (int b0 = 0;; b0 += 32) {          // ends: u0 < U
+    for (int b0 = 0; b0 < a.tab.n_seqs; b0 += 32) {
         Seq mine;
         mine.nrt = 0;
         if (b0 + lane < a.tab.n_seqs) mine = load_seq(a, b0 + lane, RT, false);
@@ -175,6 +175,8 @@ __device__ __forceinline__ Start my_start(const AttnArgs &a) {
             base += __shfl_sync(0xffffffffu, incl, 31);
         }
     }
+    r.u0 = r.u1 = 0;                       // u0 < U: only if the lengths changed since they were added up
+    return r;
 }
 // A segment: key tiles c0 .. c0 + n - 1 of an item (all cu of them, or a part).
 struct Seg {
@@ -788,15 +790,17 @@ __global__ void __launch_bounds__(Roles<T>::THREADS, 1) prefill_kernel(const Att
                     g.cu = cu, g.b = b, g.kvh = kvh, g.rt = rt, g.q0 = sq.q0, g.nq = sq.nq, g.len = sq.len, g.row = sq.row, g.item = item;
                     item += cu + kLead;
                     u = item;
-                    if (u < at.u1 && ++rt == sq.nrt) {
+                    if (u < at.u1 && ++rt >= sq.nrt) {
                         rt = 0;
                         if (++kvh == a.pool.nkv) {
                             kvh = 0;
-                            do sq = load_seq(a, ++b, RT, false);
-                            while (!sq.nrt);
+                            do {
+                                if (++b < a.tab.n_seqs) sq = load_seq(a, b, RT, false);
+                                else u = at.u1;
+                            } while (!sq.nrt && u < at.u1);
                         }
                     }
-                    if (g.n == 0) continue;
+                    if (g.n <= 0) continue;
                 }
                 ok = wait(&bars.seg_empty[nseg % kSegs], (nseg / kSegs & 1) ^ 1);
                 if (!ok) break;
@@ -829,7 +833,8 @@ __global__ void __launch_bounds__(kPfRows) prefill_merge_kernel(const AttnArgs a
         slot0 = 2 * c - 2;
     }
     const int b = here.y, rt = here.w & (kInside - 1), r = rt * RT + row;
-    const int q0 = a.q_start ? a.q_start[b] : b, nq = a.q_start ? a.q_start[b + 1] - q0 : 1;
+    int q0, nq;
+    load_rows(a, b, q0, nq);
     if (row >= RT || r >= nq * a.G) return;
     float m = -INFINITY, l = 0.f, o[16] = {};
     for (int i = c - 1; i < grid; ++i) {
