@@ -349,7 +349,10 @@ x100q_model *x100q_model_create(const x100q_model_cfg *cfg);
  * page_table [max_batch][table_stride] (device) serves every layer; its row b is
  * slot b.  Pages and table are the caller's, stay where they are while the model
  * lives, and may be read and written between steps: a slot takes another
- * sequence, or gets another page, by changing its row.
+ * sequence, or gets another page, by changing its row.  The calls with host
+ * pointers (x100q_model_forward, x100q_model_prefill) run on the library's own
+ * stream: they wait for what the default stream has under way, but work of any other
+ * stream on the table or the pages has to be finished before the call.
  * A step takes pos < 0 as a padding token: nothing is stored for it, and its
  * logits mean nothing.  A position >= ctx, or one that the table does not cover,
  * makes the next synchronising call report X100_E_ARG.  x100q_model_kv_copy

@@ -1411,6 +1411,14 @@ const char *x100q_timing_bucket_name(int bucket) {
     return bucket >= 0 && bucket < X100Q_NBUCKETS ? names[bucket] : nullptr;
 }
 
+// The host-pointer calls run on the library's own stream, which no other stream orders.  A paged model reads the caller's
+// table and pages there, so they first wait for what the caller's default stream has under way (c->mu is held).
+static int after_default_stream(x100q_model *m, DevCtx *c) {
+    if (!m->paged) return X100_OK;
+    const int st = check_cuda(cudaEventRecord(c->ev[0], cudaStreamLegacy), X100_E_LAUNCH);
+    return st ? st : check_cuda(cudaStreamWaitEvent(c->stream, c->ev[0], 0), X100_E_LAUNCH);
+}
+
 int x100q_model_forward(x100q_model *m, const int *tokens, const int *pos, float *logits, int batch) {
     set_error(X100_OK);
     if (!m || !tokens || !pos || !logits || batch < 1 || batch > m->cfg.max_batch || !m->tok_embd) {
@@ -1430,7 +1438,8 @@ int x100q_model_forward(x100q_model *m, const int *tokens, const int *pos, float
     float *dh = reinterpret_cast<float *>(buf + 2 * tb);
     float *dl = static_cast<float *>(stage_buf(c, 1, lb));
     if (!dl) return get_error();
-    int st = check_cuda(cudaMemcpyAsync(dtok, tokens, batch * 4, cudaMemcpyDefault, c->stream), X100_E_COPY);
+    int st = after_default_stream(m, c);
+    if (!st) st = check_cuda(cudaMemcpyAsync(dtok, tokens, batch * 4, cudaMemcpyDefault, c->stream), X100_E_COPY);
     if (!st) st = check_cuda(cudaMemcpyAsync(dpos, pos, batch * 4, cudaMemcpyDefault, c->stream), X100_E_COPY);
     if (!st) st = x100q_model_forward_dev(m, dtok, dh, dpos, dl, batch, c->stream);
     if (!st) st = check_cuda(cudaMemcpyAsync(logits, dl, lb, cudaMemcpyDefault, c->stream), X100_E_COPY);
@@ -1464,7 +1473,8 @@ int x100q_model_prefill(x100q_model *m, int slot, const int *tokens, int n, int 
     if (logits && !(dl = static_cast<float *>(stage_buf(c, 1, lb)))) return get_error();
     std::vector<int> hp(n), hs(n, slot);
     for (int i = 0; i < n; ++i) hp[i] = pos0 + i;
-    int st = check_cuda(cudaMemcpyAsync(dtok, tokens, n * 4, cudaMemcpyDefault, c->stream), X100_E_COPY);
+    int st = after_default_stream(m, c);
+    if (!st) st = check_cuda(cudaMemcpyAsync(dtok, tokens, n * 4, cudaMemcpyDefault, c->stream), X100_E_COPY);
     if (!st) st = check_cuda(cudaMemcpyAsync(dpos, hp.data(), n * 4, cudaMemcpyHostToDevice, c->stream), X100_E_COPY);
     if (!st) st = check_cuda(cudaMemcpyAsync(dslot, hs.data(), n * 4, cudaMemcpyHostToDevice, c->stream), X100_E_COPY);
     if (!st) st = forward_impl(m, dtok, dh, dpos, dslot, dl, n, c->stream);
@@ -1505,7 +1515,7 @@ static int prefill_tc(x100q_model *m, int slot, const int *tokens, int n, int po
     if (logits && !(dl = static_cast<float *>(stage_buf(c, 1, lb)))) return get_error();
     std::vector<int> hp(T), hs(T, slot);
     int hq[2] = {0, 0};
-    int st = X100_OK;
+    int st = after_default_stream(m, c);
     for (int c0 = 0; st == X100_OK && c0 < n; c0 += T) {
         const int cn = n - c0 < T ? n - c0 : T;
         for (int i = 0; i < cn; ++i) hp[i] = pos0 + c0 + i;

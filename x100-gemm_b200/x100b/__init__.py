@@ -412,12 +412,21 @@ class Model:
         check(lib().x100q_model_forward_slots_dev(self.h, _p(tokens), _p(h), _p(pos), _p(slot), _p(logits), batch,
                                                   _stream(stream)), "x100q_model_forward_slots_dev")
 
+    def _ordered(self):
+        """The host calls run on the library's own stream and read a paged cache's table and pages, which the
+        caller writes on the current one: wait for that (the call itself waits for the default stream)."""
+        if self._kv4 is not None:
+            s = _torch()[0].cuda.current_stream(self._pages.device)
+            if s.cuda_stream:
+                s.synchronize()
+
     def prefill(self, slot: int, tokens, pos0: int, logits: bool = True):
         """n tokens of the sequence in `slot` at positions pos0 .. pos0+n-1 in
         one step; returns their logits [n][vocab] (or None)."""
         tokens = np.ascontiguousarray(tokens, np.int32)
         n = tokens.shape[0]
         out = np.empty((n, self.cfg.vocab), np.float32) if logits else None
+        self._ordered()
         check(lib().x100q_model_prefill(self.h, slot, _p(tokens), n, pos0, _p(out)), "x100q_model_prefill")
         return out
 
@@ -426,6 +435,7 @@ class Model:
         pos = np.ascontiguousarray(pos, np.int32)
         B = tokens.shape[0]
         logits = np.empty((B, self.cfg.vocab), np.float32)
+        self._ordered()
         check(lib().x100q_model_forward(self.h, _p(tokens), _p(pos), _p(logits), B), "x100q_model_forward")
         return logits
 
