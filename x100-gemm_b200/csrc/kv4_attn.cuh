@@ -22,7 +22,7 @@ struct AttnArgs {
     long qs, os;
     const int *q_start, *kv_len;
     // the model's calls: sequence b reads row row_of[b] < n_rows of the page table (null: row b) and has
-    // kv_len[b] + len_add positions
+    // kv_len[b] + len_add positions, none where kv_len[b] is negative
     const int *row_of = nullptr;
     int n_rows = 0, len_add = 0;
     int nrt_max;                         // row tiles of a sequence of max_q tokens (clusters)
@@ -65,9 +65,10 @@ __device__ __forceinline__ bool load_rows(const AttnArgs &a, int b, int &q0, int
 __device__ __forceinline__ Seq load_seq(const AttnArgs &a, int b, int R, bool report) {
     Seq s;
     const bool bad_q = !load_rows(a, b, s.q0, s.nq);
-    s.len = (int)((unsigned)a.kv_len[b] + a.len_add);
+    s.len = a.kv_len[b];
+    if (a.len_add) s.len = s.len < 0 ? 0 : (int)((unsigned)s.len + a.len_add);   // a position; any below 0 is padding
     s.row = a.row_of ? a.row_of[b] : b;
-    if (a.row_of && (unsigned)s.row >= (unsigned)a.n_rows) s.row = 0, s.len = -1;
+    if (a.row_of && (unsigned)s.row >= (unsigned)a.n_rows) s.row = 0, s.len = s.len ? -1 : 0;
     const int cover = min(a.tab.stride, kMostPositions >> a.pool.page_shift) << a.pool.page_shift;
     if (bad_q || s.len < 0 || s.len > cover) {
         if (report) atomicCAS(a.status, 0, X100_E_ARG);
