@@ -730,12 +730,18 @@ class Kv4Cache:
         return out
 
 
-def rope_table(n_pos: int, head_dim: int, base: float, stream=None):
-    """x100q_rope_table_dev: (cos, sin) [n_pos, head_dim / 2, 2] for Kv4Cache.append."""
-    torch = _torch()[0]
-    t = torch.empty(n_pos, head_dim // 2, 2, dtype=torch.float32, device="cuda")
-    check(lib().x100q_rope_table_dev(t.data_ptr(), n_pos, head_dim, base, _stream(stream)), "x100q_rope_table_dev")
-    return t
+def rope_table(n_pos: int, head_dim: int, base: float, stream=None, out=None):
+    """x100q_rope_table_dev: (cos, sin) [n_pos, head_dim / 2, 2] for Kv4Cache.append, into out (made when None)."""
+    torch, _, _, f32, _, _, _, device, _ = _torch()
+    if out is None:
+        if stream is not None:
+            _refuse("rope_table", _OWN_STREAM)
+        out = torch.empty(n_pos, head_dim // 2, 2, dtype=f32, device="cuda")
+    _placed("rope_table", device(), out=(out, f32))
+    if out.shape != (n_pos, head_dim // 2, 2) or not out.is_contiguous():
+        _refuse("rope_table", f"out has to be [{n_pos}, {head_dim // 2}, 2] contiguous values")
+    check(lib().x100q_rope_table_dev(out.data_ptr(), n_pos, head_dim, base, _stream(stream)), "x100q_rope_table_dev")
+    return out
 
 
 def add_rmsnorm_q8(x, w, q, scales, residual=None, residual_out=None, eps=1e-6, group=0, stream=None):
