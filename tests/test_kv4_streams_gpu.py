@@ -24,3 +24,15 @@ def test_rope_table_on_a_stream_takes_its_output():
         with pytest.raises(x100b.X100Error) as e:
             x100b.rope_table(100, 64, 1e4, out=bad)
         assert e.value.code == x100b.X100_E_ARG
+
+
+def test_a_new_pool_is_zeroed_before_another_stream_appends():
+    side, pos, table, seq = torch.cuda.Stream(), ints([0]), ints([[0]]), ints([0])
+    x = torch.ones(1, 1, 64, device="cuda")
+    torch.cuda.synchronize()
+    torch.cuda._sleep(200_000_000)                        # about a tenth of a second on the current stream
+    cache = x100b.Kv4Cache(1, 16, 1, 64)
+    cache.append(x, x, pos, table, seq=seq, stream=side)
+    torch.cuda.synchronize()
+    k, v = cache.read(pos, table, seq=seq)
+    assert (k == 1).all() and (v == 1).all() and status() == 0

@@ -610,6 +610,7 @@ class Kv4Cache:
             _refuse("Kv4Cache", f"no pool of {n_pages} pages of {page_size} x {n_kv_heads} x {head_dim}")
         if pages is None:
             pages = torch.zeros(n, dtype=torch.uint8, device="cuda")
+            torch.cuda.current_stream().synchronize()   # zeroed before an append on another stream
         if pages.dtype is not torch.uint8 or not pages.is_cuda or not pages.is_contiguous() or pages.numel() < n:
             _refuse("Kv4Cache", f"pages has to be {n} contiguous uint8 on a GPU")
         self.pages, self.kv.pages, self.device = pages, pages.data_ptr(), pages.get_device()
