@@ -1,0 +1,62 @@
+"""Attention over the 4-bit cache where one position dominates the row: the small probabilities under it count."""
+import numpy as np
+import pytest
+import torch
+
+import kv4_ref as ref
+import x100b
+from test_kv4_gpu import DT, ints, status
+
+pytestmark = pytest.mark.gpu
+
+
+def tail_bound(z, v, n, kind):
+    """Largest error of rows of scores z (nats, [rows, n]) over values v >= 0 ([n]) in float64, and the rows' outputs.
+
+    A probability relative to the row's largest, p, is held to 2^-36 of the largest (fp16's subnormal step 2^-24, half of it, under
+    the factor 2^11) or, where that is more, to 2^-11 (fp16) or 2^-21 (both halves, and exp2) of itself; a score's own error is
+    added to it: 40 fp32 steps of its largest product sum, which is the score here (one sign).  The tensor core's sums truncate,
+    2^-23 of the sum for each of its additions: fp16 q n / 16 for prompts and no more for few rows; fp32 q 16 a tile and an fp32
+    addition for each of n / 128.  The denominator is fp32 additions, n / 128 and 330 for the joins; both count with the output."""
+    top = z.max(-1, keepdims=True)
+    p = np.where(np.isfinite(z), np.exp(z - top), 0.0)
+    total = p.sum(-1)
+    out = p @ v / total
+    score = 2 * 40 * 2.0 ** -24 * np.abs(top[:, 0])
+    rel = 2.0 ** -11 if kind == "f16" else 2.0 ** -21
+    held = np.maximum(rel * p, np.where(p > 0, 2.0 ** -36, 0.0)) @ v / total
+    sums = n / 16 + 8 if kind == "f16" else 16 + n / 128
+    bound = held + out * (score + sums * 2.0 ** -23 + (n / 128 + 330) * 2.0 ** -24)
+    if kind == "f16":
+        bound += np.maximum(out * 2.0 ** -11, 2.0 ** -25)
+    return bound, out
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+@pytest.mark.parametrize("T", [1, 3, 32, 300])
+@pytest.mark.parametrize("n", [2600, 131072])
+@pytest.mark.parametrize("nats,spread", [(16.85, 0.0), (24.0, 0.0), (17.0, 1.0), (12.0, 1.0), (5.0, 0.0)])
+def test_a_tail_under_one_position(kind, T, n, nats, spread):
+    """One position `nats` above the others (flat, or spread normally), its v zero and theirs one."""
+    D, page, G, sink = 128, 64, 8, 5
+    rng = np.random.default_rng(n + T)
+    cache = x100b.Kv4Cache(-(-n // page), page, 1, D)
+    score = spread * rng.normal(size=n)
+    score[sink] = nats
+    # every element of a key is one value and every q element 1 / 8: a score is D^-0.5 * D / 8 times it
+    k = torch.from_numpy((score / (D ** 0.5 / 8)).astype(np.float32)).cuda()[:, None, None].expand(n, 1, D).contiguous()
+    v = torch.ones(n, 1, D, device="cuda")
+    v[sink] = 0
+    pos, table = ints(np.arange(n)), ints(np.arange(-(-n // page))[None])
+    seq = torch.zeros_like(pos)
+    cache.append(k, v, pos, table, seq=seq)
+    kb, vb = (t[:, 0, 0].double().cpu().numpy() for t in cache.read(pos, table, seq=seq))
+    assert (np.delete(vb, sink) == 1).all() and vb[sink] == 0
+    q = torch.full((T, G, D), 0.125, device="cuda", dtype=DT[kind])
+    out = cache.attend(q, None, table, ints([n]), q_start=ints([0, T]), max_q=T).double().cpu().numpy()
+    assert status() == 0 and (out == out[:, :1, :1]).all()
+    rows = sorted({0, T // 2, T - 1})
+    z = np.where(np.arange(n)[None] <= n - T + np.array(rows)[:, None], (D ** 0.5 / 8) * kb[None], -np.inf)
+    bound, want = tail_bound(z, vb, n, kind)
+    err = np.abs(out[rows, 0, 0] - want)
+    assert (err <= bound).all(), (err / want, bound / want)

@@ -295,7 +295,7 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
             }
         }
         const bool any_hole = __syncthreads_or(hole);
-        float m[NR][2], nm[NR][2], l[NR][2], o[NR][MT][4];   // m in units of log2: score * sl; nm = -m, or 0 at the start
+        float m[NR][2], nm[NR][2], l[NR][2], o[NR][MT][4];   // m in units of log2: score * sl; nm = kUp - m, or 0 at the start
         int lim[NR][2];                         // positions that rows 2 t, 2 t + 1 of a group see
         float qi[NR == 1 && !HL ? NB : 1][2];   // the lane's qb, in registers where they fit
 #pragma unroll
@@ -403,8 +403,6 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
                         for (int i = 0; i < 4; ++i)
                             if (gone[tt] || p0 + tt * kTile + k0 + 8 * (i >> 1) >= lim[nr][i & 1]) sc[tt][nr][i] = -INFINITY;
             }
-            // The running max follows only when a score passes it by 2^8: until then exp2 of the
-            // difference stays within fp16 and the sums need no rescaling.
             bool grow = false;
             float top[NR][2];
 #pragma unroll
@@ -413,7 +411,7 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
                 for (int i = 0; i < 2; ++i) {
                     top[nr][i] = fmaxf(sc[0][nr][i], sc[0][nr][i + 2]);
                     if constexpr (TT == 2) top[nr][i] = fmaxf(top[nr][i], fmaxf(sc[1][nr][i], sc[1][nr][i + 2]));
-                    grow = grow || top[nr][i] * a.sl > m[nr][i] + 8.f;
+                    grow = grow || top[nr][i] * a.sl > m[nr][i] + kLag;
                 }
             if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
@@ -427,7 +425,7 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
                         const float mn = fmaxf(m[nr][i], x * a.sl);
                         const float f = mn == -INFINITY ? 1.f : ex2(m[nr][i] - mn);
                         m[nr][i] = mn;
-                        nm[nr][i] = mn == -INFINITY ? 0.f : -mn;
+                        nm[nr][i] = mn == -INFINITY ? 0.f : kUp - mn;
                         l[nr][i] *= f;
 #pragma unroll
                         for (int k = 0; k < MT; ++k) o[nr][k][i] *= f, o[nr][k][i + 2] *= f;

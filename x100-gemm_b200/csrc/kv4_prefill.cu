@@ -5,7 +5,7 @@
 // tiles of 128 positions.  Per key tile and row tile S = Q K^T and O += P V, both
 // 128 x 128 x D tcgen05.mma with S, P (over S) and O in TMEM.  One CTA per SM:
 //   warps 0-3, 4-7   softmax of step X = 0, 1: a thread owns a row; S from TMEM, running max
-//                    (moved only when a score passes it by 2^8), P as fp16 back to TMEM
+//                    (moved only when a score passes it by 2^kLag), P as fp16 back to TMEM
 //   fp32 q: 4 warps  add up the products of the steps, a row each (below)
 //   4 or 8 warps     raw codes in shared memory -> fp16 K and V tiles in the 128-byte-swizzled
 //                    layouts the MMA reads; scale * (code - 8) is an fp16 value, so exact
@@ -420,10 +420,10 @@ __global__ void __launch_bounds__(Roles<T>::THREADS, 1) prefill_kernel(const Att
                     for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], s[124 + k]);
                 }
                 const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.sl;
-                if (__any_sync(0xffffffffu, top > m + 8.f)) {
+                if (__any_sync(0xffffffffu, top > m + kLag)) {
                     const float mn = fmaxf(m, top), f = mn == -INFINITY ? 1.f : ex2(m - mn);
                     m = mn;
-                    nm = mn == -INFINITY ? 0.f : -mn;
+                    nm = mn == -INFINITY ? 0.f : kUp - mn;
                     l *= f;
                     if (!HL && c >= 1) {         // O holds sums
                         ok = wait(&bars.o_done[X][(step - 1) & 1], (step - 1) >> 1 & 1);
