@@ -103,13 +103,13 @@ __device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
     return v;
 }
-// D = A B + C with C apart (registers or zeros)
+// D = A B
 __device__ __forceinline__ void mma_init(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1, float c0, float c1) {
+                                         uint32_t b1) {
     asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 template <int D, int NR>
 struct Cfg {
@@ -117,18 +117,17 @@ struct Cfg {
     static constexpr int RING = kWarps * ST * 2 * Lay<D>::BYTES;
     static constexpr int RED = kWarps * 8 * D * 4;            // one 8-row group of every warp, over the idle ring
     static constexpr int QF = NR * (D / 16) * 32 * 16;        // Q fragments: (hi b0, b1, lo b0, b1) per lane
-    static constexpr int QB = NR * (D / 32) * 8 * 4;          // -bias sums of every row and block
     static constexpr int ML = kWarps * 8 * NR * 2 * 4;
-    static constexpr int SMEM = RING + QF + QB + ML;
+    static constexpr int SMEM = RING + QF + ML;
     static_assert(RED <= RING, "");
 };
 
 // S^T = K Q^T and O^T = V^T P^T: positions (then dims) are the M side of
 // m16n8k16, the 8 query rows the N side, so that a group of 8 heads wastes no
-// tensor rows.  For fp16 q K codes go into the product as 64 + code or 1024 + code, one instruction each, and the
-// sum starts from -sum (72 or 1032) q, which each row and block has once: what is left is
-// sum (code - 8) q, which the block's scale multiplies in fp32.  What cancels there costs fp32 q too many bits
-// (outputs off by 5e-6 instead of 3e-7): its codes are made code - 8 first.  V codes become scale * (code - 8), an exact fp16.
+// tensor rows.  K codes go into the product as code - 8 and the block's scale multiplies its sum in fp32; V codes become
+// scale * (code - 8), an exact fp16.  (K as 1024 + code, an instruction less each, with sums that start from -1032 sum q: what cancels
+// there is 129 times what is left, which one large element of q makes an error of the score, and it took longer, 33.6 against
+// 32.4 us for 16 fp16 tokens over 16384 positions each, for the registers that those starts need.)
 // Position k of a tile's MMA rows r: r / 2 + 4 (r % 2) of each half, so that
 // transposing the score fragment gives P^T's B fragment for the positions t,
 // t + 4, t + 8, t + 12 that a lane's V codes hold.  HL (fp32 q): q and p as hi + lo halves, and each tile's
@@ -148,8 +147,7 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
     uint8_t *ring = smem;
     float4 *red = reinterpret_cast<float4 *>(smem);
     uint4 *qf = reinterpret_cast<uint4 *>(smem + C::RING);
-    float *qb = reinterpret_cast<float *>(smem + C::RING + C::QF);
-    float *sm = reinterpret_cast<float *>(smem + C::RING + C::QF + C::QB), *sl = sm + kWarps * R;
+    float *sm = reinterpret_cast<float *>(smem + C::RING + C::QF), *sl = sm + kWarps * R;
     __shared__ uint64_t bars[kWarps * C::ST];
     __shared__ Share s_share;
     __shared__ int abort_flag;
@@ -279,25 +277,17 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
                 }
             }
             // half2 number j of a block's K words holds codes j and j + 4
-            [[maybe_unused]] float bias = 0.f;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 uint4 f;
                 split2(x[2 * j], x[2 * j + 4], f.x, f.z);
                 split2(x[2 * j + 1], x[2 * j + 5], f.y, f.w);
                 qf[(nr * (D / 16) + 2 * blk + j) * 32 + ln] = f;
-                bias = fmaf(-1032.f, x[2 * j] + x[2 * j + 4], fmaf(-72.f, x[2 * j + 1] + x[2 * j + 5], bias));
-            }
-            if constexpr (!HL) {
-                bias += __shfl_xor_sync(0xffffffffu, bias, 1);    // e runs over whole warps
-                bias += __shfl_xor_sync(0xffffffffu, bias, 2);
-                if ((ln & 3) == 0) qb[(nr * NB + blk) * 8 + ln / 4] = bias;
             }
         }
         const bool any_hole = __syncthreads_or(hole);
         float m[NR][2], nm[NR][2], l[NR][2], o[NR][MT][4];   // m in units of log2: score * sl; nm = kUp - m, or 0 at the start
         int lim[NR][2];                         // positions that rows 2 t, 2 t + 1 of a group see
-        float qi[NR == 1 && !HL ? NB : 1][2];   // the lane's qb, in registers where they fit
 #pragma unroll
         for (int nr = 0; nr < NR; ++nr) {
 #pragma unroll
@@ -308,10 +298,6 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
             }
 #pragma unroll
             for (int i = 0; i < MT; ++i) o[nr][i][0] = o[nr][i][1] = o[nr][i][2] = o[nr][i][3] = 0.f;
-        }
-        if constexpr (NR == 1 && !HL) {
-#pragma unroll
-            for (int blk = 0; blk < NB; ++blk) qi[blk][0] = qb[blk * 8 + 2 * t], qi[blk][1] = qb[blk * 8 + 2 * t + 1];
         }
         const int minlim = max(0, first + div_g(a, rt * R) + 1);
         const int k0 = (g >> 1) + 4 * (g & 1);              // this lane's two positions of a tile: k0, k0 + 8
@@ -350,25 +336,13 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const uint32_t w = kw[i][blk];
-                        if constexpr (HL) {
-                            f[i][0] = u32(low_codes(w, expo)), f[i][1] = u32(high_codes(w, expo));
-                            f[i][2] = u32(low_codes(w >> 8, expo)), f[i][3] = u32(high_codes(w >> 8, expo));
-                        } else {
-                            f[i][0] = field(w, kLow, expo.e1024), f[i][1] = field(w, kHigh, expo.e64);
-                            f[i][2] = field(w >> 8, kLow, expo.e1024), f[i][3] = field(w >> 8, kHigh, expo.e64);
-                        }
+                        f[i][0] = u32(low_codes(w, expo)), f[i][1] = u32(high_codes(w, expo));
+                        f[i][2] = u32(low_codes(w >> 8, expo)), f[i][3] = u32(high_codes(w >> 8, expo));
                     }
                     const float d0 = __half2float(kd[0][blk]), d1 = __half2float(kd[1][blk]);
 #pragma unroll
                     for (int nr = 0; nr < NR; ++nr) {
                         float acc[4];
-                        [[maybe_unused]] float i0 = 0.f, i1 = 0.f;
-                        if constexpr (HL) {
-                        } else if constexpr (NR == 1) i0 = qi[blk][0], i1 = qi[blk][1];
-                        else {
-                            const float2 v = *reinterpret_cast<const float2 *>(qb + (nr * NB + blk) * 8 + 2 * t);
-                            i0 = v.x, i1 = v.y;
-                        }
                         const uint4 *qp = qf + (nr * (D / 16) + 2 * blk) * 32 + lane;
                         uint4 q[2];
 #pragma unroll
@@ -377,11 +351,11 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
                             else *reinterpret_cast<uint2 *>(q + h) = *reinterpret_cast<const uint2 *>(qp + h * 32);
                         }
                         if constexpr (HL) {             // lo first: what is added to is small then, and with it what is cut off
-                            mma_init(acc, f[0][0], f[1][0], f[0][1], f[1][1], q[0].z, q[0].w, 0.f, 0.f);
+                            mma_init(acc, f[0][0], f[1][0], f[0][1], f[1][1], q[0].z, q[0].w);
                             mma(acc, f[0][2], f[1][2], f[0][3], f[1][3], q[1].z, q[1].w);
                             mma(acc, f[0][0], f[1][0], f[0][1], f[1][1], q[0].x, q[0].y);
                         } else {
-                            mma_init(acc, f[0][0], f[1][0], f[0][1], f[1][1], q[0].x, q[0].y, i0, i1);
+                            mma_init(acc, f[0][0], f[1][0], f[0][1], f[1][1], q[0].x, q[0].y);
                         }
                         mma(acc, f[0][2], f[1][2], f[0][3], f[1][3], q[1].x, q[1].y);
                         float(&x)[4] = sc[tt][nr];
@@ -494,7 +468,7 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
                                 float(&sum)[4] = o[nr][4 * w + 2 * hf + e];
                                 if constexpr (HL) {
                                     float x4[4];
-                                    mma_init(x4, a0, a1, a2, a3, pl[nr][0], pl[nr][1], 0.f, 0.f);
+                                    mma_init(x4, a0, a1, a2, a3, pl[nr][0], pl[nr][1]);
                                     mma(x4, a0, a1, a2, a3, ph[nr][0], ph[nr][1]);
 #pragma unroll
                                     for (int i = 0; i < 4; ++i) sum[i] += x4[i];

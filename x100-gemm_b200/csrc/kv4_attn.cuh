@@ -83,16 +83,13 @@ __device__ __forceinline__ Seq load_seq(const AttnArgs &a, int b, int R, bool re
 __device__ __forceinline__ uint32_t u32(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
 __device__ __forceinline__ __half2 h2(uint32_t u) { return *reinterpret_cast<__half2 *>(&u); }
 // Codes of both halves of a word as fp16 by placing them under an exponent:
-// bits 0-3 under 1024's read as 1024 + code, bits 4-7 as 1024 + 16 code, and bits
-// 4-7 under 64's as 64 + code.  The exponents come in registers that the
-// compiler cannot see through: with both as immediates each (w & mask) | exponent
+// bits 0-3 under 1024's read as 1024 + code, bits 4-7 as 1024 + 16 code (the int4 to fp16 conversion of Kim et al., "Who Says
+// Elephants Can't Run: Bringing Large Scale MoE Models into Cloud Scale Production", 2022).  The exponent comes in a register that the
+// compiler cannot see through: with it as an immediate each (w & mask) | exponent
 // would be two instructions instead of one.
 struct Exponents {
-    uint32_t e1024, e64;
-    __device__ Exponents() {
-        asm volatile("mov.b32 %0, 0x64006400;" : "=r"(e1024));
-        asm volatile("mov.b32 %0, 0x54005400;" : "=r"(e64));
-    }
+    uint32_t e1024;
+    __device__ Exponents() { asm volatile("mov.b32 %0, 0x64006400;" : "=r"(e1024)); }
 };
 __device__ __forceinline__ uint32_t field(uint32_t w, uint32_t mask, uint32_t expo) {
     uint32_t r;
