@@ -202,9 +202,11 @@ int x100q_rope_table_dev(float *rope, int n_pos, int head_dim, float base, void 
  * stay until the call has run.  max_q bounds the tokens of any one sequence, and q_start must
  * not decrease or pass n_tokens; a sequence that breaks this is left out, and the
  * next synchronising call reports X100_E_ARG.
- * X100Q_F32: q (|q| <= 65504, as two fp16 halves) is used to 22 bits, the
- * probabilities to 22 bits down to 2^-14 of the row's largest and below to 2^-36 of it,
- * and sums are fp32 additions over tiles of 16 or 128 positions.
+ * X100Q_F32: q times the power of two next to scale * sqrt(head_dim), which is 1 for
+ * the usual scale, is held as two fp16 halves: it may be 65504 at most, and is used to 22
+ * bits from 1/8 up and to 2^-25 below.  Probabilities are used to 22 bits down to 2^-14
+ * of the row's largest and below to 2^-36 of it, and sums are fp32 additions over
+ * tiles of 16 or 128 positions.
  * X100Q_F16: probabilities are rounded to fp16 (11 bits down to 2^-25 of the row's
  * largest, below to 2^-36 of it) and out is rounded once; sums are the
  * tensor cores' own, fp32 and truncating, which over 131072 positions loses less

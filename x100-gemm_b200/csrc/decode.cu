@@ -950,7 +950,7 @@ static int kv4_step(x100q_model *m, DevCtx *c, int layer, float *qkv, float *att
     a.q_start = q_start, a.kv_len = q_start ? pos + n - 1 : pos, a.len_add = 1;
     a.row_of = slot, a.n_rows = g.max_batch;
     a.n_tokens = n, a.max_q = q_start ? n : 1;
-    kv4::attn_shape(a, g.n_heads, 1.0f / sqrtf((float)g.head_dim));
+    kv4::attn_shape(a, g.n_heads, 1.0f / sqrtf((float)g.head_dim), X100Q_F32, g.head_dim);
     a.part = static_cast<float *>(m->kv4_work);
     a.status = c->d_status;
     return kv4::launch_attention(c, a, X100Q_F32, g.head_dim, s);

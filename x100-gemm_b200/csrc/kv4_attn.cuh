@@ -30,7 +30,8 @@ struct AttnArgs {
     uint32_t g_mul;                      // ceil(2^32 / G): n / G = umulhi(n, g_mul) for n < 2^32 / G
     int unit_shift;                      // positions per unit, a power of two (128 unless the list would pass 2^31 units)
     int lead;                            // units that an item counts for besides its positions' (see kv4_attn.cu)
-    float sl;                            // scale * log2(e)
+    float sl;                            // scale * log2(e) / q_up
+    float q_up;                          // power of two that fp32 q is multiplied with before it is split (attn_shape)
     // work: of the first (slot 0) and last (slot 1) item that a run has a part of only
     float *part;                         // [kMaxCtas][2][8 NR * D] o in fragment order
     float2 *ml;                          // [kMaxCtas][2][8 NR] running max (log2 units) and sum
@@ -118,7 +119,8 @@ __device__ __forceinline__ float ex2(float x) {
 // against 405 us for 4096 tokens over 8192 positions) and the same elsewhere; 2 and 1 cost them 9 and 15 %.
 constexpr float kLag = 4.f, kUp = 11.f;
 
-// x = hi + lo: 22 bits from 2^-3 up, and to 2^-25 below
+// x = hi + lo: 22 bits from 2^-3 up, and to 2^-25 below.  q is brought near the size that it has with a scale of head_dim^-0.5 first
+// (attn_shape), so that 2^-25 of it is as little of a score whatever the scale.
 __device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t &lo) {
     const __half2 h = __floats2half2_rn(x, y);
     const float2 f = __half22float2(h);
@@ -134,7 +136,7 @@ bool prefill_fits(const AttnArgs &a, int dtype);   // its units can be counted i
 int launch_prefill(DevCtx *c, AttnArgs &a, int dtype, int head_dim, cudaStream_t s);
 
 // n_heads, G and the scale; then the call, its arguments checked (kv4_attn.cu).
-void attn_shape(AttnArgs &p, int n_heads, float scale);
+void attn_shape(AttnArgs &p, int n_heads, float scale, int dtype, int head_dim);
 int launch_attention(DevCtx *c, AttnArgs &p, int dtype, int head_dim, cudaStream_t s);
 
 }  // namespace kv4
