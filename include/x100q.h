@@ -207,8 +207,9 @@ int x100q_rope_table_dev(float *rope, int n_pos, int head_dim, float base, void 
  * bits from 1/8 up and to 2^-25 below.  Probabilities are used to 22 bits down to 2^-14
  * of the row's largest and below to 2^-36 of it, and sums are fp32 additions over
  * tiles of 16 or 128 positions.
- * X100Q_F16: probabilities are rounded to fp16 (11 bits down to 2^-25 of the row's
- * largest, below to 2^-36 of it) and out is rounded once; sums are the
+ * X100Q_F16: out is rounded once; probabilities are as for fp32 q, but where max_q tokens
+ * make 256 rows of a kv head or more they are rounded to fp16 (11 bits down to 2^-25
+ * of the row's largest, below to 2^-36 of it); sums are the
  * tensor cores' own, fp32 and truncating, which over 131072 positions loses less
  * than 1e-4 of them.
  * The result does not depend on the order in which blocks run.

@@ -5,7 +5,7 @@ import torch
 
 import kv4_ref as ref
 import x100b
-from test_kv4_gpu import DT, ints, status
+from test_kv4_gpu import DT, cache_of, dev, ints, page_table, status
 
 pytestmark = pytest.mark.gpu
 
@@ -60,3 +60,34 @@ def test_a_tail_under_one_position(kind, T, n, nats, spread):
     bound, want = tail_bound(z, vb, n, kind)
     err = np.abs(out[rows, 0, 0] - want)
     assert (err <= bound).all(), (err / want, bound / want)
+
+
+@pytest.mark.parametrize("D,page,kv,G,T", [(128, 64, 2, 8, 1), (64, 16, 2, 5, 1), (128, 32, 1, 7, 3), (64, 64, 2, 8, 4), (128, 64, 1, 8, 4), (64, 32, 1, 31, 1)])
+def test_few_fp16_rows_are_off_by_the_outputs_rounding(D, page, kv, G, T):
+    """Under 256 rows fp16 q is as near as fp32 q before the output is rounded: wherever that settles the rounding, it is the right one.
+
+    Before it, as ref.attention_bound has it for fp32 q, row by row: the score's errors with A the row's own largest scale * sum |q k|, twice
+    (numerator and sum), exp2 and the halves of p; then sums over n / 16 steps of a warp and the joins of 8 warps and n / 128 + 2 runs."""
+    rng = np.random.default_rng(D + G)
+    lens = [2, 5, 16, 33]
+    pool = ref.random_pool(rng, sum(-(-n // page) for n in lens), page, kv, D)
+    table = page_table(rng, lens, page, pool.raw.shape[0])
+    q = rng.normal(size=(4 * T, kv * G, D)).astype(np.float16)
+    checked = []
+    for t in (table, np.concatenate([table, np.full((4, 6000), -1, np.int32)], 1)):          # clusters, and runs with a merge
+        got = cache_of(pool).attend(dev(q), None, ints(t), ints(lens), q_start=ints(np.arange(5) * T), max_q=T).cpu().numpy()
+        assert status() == 0
+        for i, n in enumerate(lens):
+            rows = slice(i * T, i * T + T)
+            k, v = pool.values(table[i], n, False), pool.values(table[i], n, True)
+            want = ref.attention(q[rows], k, v, n - T, D ** -0.5)
+            size = np.abs(q[rows].astype(np.float64)).reshape(T, kv, G, D)
+            A = D ** -0.5 * np.einsum("tkgd,nkd->tkgn", size, np.abs(k)).max(-1).reshape(T, kv * G, 1)
+            rel = 2 * (A * (2.0 ** -22 + (D / 8 + D / 32 + 1) * 2.0 ** -23) + 2.0 ** -21) + (n / 16 + 2) * 2.0 ** -23 + (n / 128 + 10) * 2.0 ** -24
+            off = rel * np.abs(v).max()
+            near = want.astype(np.float16)
+            step = np.spacing(np.abs(near)).astype(np.float64)
+            sure = step / 2 - np.abs(want - near) > off          # so far from a tie that the rounding is known
+            checked.append(sure.mean())
+            assert np.array_equal(got[rows][sure], near[sure]), (n, (got[rows][sure] != near[sure]).mean())
+    assert max(checked) > 0.25                                   # the bound settles enough of them to tell

@@ -130,9 +130,10 @@ struct Cfg {
 // 32.4 us for 16 fp16 tokens over 16384 positions each, for the registers that those starts need.)
 // Position k of a tile's MMA rows r: r / 2 + 4 (r % 2) of each half, so that
 // transposing the score fragment gives P^T's B fragment for the positions t,
-// t + 4, t + 8, t + 12 that a lane's V codes hold.  HL (fp32 q): q and p as hi + lo halves, and each tile's
+// t + 4, t + 8, t + 12 that a lane's V codes hold.  p goes in as hi + lo halves: rounded to fp16 it was as far off as the output's own
+// rounding, 2.8e-4 instead of 2.1e-4 of the result together (16 x 16384 positions 32.5 -> 34.4 us).  HL (fp32 q): q as hi + lo halves
+// too, and each tile's
 // P V in sums of its own that fp32 additions take up: the tensor core truncates what it adds to, 1.2e-8 of it a step.
-// fp16 q: p rounded to fp16, whose error is no larger than the output's own rounding (16 x 16384 positions 36.5 -> 33.9 us).
 // Every warp walks its own positions with its own ring of bulk copies (two tiles a
 // stage), so the loop has no CTA barrier.
 // CLUSTER: an item is a cluster's, its positions shared out among the CTAs and their sums joined through shared memory,
@@ -411,8 +412,7 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
 #pragma unroll
             for (int tt = 0; tt < TT; ++tt) {
                 if (EDGE && tt >= n) break;
-                uint32_t ph[NR][2];
-                [[maybe_unused]] uint32_t pl[NR][2];
+                uint32_t ph[NR][2], pl[NR][2];
 #pragma unroll
                 for (int nr = 0; nr < NR; ++nr) {
                     float p[4];
@@ -422,13 +422,8 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
                     l[nr][1] += p[1] + p[3];
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        if constexpr (HL) {
-                            split2(p[2 * i], p[2 * i + 1], ph[nr][i], pl[nr][i]);
-                            pl[nr][i] = transpose8(pl[nr][i]);
-                        } else {
-                            ph[nr][i] = u32(__floats2half2_rn(p[2 * i], p[2 * i + 1]));
-                        }
-                        ph[nr][i] = transpose8(ph[nr][i]);
+                        split2(p[2 * i], p[2 * i + 1], ph[nr][i], pl[nr][i]);
+                        ph[nr][i] = transpose8(ph[nr][i]), pl[nr][i] = transpose8(pl[nr][i]);
                     }
                 }
                 // ---- O += P V: this lane's positions t + 4 m, dims g * D / 8 .. ----
@@ -476,6 +471,7 @@ __global__ void __launch_bounds__(kWarps * 32, NR == 1 ? 2 : 1) attn_kernel(cons
 #pragma unroll
                                     for (int i = 0; i < 4; ++i) sum[i] += x4[i];
                                 } else {
+                                    mma(sum, a0, a1, a2, a3, pl[nr][0], pl[nr][1]);
                                     mma(sum, a0, a1, a2, a3, ph[nr][0], ph[nr][1]);
                                 }
                             }
