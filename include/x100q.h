@@ -239,7 +239,9 @@ int x100q_kv4_attn_dev(const x100q_kv4 *kv, const x100q_kv4_attn_args *a, void *
  * residual_out; no addition where residual is NULL), y = h * w / sqrt(mean(h^2) +
  * eps), and y in int8 with one fp32 scale per `group` elements (0: per row;
  * 32, 64 or 128, dividing d): y ~ q * scale.  The rows are the A operand of
- * gemm_ime_i8_dev_ld, as x100q_pack_act_dev makes the packed records.
+ * gemm_ime_i8_dev_ld.  A scale per row multiplies the rows of its product; scales per
+ * group, which int32 sums over all of K cannot carry, those of one product per group
+ * (K = group, A from column i * group, B from its row), to be added up.
  * With a = max |h w| over the group: q = rint(h w * (127 / a)), scale = a / 127 / rms.
  * Groups with a < 2^-110 are zeros with scale 0; a group with a NaN or an
  * infinity has q = 0 and scale NaN.
