@@ -244,7 +244,8 @@ int x100q_kv4_attn_dev(const x100q_kv4 *kv, const x100q_kv4_attn_args *a, void *
  * (K = group, A from column i * group, B from its row), to be added up.
  * With a = max |h w| over the group: q = rint(h w * (127 / a)), scale = a / 127 / rms.
  * Groups with a < 2^-110 are zeros with scale 0; a group with a NaN or an
- * infinity has q = 0 and scale NaN.
+ * infinity has q = 0 and scale NaN.  The sum of squares is fp32: a row whose sum passes
+ * its range (elements of some 1e19) has all scales NaN.
  * x, residual, residual_out: dtype elements (X100Q_F32 or X100Q_F16), row pitches in
  * elements; residual_out may be residual, or x.  q: int8, row pitch ldq
  * >= d; the pad is left as it was.  scales [rows][d / group] (or [rows]).

@@ -50,7 +50,7 @@ __device__ __forceinline__ float mag(float t) {
 }
 __device__ __forceinline__ float inv_of(float top) { return top < kTiny || top == INFINITY ? 0.f : __fdiv_rn(127.f, top); }
 __device__ __forceinline__ float scale_of(float top, float rstd) {
-    return top == INFINITY ? NAN : top < kTiny ? 0.f : top * (1.f / 127.f) * rstd;
+    return top == INFINITY || rstd == 0.f ? NAN : top < kTiny ? 0.f : top * (1.f / 127.f) * rstd;   // rstd 0: the sum of squares is infinite
 }
 __device__ __forceinline__ int code_of(float t, float inv) {
     return inv == 0.f ? 0 : __float2int_rn(fminf(fmaxf(__fmul_rn(t, inv), -127.f), 127.f));
