@@ -157,7 +157,8 @@ size_t x100q_kv4_bytes(const x100q_kv4 *kv);
  * then times 1 / sqrt(mean(x^2) + eps) where there is a norm weight: the
  * order rmsnorm-then-rope of the model's step up to rounding.  The rotated q goes
  * to q_out (may be q itself), k and v to the cache.  Codes come from the
- * value before the factor 1 / rms, which only scales d.
+ * value before the factor 1 / rms, which only scales d.  A head whose sum of squares
+ * passes fp32's range counts as not finite: q_out is NaN, k's blocks are zeros and reported.
  * q, k, v, q_out: dtype elements, 16-byte aligned; token i's heads lie side by
  * side from element i * stride; strides in elements, multiples of 16 bytes.
  * Several tokens of one sequence may be appended at once, at different

@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 3 : 4) append_kernel(con
             for (int e = 0; e < 8; ++e) ss = fmaf(t[e], t[e], ss);
 #pragma unroll
             for (int o = LH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            s = __frsqrt_rn(ss * (1.f / D) + a.eps);
+            s = ss < INFINITY ? __frsqrt_rn(ss * (1.f / D) + a.eps) : NAN;   // past fp32's range: not a head of zeros
 #pragma unroll
             for (int e = 0; e < 8; ++e) t[e] = __fmul_rn(t[e], sizeof(T) == 4 && is_q ? wq[sizeof(T) == 4 ? e : 0] : __ldg(w + in * 8 + e));
         }
