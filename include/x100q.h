@@ -156,7 +156,7 @@ size_t x100q_kv4_bytes(const x100q_kv4 *kv);
  * none; element j with j + head_dim / 2, as rope_apply, qwen_moe_q3k.c:1173-1175),
  * then times 1 / sqrt(mean(x^2) + eps) where there is a norm weight: the
  * order rmsnorm-then-rope of the model's step up to rounding.  The rotated q goes
- * to q_out (may be q itself), k and v to the cache.  Codes come from the
+ * to q_out (may be q itself, with its stride), k and v to the cache.  Codes come from the
  * value before the factor 1 / rms, which only scales d.  A head whose sum of squares
  * passes fp32's range counts as not finite: q_out is NaN, k's blocks are zeros and reported.
  * q, k, v, q_out: dtype elements, 16-byte aligned; token i's heads lie side by
@@ -199,7 +199,7 @@ int x100q_rope_table_dev(float *rope, int n_pos, int head_dim, float base, void 
  * (NULL: one token each, row b); they are its last positions, and each attends to
  * all positions up to its own.  A row that sees no position (kv_len[b]
  * shorter than the sequence's tokens) is zero.  Rows past q_start[n_seqs] stay as
- * they were; out may be q itself.  What q_start, kv_len and the page table hold has to
+ * they were; out may be q itself, with its stride.  What q_start, kv_len and the page table hold has to
  * stay until the call has run.  max_q bounds the tokens of any one sequence, and q_start must
  * not decrease or pass n_tokens; a sequence that breaks this is left out, and the
  * next synchronising call reports X100_E_ARG.
@@ -248,7 +248,7 @@ int x100q_kv4_attn_dev(const x100q_kv4 *kv, const x100q_kv4_attn_args *a, void *
  * infinity has q = 0 and scale NaN.  The sum of squares is fp32: a row whose sum passes
  * its range (elements of some 1e19) has all scales NaN.
  * x, residual, residual_out: dtype elements (X100Q_F32 or X100Q_F16), row pitches in
- * elements; residual_out may be residual, or x.  q: int8, row pitch ldq
+ * elements; residual_out may be residual, or x, with its pitch.  q: int8, row pitch ldq
  * >= d; the pad is left as it was.  scales [rows][d / group] (or [rows]).
  * Fastest when the pointers are 16-byte aligned and d and the pitches are
  * multiples of 16.                                                          */

@@ -290,7 +290,8 @@ int x100q_kv4_append_dev(const x100q_kv4 *kv, const x100q_kv4_append_args *a, vo
         return refuse(X100_E_ARG);
     if (a->q && (a->n_heads < 1 || a->n_heads > 4096 || !a->q_out || !aligned16(a->q) || !aligned16(a->q_out) ||
                  !pitch_ok(a->q_stride, a->n_heads * kv->head_dim, es) ||
-                 !pitch_ok(a->q_out_stride, a->n_heads * kv->head_dim, es)))
+                 !pitch_ok(a->q_out_stride, a->n_heads * kv->head_dim, es) ||
+                 !in_place_ok(a->q, a->q_stride, a->q_out, a->q_out_stride, a->n_tokens)))
         return refuse(X100_E_ARG);
     DevCtx *c = ctx();
     if (!c) return get_error();

@@ -65,6 +65,10 @@ inline Pool make_pool(const x100q_kv4 *kv) {
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 // a row pitch in elements: whole 16 bytes, and rows do not overlap
 inline bool pitch_ok(long stride, int width, int esize) { return stride >= width && stride * esize % 16 == 0; }
+// an output may be its input itself, row for row: with another pitch one row's output would be another row's input
+inline bool in_place_ok(const void *in, long stride, const void *out, long out_stride, int rows) {
+    return in != out || stride == out_stride || rows < 2;
+}
 
 // Tile of position `pos` of sequence `seq` for kv head `h`, or nullptr when
 // the table or the pool does not cover it.

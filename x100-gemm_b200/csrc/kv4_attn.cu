@@ -827,6 +827,7 @@ int x100q_kv4_attn_dev(const x100q_kv4 *kv, const x100q_kv4_attn_args *a, void *
         !a->out || !aligned16(a->q) || !aligned16(a->out) || !a->kv_len || !a->page_table || a->table_stride < 1 ||
         a->n_seqs < 1 || a->max_q < 1 || (!a->q_start && a->n_tokens != a->n_seqs) ||
         !pitch_ok(a->q_stride, a->n_heads * kv->head_dim, es) || !pitch_ok(a->out_stride, a->n_heads * kv->head_dim, es) ||
+        !in_place_ok(a->q, a->q_stride, a->out, a->out_stride, a->n_tokens) ||
         !(a->scale > 0.f) || !(a->scale < INFINITY) || !a->work || !aligned16(a->work))
         return refuse(X100_E_ARG);
     if (a->work_bytes < x100q_kv4_attn_work(kv, a->n_tokens, a->n_heads, a->n_seqs)) return refuse(X100_E_TOO_LARGE);

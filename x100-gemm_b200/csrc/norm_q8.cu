@@ -267,6 +267,9 @@ extern "C" int x100q_add_rmsnorm_q8_dev(const x100q_norm_q8_args *a, void *strea
         !al(a->residual_out) || (a->residual && a->ldr < a->d) || (a->residual && a->residual_out && a->ldo < a->d) ||
         (!a->residual && a->residual_out) || reinterpret_cast<uintptr_t>(a->w) % 4 || reinterpret_cast<uintptr_t>(a->scales) % 4)
         return refuse(X100_E_ARG);
+    // in place row for row: with another pitch one row's sum would be another row's input
+    if (a->rows > 1 && a->residual_out && ((a->residual_out == a->x && a->ldo != a->ldx) || (a->residual_out == a->residual && a->ldo != a->ldr)))
+        return refuse(X100_E_ARG);
     if (a->group != 0 && ((a->group != 32 && a->group != 64 && a->group != 128) || a->d % a->group)) return refuse(X100_E_ARG);
     DevCtx *c = ctx();
     if (!c) return get_error();
