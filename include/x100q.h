@@ -214,6 +214,9 @@ int x100q_rope_table_dev(float *rope, int n_pos, int head_dim, float base, void 
  * tensor cores' own, fp32 and truncating, which over 131072 positions loses less
  * than 1e-4 of them.
  * The result does not depend on the order in which blocks run.
+ * max_q chooses the kernel for the whole call: one sequence of 256 rows sends all through
+ * the one for prompts, where a single token costs as much as a tile of 128 or 256 rows.
+ * A prompt beside single tokens is faster as two calls.
  * work: 16-byte aligned device scratch of x100q_kv4_attn_work() bytes; its
  * contents need not be kept or cleared, but calls that overlap on the GPU
  * (other streams, replayed graphs) need one each.                          */

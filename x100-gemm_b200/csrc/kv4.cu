@@ -71,9 +71,10 @@ struct Eight {
 // makes the codes the same on any machine that follows the formula.  Codes are taken before the factor
 // 1 / rms, which a block's scale carries: rounding of the sum of squares cannot move a value over a code's
 // border.
-// Bound by instructions when there are many tokens (issue slots 0.75 busy for fp16, DRAM 0.27), by the launch when there are
-// few.  1024 tokens of 32 + 2 x 4 heads of 128, fp32: 38 MB in 10.6 us; 8 x 2047 of 14 + 2 x 2 heads of 64, fp16: 76 MB in
-// 33 us.  A warp per head with 4 elements a lane took 195 us there (with the read-back), a loop per kind of head 4 us more than
+// Bound by instructions when there are many tokens (issue slots 0.72 busy for fp16, DRAM 0.28; 8 shuffles a lane and group are the
+// partners' elements, which this layout has in another lane), by the launch when there are
+// few.  1024 tokens of 32 + 2 x 4 heads of 128, fp32: 38 MB in 10.8 us; 8 x 2047 of 16 + 2 x 8 heads of 64, fp16: 112 MB in
+// 33.5 us.  A warp per head with 4 elements a lane took 195 us there (with the read-back), a loop per kind of head 4 us more than
 // one over all, two groups on their way or k's and v's heads as one list the same.
 template <typename T, int D>
 __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 3 : 4) append_kernel(const AppendArgs a) {

@@ -8,9 +8,10 @@
 // knows).  Row tiles that a run cuts leave partial (o, m, l) sums in `work`;
 // merge_kernel joins them in run order, so results do not depend on timing.  Few items of
 // few positions take clusters instead, which join without it.
-// Long contexts are bound by instructions, not bytes: 233 for 16 positions of 8 fp16 rows, most of them unpacking, issued at half
-// of the peak rate over the whole kernel (DRAM 0.35, tensor pipe 0.17): 16 tokens over 16384 positions each, 85 MB, in 34 us; one
-// fp32 token over 131071, 76 MB, in 32 us.  Short ones by a chain of round trips: one token over 4096 positions 8.9 us.
+// Long contexts are not bound by bytes: 255 instructions for 16 positions of 8 fp16 rows, most of them unpacking, of which an SM issues one
+// in two cycles (each waits 1.2 cycles for a fixed latency and 1.0 for the mma pipe; DRAM 0.33, tensor pipe 0.24), and some 8 us that
+// do not depend on the length (the list, the first round trips, the joins): 16 tokens over 16384 positions each, 85 MB, in 34.4 us; one
+// fp32 token over 131071, 76 MB, in 32.4 us.  Short ones by a chain of round trips: one token over 4096 positions 8.1 us.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -24,9 +25,9 @@ constexpr int kWarps = 8;
 constexpr int kLead = 3;                // units (of 128 positions) that starting an item costs: 2 and 5 measured alike, 0 5 % slower
 
 // Few items over a table that cannot hold long sequences go to clusters: of the most CTAs of which all items' fit the card at
-// once, if that makes at most cluster_units units a CTA.  One fp32 token over 1024, 4096, 8192 positions 9.5, 10.6,
-// 12.5 us by runs and 7.7, 8.1, 11.3 by clusters of 16, over 12288 (6 units each) 13.4 and 14.3; 16 fp16 tokens over 4096 each (8 units)
-// 17.0 and 14.2; with several row groups 2 units a CTA took as long either way.
+// once, if that makes at most cluster_units units a CTA.  One fp32 token over 1024, 4096, 8192 positions 9.6, 10.8,
+// 12.7 us by runs and 7.5, 8.1, 11.3 by clusters of 16, over 12288 (6 units each) 13.3 and 14.3; 16 fp16 tokens over 4096 each (8 units)
+// 16.5 and 14.6; with several row groups 2 units a CTA took as long either way.
 constexpr int cluster_units(int row_groups, bool fp32) { return row_groups > 1 ? 1 : fp32 ? 4 : 8; }
 
 // A run's share of the list, found by one whole warp: its units, and the
@@ -135,7 +136,8 @@ struct Cfg {
 // too, and each tile's
 // P V in sums of its own that fp32 additions take up: the tensor core truncates what it adds to, 1.2e-8 of it a step.
 // Every warp walks its own positions with its own ring of bulk copies (two tiles a
-// stage), so the loop has no CTA barrier.
+// stage), so the loop has no CTA barrier.  One row group at heads of 128 takes all of the 128 registers that two CTAs an SM leave it
+// (32 to 40 bytes spilled).
 // CLUSTER: an item is a cluster's, its positions shared out among the CTAs and their sums joined through shared memory,
 // with no second kernel.
 template <typename T, int D, int NR, bool CLUSTER>
@@ -773,7 +775,7 @@ static int launch(DevCtx *c, AttnArgs &a, cudaStream_t s) {
 template <typename T, int D>
 static int launch_rows(DevCtx *c, AttnArgs &a, cudaStream_t s) {
     // row tiles of up to 4 groups of 8 rows, as few as there can be and as even: 35 rows go as 24 + 11 (3 groups each), not 32 + 3
-    // (7 x 5 tokens of 14 heads over 2 kv heads of 64, 8192 positions: 17.5 us against 19.9; 3 fp32 tokens over 4096, 24 rows, 15.3 against 18.1)
+    // (7 x 5 tokens of 14 heads over 2 kv heads of 64, 8192 positions: 17.8 us against 20.4; 3 fp32 tokens over 4096, 24 rows, 15.2 against 18.1)
     const int groups = (int)(((long)a.max_q * a.G + 7) / 8), nrt = (groups + 3) / 4, nr = (groups + nrt - 1) / nrt;
     if (nr == 1) return launch<T, D, 1>(c, a, s);
     if (nr == 2) return launch<T, D, 2>(c, a, s);

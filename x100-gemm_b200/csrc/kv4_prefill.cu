@@ -14,8 +14,10 @@
 // fp16 q: the steps X are two row tiles over the same key tile (256 rows per item), so that
 // a key tile is unpacked once for both; O stays in TMEM.  fp32 q: q and P are carried as hi + lo halves, two
 // products each, the steps X are every other key tile of one row tile, and O of a step is added to fp32
-// registers: summed in TMEM it was off by 3e-6 at 2600 positions and more at each further one, and is now by 5e-7,
-// for 134 us instead of 108 (1024 tokens over 2600 positions, 32 heads).
+// registers: summed in TMEM it was off by 3e-6 at 2600 positions and more at each further one, and is now by 5e-7, for
+// some 22 us more (1024 tokens over 2600 positions, 32 heads: 124 us; tensor pipe 0.28 busy, issue slots 0.31, every role waits for others
+// most of the time).  fp16 q: 4096 tokens over 8192 positions 405 us (tensor pipe 0.48, issue slots 0.44); p in hi + lo halves there too would
+// take 644, so it is rounded to fp16, which with the output's own rounding makes 2.9e-4 instead of 2.1e-4 of the result.
 // Either way one step's softmax runs beside the other's products.
 //
 // The work list is the one of kv4_attn.cu with units of 128 positions, each row

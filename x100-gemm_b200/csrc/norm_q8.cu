@@ -156,7 +156,8 @@ __global__ void __launch_bounds__(NT > 256 ? NT : 256) row_kernel(const Args a) 
 // Any width, alignment and pitch: one CTA per row, element by element, three
 // walks over the row (the later ones from cache).  A warp takes 128 neighbouring
 // elements at a time, lane + 32 j, so groups lie within one.  Two to four times row_kernel's time (a row of 2048 4.1 us,
-// 16384 rows of 4096 294 us), and only for rows that it cannot take.
+// 16384 rows of 4096 300 us), and only for rows that it cannot take: other alignments and pitches, and rows past its registers (fp32
+// from 8192 elements, fp16 from 16384).
 template <typename T>
 __global__ void __launch_bounds__(256) any_kernel(const Args a) {
     __shared__ float s_sum[8], s_top[8];
