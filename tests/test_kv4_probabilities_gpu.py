@@ -91,3 +91,36 @@ def test_few_fp16_rows_are_off_by_the_outputs_rounding(D, page, kv, G, T):
             checked.append(sure.mean())
             assert np.array_equal(got[rows][sure], near[sure]), (n, (got[rows][sure] != near[sure]).mean())
     assert max(checked) > 0.25                                   # the bound settles enough of them to tell
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+@pytest.mark.parametrize("T", [1, 3, 64])
+@pytest.mark.parametrize("n", [300, 1024, 5000])
+def test_large_common_scores_cancel(kind, T, n):
+    """Scores of 163840 + 0 .. 60 in steps of 1/4, all exact sums in fp32: the softmax is that of the small part.
+
+    What is left of a probability's error is the rounding of its exponent, which lies in -60 .. 15 (2^-19 of a power of two), exp2's
+    and the halves' 2^-21 (fp16 prompts 2^-11), the scale's 2^-24 on the small part (8 powers of two), and the sums: n / 16 + 16 steps
+    of 2^-23 (of 16 positions or fewer additions) and joins of 8 warps and n / 128 + 2 runs; numerator and sum carry it."""
+    D, page, G = 128, 32, 8
+    rng = np.random.default_rng(n + T)
+    small = rng.integers(0, 241, n) / 4
+    k = np.zeros((n, 1, D), np.float32)
+    k[:, 0, :32], k[:, 0, 32:64] = 5120, small[:, None]
+    v = rng.choice([-1.0, 1.0], (n, 1, D)).astype(np.float32)
+    cache, pos, table = x100b.Kv4Cache(-(-n // page), page, 1, D), ints(np.arange(n)), ints(np.arange(-(-n // page))[None])
+    seq = torch.zeros_like(pos)
+    cache.append(dev(k), dev(v), pos, table, seq=seq)
+    kb, vb = (t.double().cpu().numpy() for t in cache.read(pos, table, seq=seq))
+    assert np.array_equal(kb, k)                          # 240 has 8 significant bits
+    q = np.zeros((T, G, D), np.float32 if kind == "f32" else np.float16)
+    q[..., :32], q[..., 32:64] = 1, 1 / 32
+    out = cache.attend(dev(q), None, table, ints([n]), q_start=ints([0, T]), max_q=T).cpu().numpy()
+    assert status() == 0
+    rel = 2 * (2.0 ** -19 + (2.0 ** -11 if kind == "f16" and T * G >= 256 else 2.0 ** -21) + 8 * 2.0 ** -24) + (n / 16 + 16) * 2.0 ** -23 + (n / 128 + 10) * 2.0 ** -24
+    for i in range(T):
+        sees = n - T + i + 1
+        p = np.exp(D ** -0.5 * (small[:sees] - small[:sees].max()))
+        want = p @ vb[:sees, 0] / p.sum()
+        bound = rel * np.abs(vb).max() + (np.abs(want) * 2.0 ** -11 if kind == "f16" else 0)
+        assert (np.abs(out[i].astype(np.float64) - want) <= bound).all(), (i, np.abs(out[i] - want).max(), rel)
